@@ -95,6 +95,16 @@ _SIGS = {
                                   _L, _L, _L, _P, _P, _P, _P, _P, _P, _I, _I,
                                   _I, _P, _L, _P, _P, _P, _P, _P, _P, _I, _I,
                                   _P, _L, _L, _F, _I, _I, _I, _I, _I, _I, _P],
+    "amass_pages_begin": [_P, _I, _P, _L, _P, _P, _P, _I, _P, _P, _P, _I, _P,
+                          _P, _P, _I, _I, _P],
+    "amass_pages_trim": [_P, _I, _I, _P, _L, _P, _P, _P, _I, _P, _I, _I, _P],
+    "amass_slot_map": [_P, _L, _P, _P, _I, _P, _P, _I, _I, _I, _P],
+    "amass_rotary_write": [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L,
+                           _P, _L, _L, _L, _P, _L, _L, _L, _P, _I, _I, _P,
+                           _I, _P, _F, _I, _I, _I, _I, _I, _I, _I, _P],
+    "amass_paged_chunk": [_P, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _I, _P,
+                          _L, _P, _P, _P, _P, _P, _I, _P, _P, _L, _L, _P, _F,
+                          _I, _I, _I, _I, _I, _I, _I, _I, _I, _P],
 }
 
 _lib = None

@@ -12,6 +12,9 @@ runs of the flat page list, one per warp of the grid, so ragged batches
 balance); the reference's chunk rule pps = max(ceil(cnt/split), PPS_MIN)
 (decode.py:154-160) is another cut of the same exact softmax re-association.
 ``pps_min`` here is the floor on pages per run.
+
+``paged_chunk_attention`` is the prefill side: dense attention of a step's new
+tokens (chunks, single tokens, mixtures) over the same cache.
 """
 from __future__ import annotations
 
@@ -108,3 +111,132 @@ def sparse_paged_decode_batched_cuda(q, kv_cache, block_table, seq_lens, st,
 
 
 sparse_paged_decode_batched = sparse_paged_decode_batched_cuda
+
+
+# --------------------------------------------------------------------------- #
+# attention of a chunk of new tokens (prefill, mixed batches)                 #
+# --------------------------------------------------------------------------- #
+DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def check_i32(device, **tensors) -> None:
+    """int32 index tensors on ``device`` with a contiguous last dimension."""
+    for name, t in tensors.items():
+        if t.dtype != torch.int32:
+            raise ValueError(f"{name} must be int32, got {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+        if t.dim() < 1 or (t.shape[-1] > 1 and t.stride(-1) != 1):
+            raise ValueError(f"{name} must have a contiguous last dimension")
+
+
+class ChunkBuffers:
+    """Scratch of ``paged_chunk_attention`` for one head geometry, allocated
+    once (outside any graph): the fp32 partials of the rows that two or more
+    SMs share.  Calls that may overlap on the GPU -- other streams, two
+    captured graphs replayed at once -- need a ``ChunkBuffers`` each.
+
+    ``fault`` (1,) int32 latches 1 when a kernel gave up a bounded wait;
+    ``check()`` reads it (synchronises) and raises."""
+
+    def __init__(self, device, *, n_kv: int, G: int, head_dim: int):
+        if head_dim not in (64, 128) or not 1 <= G <= 8 or n_kv < 1:
+            raise ValueError(f"no kernel for head_dim {head_dim}, G {G}, "
+                             f"n_kv {n_kv}")
+        dev = torch.device(device)
+        if dev.index is None and dev.type == "cuda":
+            dev = torch.device("cuda", torch.cuda.current_device())
+        self.device, self.n_kv, self.G, self.d = dev, n_kv, G, head_dim
+        n = torch.cuda.get_device_properties(dev).multi_processor_count
+        self.n_ctas = n
+        f32 = torch.float32
+        self.acc_part = torch.empty(n, 2, head_dim // 4, 256, 4, device=dev,
+                                    dtype=f32)
+        self.ml_part = torch.empty(n, 2, 256, 2, device=dev, dtype=f32)
+        self.meta = torch.zeros(n, 4, device=dev, dtype=torch.int32)
+        self.fault = torch.zeros(1, device=dev, dtype=torch.int32)
+
+    def check(self) -> None:
+        if int(self.fault.item()):
+            raise RuntimeError("paged_chunk_attention: a kernel gave up a "
+                               "bounded wait; its outputs are incomplete")
+
+
+def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
+                          out, buf, *, scale=None, window=None, lse=None,
+                          vsource=None) -> None:
+    """Dense attention of the step's new tokens over the paged cache, which
+    already holds their keys and values.
+
+    q, out (T, H, d) bf16 or fp16 (the cache's type), H = n_kv * G; rows
+    query_start_loc[r] .. query_start_loc[r + 1] - 1 are the last tokens of
+    request r's ``seq_lens[r]``; a row at position p sees the keys
+    max(0, p - window + 1) .. p (``window=None``: from 0).  Rows without a
+    key become 0, rows outside every request are left as they are.  ``lse``
+    (T, H) fp32, contiguous, receives the rows' natural log-sum-exp (-inf
+    without a key).  ``n_req = seq_lens.shape[0]``; ``buf`` is a
+    ``ChunkBuffers``.  Cache slots behind a request's last token may hold
+    anything; a NaN or infinity at a position a request has reached may
+    reach any row of its tile, as in a product over the whole tile.
+    One pass, no allocation, no synchronisation."""
+    k, v = split_kv(kv_cache)
+    if vsource is not None:
+        v = vsource.args()[0]
+    if v is None:
+        raise ValueError("no V source")
+    if q.dim() != 3 or out.shape != q.shape:
+        raise ValueError("q and out must be (T, H, d) of the same shape")
+    if q.dtype not in DTYPES or k.dtype != q.dtype or v.dtype != q.dtype or \
+            out.dtype != q.dtype:
+        raise ValueError("q, kv_cache and out must all be bf16 or all fp16")
+    NB, page, n_kv, d = k.shape
+    T, H, dq = q.shape
+    if v.shape != k.shape:
+        raise ValueError(f"V {tuple(v.shape)} does not match K "
+                         f"{tuple(k.shape)}")
+    if dq != d or H != n_kv * buf.G or d != buf.d or n_kv != buf.n_kv:
+        raise ValueError(f"q {tuple(q.shape)} and a cache of {n_kv} heads of "
+                         f"{d} do not fit buffers for {buf.n_kv} x {buf.G} "
+                         f"heads of {buf.d}")
+    dev = buf.device
+    for name, t in (("q", q), ("kv_cache", k), ("V", v), ("out", out)):
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, not on {dev}")
+        if t.stride(-1) != 1:
+            raise ValueError(f"{name} must have a contiguous head_dim")
+        if t.data_ptr() % 16 or any(
+                n > 1 and (st <= 0 or st % 8)
+                for n, st in zip(t.shape[:-1], t.stride()[:-1])):
+            raise ValueError(f"{name} must be 16-byte aligned, with strides "
+                             "that are positive multiples of 8 elements")
+    check_i32(dev, block_table=block_table, seq_lens=seq_lens,
+              query_start_loc=query_start_loc)
+    n_req = seq_lens.shape[0]
+    if block_table.dim() != 2 or block_table.shape[0] < n_req or \
+            query_start_loc.shape[0] < n_req + 1:
+        raise ValueError(f"block_table {tuple(block_table.shape)} and "
+                         f"query_start_loc {tuple(query_start_loc.shape)} do "
+                         f"not cover {n_req} requests")
+    if window is not None and window < 1:
+        raise ValueError(f"window must be at least 1, got {window}")
+    if lse is not None and (lse.dtype != torch.float32 or lse.device != dev or
+                            tuple(lse.shape) != (T, H) or
+                            not lse.is_contiguous()):
+        raise ValueError(f"lse must be a contiguous fp32 ({T}, {H}) tensor")
+    if scale is None:
+        scale = d ** -0.5
+    if not 0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive, got {scale}")
+    if block_table.shape[1] == 0 and n_req:
+        raise ValueError("block_table has no columns")
+    with torch.cuda.device(dev):
+        _lib.call("amass_paged_chunk", ptr(q), q.stride(0), q.stride(1),
+                  ptr(k), k.stride(0), k.stride(1), k.stride(2), ptr(v),
+                  v.stride(0), v.stride(1), v.stride(2), int(NB),
+                  ptr(block_table), block_table.stride(0), ptr(seq_lens),
+                  ptr(query_start_loc), ptr(buf.acc_part), ptr(buf.ml_part),
+                  ptr(buf.meta), buf.n_ctas, ptr(buf.fault), ptr(out),
+                  out.stride(0), out.stride(1), ptr(lse), float(scale),
+                  int(window or 0), int(T), int(n_req), int(n_kv), buf.G,
+                  int(d), int(page), max(1, int(block_table.shape[1])),
+                  DTYPES[q.dtype], _lib.stream_of(dev))

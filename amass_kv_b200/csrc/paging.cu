@@ -1,0 +1,349 @@
+// Page bookkeeping of a serving step on the GPU: block allocation, block
+// table, query start offsets, token positions and slot mapping from the new
+// token count of each request, and the way back (truncate / release).
+//
+//   begin   have_r = ceil(old_r / P), need_r = ceil((old_r + new_r)/P) - have_r,
+//           upto_r = need_0 + .. + need_r; request r is granted its pages iff
+//           need_r = 0 or upto_r <= free blocks (in order: the first that
+//           does not fit also refuses every later one that needs pages);
+//           its j-th new page takes free_stack[top - 1 - (upto_r - need_r + j)];
+//           token t of request r (start_r <= t < start_r + new_r) has position
+//           old_r + t - start_r and slot table[r][pos / P] * P + pos % P.
+//   trim    the pages behind the kept tokens return to the stack, last
+//           request and last page first, so a trim of everything a begin
+//           granted restores the stack to the same order.
+//
+// Bound: launch latency (a few KB to a few hundred KB move).  So each is one
+// launch: every CTA scans all requests for itself (two sums, in shared
+// memory), maps its share of the tokens, and takes the block of a new page
+// straight from the free stack -- it never waits for another CTA's table
+// write.  The token that opens a page writes that page's table entry.  What
+// other CTAs still read (lengths, the stack's top) is committed by the CTA
+// that draws the last ticket.
+#include "common.cuh"
+
+namespace amass {
+namespace {
+
+constexpr int kPgThreads = 512;
+constexpr int kPgMaxReq = 4096;          // 32 KB of request sums
+
+AMASS_DEV int pages_of(int64_t tokens, int page) {
+  return (int)((tokens + page - 1) / page);
+}
+
+// exclusive prefix of (a, b) over the CTA's threads; *ta, *tb the totals
+AMASS_DEV void scan2(int& a, int& b, int* ta, int* tb) {
+  __shared__ int wa[kPgThreads / 32], wb[kPgThreads / 32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int ia = a, ib = b;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int xa = __shfl_up_sync(~0u, ia, o), xb = __shfl_up_sync(~0u, ib, o);
+    if (lane >= o) { ia += xa; ib += xb; }
+  }
+  if (lane == 31) { wa[w] = ia; wb[w] = ib; }
+  __syncthreads();
+  int oa = 0, ob = 0, sa = 0, sb = 0;
+#pragma unroll
+  for (int i = 0; i < kPgThreads / 32; ++i) {
+    if (i < w) { oa += wa[i]; ob += wb[i]; }
+    sa += wa[i];
+    sb += wb[i];
+  }
+  __syncthreads();
+  a = oa + ia - a;
+  b = ob + ib - b;
+  *ta = sa;
+  *tb = sb;
+}
+
+// last i in [0, n) with start[i] <= t (start ascending, start[0] <= t)
+AMASS_DEV int find_start(const int* start, int n, int t) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int m = (lo + hi) >> 1;
+    if (start[m] <= t) lo = m; else hi = m;
+  }
+  return lo;
+}
+
+// true in every thread of the CTA that finishes last; its ticket is reset
+AMASS_DEV bool last_cta(int32_t* ticket) {
+  __shared__ int last;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    last = atomicAdd(ticket, 1) == (int)gridDim.x - 1;
+    if (last) *ticket = 0;
+    __threadfence();
+  }
+  __syncthreads();
+  return last != 0;
+}
+
+__global__ void __launch_bounds__(kPgThreads)
+pages_begin_kernel(const int32_t* __restrict__ new_tokens, int n_req,
+                   int32_t* block_table, int64_t bt_stride, int32_t* seq_lens,
+                   const int32_t* __restrict__ free_stack, int32_t* free_top,
+                   int num_blocks, int32_t* query_start_loc,
+                   int64_t* positions, int64_t* slot_mapping, int n_tokens,
+                   int32_t* status, int32_t* overflow, int32_t* ticket,
+                   int max_pages, int page) {
+  grid_dep_wait();
+  grid_dep_launch();
+  extern __shared__ int sm[];
+  int* start = sm;                       // n_req + 1: first token
+  int* pre = sm + n_req + 1;             // n_req: first new block, -1 refused
+  const int tid = threadIdx.x;
+  const int top = min(max(*free_top, 0), num_blocks);
+  const int per = (n_req + kPgThreads - 1) / kPgThreads;
+  const int r0 = min(n_req, tid * per), r1 = min(n_req, r0 + per);
+  int sn = 0, sd = 0;
+  for (int r = r0; r < r1; ++r) {
+    const int nw = max(new_tokens[r], 0), old = max(seq_lens[r], 0);
+    const int64_t want = (int64_t)old + nw;
+    sn += nw;
+    if (want <= (int64_t)max_pages * page)
+      sd += pages_of(want, page) - pages_of(old, page);
+  }
+  int total, need_all;
+  scan2(sn, sd, &total, &need_all);
+  int flags = 0, taken = 0;
+  for (int r = r0; r < r1; ++r) {
+    const int nw = max(new_tokens[r], 0), old = max(seq_lens[r], 0);
+    const int64_t want = (int64_t)old + nw;
+    start[r] = sn;
+    sn += nw;
+    int st = 0, need = 0;
+    if (want > (int64_t)max_pages * page) {
+      st = 2;
+    } else {
+      need = pages_of(want, page) - pages_of(old, page);
+      if (need > 0 && sd + need > top) st = 1;
+    }
+    pre[r] = st ? -1 : sd;
+    sd += need;
+    flags |= st;
+    if (st == 0) taken += need;
+    if (blockIdx.x == 0) {
+      status[r] = st;
+      query_start_loc[r] = start[r];
+    }
+  }
+  if (tid == 0) {
+    start[n_req] = total;
+    if (blockIdx.x == 0) query_start_loc[n_req] = total;
+  }
+  __syncthreads();
+
+  const int end = max(total, n_tokens);
+  for (int64_t t = (int64_t)blockIdx.x * kPgThreads + tid; t < end;
+       t += (int64_t)gridDim.x * kPgThreads) {
+    int64_t pos = 0, slot = -1;
+    if (t < total) {
+      const int r = find_start(start, n_req, (int)t);
+      const int old = max(seq_lens[r], 0);   // committed after the ticket
+      pos = old + (t - start[r]);
+      const int64_t pg = pos / page;
+      const int off = (int)(pos - pg * page);
+      if (pre[r] >= 0 && pg < max_pages) {
+        const int have = pages_of(old, page);
+        int32_t* e = block_table + (int64_t)r * bt_stride + pg;
+        int b = -1;
+        if (pg < have) {
+          b = *e;
+        } else {
+          const int k = top - 1 - (pre[r] + (int)pg - have);
+          if (k >= 0) {
+            b = free_stack[k];
+            if (off == 0) *e = b;
+          }
+        }
+        if (b >= 0) slot = (int64_t)b * page + off;
+      }
+    }
+    if (t < n_tokens) {
+      positions[t] = pos;
+      slot_mapping[t] = slot;
+    }
+  }
+  const int short_f = __syncthreads_or(flags & 1);
+  const int long_f = __syncthreads_or(flags & 2);
+  if (!last_cta(ticket)) return;
+  int zero = 0, used, z;
+  scan2(taken, zero, &used, &z);
+  for (int r = r0; r < r1; ++r) {
+    if (pre[r] < 0) continue;
+    const int nx = r + 1 < n_req ? start[r + 1] : total;
+    seq_lens[r] = max(seq_lens[r], 0) + (nx - start[r]);
+  }
+  if (tid == 0) {
+    *free_top = top - used;
+    const int f = (short_f ? 1 : 0) | (long_f ? 2 : 0) |
+                  (total > n_tokens ? 4 : 0);
+    if (f) *overflow |= f;
+  }
+}
+
+__global__ void __launch_bounds__(kPgThreads)
+pages_trim_kernel(const int32_t* __restrict__ drop, int whole, int n_req,
+                  int32_t* block_table, int64_t bt_stride, int32_t* seq_lens,
+                  int32_t* free_stack, int32_t* free_top, int num_blocks,
+                  int32_t* ticket, int max_pages, int page) {
+  grid_dep_wait();
+  grid_dep_launch();
+  extern __shared__ int sm[];
+  int* start = sm;                       // n_req + 1: first freed page, in
+                                         // order of descending request
+  int* left = sm + n_req + 1;            // n_req: tokens kept, by request
+  const int tid = threadIdx.x;
+  const int top = min(max(*free_top, 0), num_blocks);
+  const int per = (n_req + kPgThreads - 1) / kPgThreads;
+  const int i0 = min(n_req, tid * per), i1 = min(n_req, i0 + per);
+  const auto kept = [&](int r, int* have) {
+    const int old = (int)min((int64_t)max(seq_lens[r], 0),
+                             (int64_t)max_pages * page);
+    const int d = whole ? (drop[r] != 0 ? old : 0)
+                        : min(max(drop[r], 0), old);
+    *have = pages_of(old, page);
+    return old - d;
+  };
+  int s = 0, zero = 0, total, z;
+  for (int i = i0; i < i1; ++i) {
+    int have;
+    const int k = kept(n_req - 1 - i, &have);
+    s += have - pages_of(k, page);
+  }
+  scan2(s, zero, &total, &z);
+  for (int i = i0; i < i1; ++i) {
+    const int r = n_req - 1 - i;
+    int have;
+    left[r] = kept(r, &have);
+    start[i] = s;
+    s += have - pages_of(left[r], page);
+  }
+  if (tid == 0) start[n_req] = total;
+  __syncthreads();
+  for (int k = blockIdx.x * kPgThreads + tid; k < total;
+       k += gridDim.x * kPgThreads) {
+    const int i = find_start(start, n_req, k), r = n_req - 1 - i;
+    // the request's freed pages are keep .. keep + n - 1, last one first
+    const int n = start[i + 1] - start[i];
+    const int pg = pages_of(left[r], page) + n - 1 - (k - start[i]);
+    int32_t* e = block_table + (int64_t)r * bt_stride + pg;
+    if (top + k < num_blocks) free_stack[top + k] = *e;
+    *e = -1;
+  }
+  if (!last_cta(ticket)) return;
+  for (int i = i0; i < i1; ++i) seq_lens[n_req - 1 - i] = left[n_req - 1 - i];
+  if (tid == 0) *free_top = min(top + total, num_blocks);
+}
+
+__global__ void __launch_bounds__(kPgThreads)
+slot_map_kernel(const int32_t* __restrict__ block_table, int64_t bt_stride,
+                const int32_t* __restrict__ seq_lens,
+                const int32_t* __restrict__ query_start_loc, int n_req,
+                int64_t* __restrict__ positions,
+                int64_t* __restrict__ slot_mapping, int n_tokens,
+                int max_pages, int page) {
+  grid_dep_wait();
+  grid_dep_launch();
+  extern __shared__ int sm[];
+  for (int i = threadIdx.x; i <= n_req; i += kPgThreads)
+    sm[i] = query_start_loc[i];
+  __syncthreads();
+  for (int64_t t = (int64_t)blockIdx.x * kPgThreads + threadIdx.x;
+       t < n_tokens; t += (int64_t)gridDim.x * kPgThreads) {
+    int64_t pos = 0, slot = -1;
+    if (t >= sm[0] && t < sm[n_req]) {
+      const int r = find_start(sm, n_req, (int)t);
+      pos = (int64_t)seq_lens[r] - (sm[r + 1] - t);
+      const int64_t pg = pos / page;
+      if (pos >= 0 && pg < max_pages) {
+        const int b = block_table[(int64_t)r * bt_stride + pg];
+        if (b >= 0) slot = (int64_t)b * page + (pos - pg * page);
+      }
+    }
+    positions[t] = pos;
+    slot_mapping[t] = slot;
+  }
+}
+
+int grid_for(int64_t items, int per_cta) {
+  const int64_t n = (items + per_cta - 1) / per_cta;
+  return (int)(n < 1 ? 1 : n > num_sms() ? num_sms() : n);
+}
+
+}  // namespace
+}  // namespace amass
+
+extern "C" int amass_pages_begin(const int32_t* new_tokens, int n_req,
+                                 int32_t* block_table, int64_t bt_stride,
+                                 int32_t* seq_lens, const int32_t* free_stack,
+                                 int32_t* free_top, int num_blocks,
+                                 int32_t* query_start_loc, int64_t* positions,
+                                 int64_t* slot_mapping, int n_tokens,
+                                 int32_t* status, int32_t* overflow,
+                                 int32_t* ticket, int max_pages, int page,
+                                 void* stream) {
+  using namespace amass;
+  if (n_req < 0 || n_tokens < 0 || num_blocks < 0 || max_pages <= 0 ||
+      page <= 0 || bt_stride < 0 || !free_top || !query_start_loc ||
+      !overflow || !ticket || (num_blocks > 0 && !free_stack) ||
+      (n_tokens > 0 && (!positions || !slot_mapping)) ||
+      (n_req > 0 && (!new_tokens || !block_table || !seq_lens || !status)))
+    return AMASS_ERR_ARG;
+  if (n_req > kPgMaxReq) return AMASS_ERR_UNSUPPORTED;
+  return launch_pdl(pages_begin_kernel, dim3(grid_for(n_tokens, kPgThreads)),
+                    dim3(kPgThreads), (2 * n_req + 1) * sizeof(int),
+                    (cudaStream_t)stream, new_tokens, n_req, block_table,
+                    bt_stride, seq_lens, free_stack, free_top, num_blocks,
+                    query_start_loc, positions, slot_mapping, n_tokens,
+                    status, overflow, ticket, max_pages, page);
+}
+
+extern "C" int amass_pages_trim(const int32_t* drop, int whole, int n_req,
+                                int32_t* block_table, int64_t bt_stride,
+                                int32_t* seq_lens, int32_t* free_stack,
+                                int32_t* free_top, int num_blocks,
+                                int32_t* ticket, int max_pages, int page,
+                                void* stream) {
+  using namespace amass;
+  if (n_req < 0 || num_blocks < 0 || max_pages <= 0 || page <= 0 ||
+      bt_stride < 0 || !free_top || !ticket ||
+      (num_blocks > 0 && !free_stack) ||
+      (n_req > 0 && (!drop || !block_table || !seq_lens)))
+    return AMASS_ERR_ARG;
+  if (n_req > kPgMaxReq) return AMASS_ERR_UNSUPPORTED;
+  if (n_req == 0) return AMASS_OK;
+  // the number of pages that return is known on the device only: a whole
+  // release may free every row, a truncation mostly a page or two per request
+  const int64_t most = whole ? (int64_t)n_req * max_pages : 4ll * n_req;
+  return launch_pdl(pages_trim_kernel, dim3(grid_for(most, 4 * kPgThreads)),
+                    dim3(kPgThreads), (2 * n_req + 1) * sizeof(int),
+                    (cudaStream_t)stream, drop, whole, n_req, block_table,
+                    bt_stride, seq_lens, free_stack, free_top, num_blocks,
+                    ticket, max_pages, page);
+}
+
+extern "C" int amass_slot_map(const int32_t* block_table, int64_t bt_stride,
+                              const int32_t* seq_lens,
+                              const int32_t* query_start_loc, int n_req,
+                              int64_t* positions, int64_t* slot_mapping,
+                              int n_tokens, int max_pages, int page,
+                              void* stream) {
+  using namespace amass;
+  if (n_req < 0 || n_tokens < 0 || max_pages <= 0 || page <= 0 ||
+      bt_stride < 0 || !query_start_loc ||
+      (n_tokens > 0 && (!positions || !slot_mapping)) ||
+      (n_req > 0 && (!block_table || !seq_lens)))
+    return AMASS_ERR_ARG;
+  if (n_req > kPgMaxReq) return AMASS_ERR_UNSUPPORTED;
+  if (n_tokens == 0) return AMASS_OK;
+  return launch_pdl(slot_map_kernel, dim3(grid_for(n_tokens, kPgThreads)),
+                    dim3(kPgThreads), (n_req + 1) * sizeof(int),
+                    (cudaStream_t)stream, block_table, bt_stride, seq_lens,
+                    query_start_loc, n_req, positions, slot_mapping, n_tokens,
+                    max_pages, page);
+}

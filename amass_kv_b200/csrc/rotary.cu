@@ -1,0 +1,255 @@
+// Rotary positions of the new tokens' q and k, with k and v written straight
+// into the paged cache.
+//
+//   y0 = m (x0 cos a - x1 sin a),  y1 = m (x1 cos a + x0 sin a),
+//   a = position * f_i,  pair i = (x_i, x_{i + r/2}) or (x_{2i}, x_{2i+1}).
+//
+// Angle: fp32 cannot hold position * f (at position 1e5 the product has two
+// or three digits left of the turn), and a table of every position costs
+// memory and a second read.  f / (2 pi) is held as a 64-bit binary fraction
+// of a turn; the 64-bit product with the position wraps to exactly the
+// fraction that matters (error position * 2^-65 turns, any position), whose
+// upper 32 bits go to sincospi in fp32: about 2^-24 of the result.
+//
+// Bound: HBM.  q, k and v are read once and written once, (2H + 4 n_kv) d
+// 16-bit values a token; the angles are formed once a token for all heads.
+// An item is 16 elements of one head: two 16-byte loads (the two halves of 8
+// pairs, or 8 neighbouring pairs), eight rotations, two 16-byte stores.  v
+// and the part behind rotary_dim go through the same items with the
+// rotation left out.
+#include "common.cuh"
+
+namespace amass {
+namespace {
+
+constexpr int kRotThreads = 256;
+constexpr int kRotMaxDim = 256;
+constexpr int kRotMaxTok = 8;            // tokens of one CTA
+
+struct RotArgs {
+  const char *q, *k, *v;
+  char *qo, *kd, *vd;
+  int64_t q_st, q_sh, qo_st, qo_sh, k_st, k_sh, v_st, v_sh;
+  int64_t kd_sb, kd_st, kd_sh, vd_sb, vd_st, vd_sh;
+  const int64_t* slots;
+  const void* pos;
+  const uint64_t* freq;
+  int64_t n_slots;
+  float mscale;
+  int page, pos64, rot, T, H, n_kv, d, tok;
+};
+
+template <bool kF16>
+AMASS_DEV float2 unpack2(uint32_t w) {
+  if (kF16) return __half22float2(*reinterpret_cast<__half2*>(&w));
+  return make_float2(bf16_lo(w), bf16_hi(w));
+}
+template <bool kF16>
+AMASS_DEV uint32_t pack2(float a, float b) {
+  return kF16 ? pack_h2(a, b) : pack_bf2(a, b);
+}
+template <bool kF16>
+AMASS_DEV float load1(const char* p) {
+  const uint16_t x = *reinterpret_cast<const uint16_t*>(p);
+  return unpack2<kF16>(x).x;
+}
+template <bool kF16>
+AMASS_DEV void store1(char* p, float x) {
+  *reinterpret_cast<uint16_t*>(p) = (uint16_t)pack2<kF16>(x, 0.f);
+}
+
+// source and destination row of row `row` (q heads, k heads, v heads) of
+// token t; false when there is nothing to write
+AMASS_DEV bool rot_row(const RotArgs& a, int t, int row, int64_t slot,
+                       const char** src, char** dst) {
+  if (row < a.H) {
+    *src = a.q + 2 * (t * a.q_st + row * a.q_sh);
+    *dst = a.qo + 2 * (t * a.qo_st + row * a.qo_sh);
+    return true;
+  }
+  if (slot < 0 || slot >= a.n_slots) return false;
+  const int64_t b = slot / a.page, o = slot - b * a.page;
+  int h = row - a.H;
+  if (h < a.n_kv) {
+    *src = a.k + 2 * (t * a.k_st + h * a.k_sh);
+    *dst = a.kd + 2 * (b * a.kd_sb + o * a.kd_st + h * a.kd_sh);
+  } else {
+    h -= a.n_kv;
+    *src = a.v + 2 * (t * a.v_st + h * a.v_sh);
+    *dst = a.vd + 2 * (b * a.vd_sb + o * a.vd_st + h * a.vd_sh);
+  }
+  return true;
+}
+
+template <bool kF16, bool kHalf, bool kVec>
+__global__ void __launch_bounds__(kRotThreads)
+rotary_write_kernel(const __grid_constant__ RotArgs a) {
+  grid_dep_wait();
+  grid_dep_launch();
+  __shared__ __align__(16) float cs[kRotMaxTok][kRotMaxDim / 2];
+  __shared__ __align__(16) float sn[kRotMaxTok][kRotMaxDim / 2];
+  __shared__ int64_t slot_s[kRotMaxTok];
+  const int t0 = blockIdx.x * a.tok;
+  const int nt = min(a.tok, a.T - t0), half = a.rot >> 1;
+  for (int i = threadIdx.x; i < nt * half; i += kRotThreads) {
+    const int j = i / half, p = i - j * half;
+    const int64_t pos = a.pos64
+        ? static_cast<const int64_t*>(a.pos)[t0 + j]
+        : (int64_t)static_cast<const int32_t*>(a.pos)[t0 + j];
+    const uint64_t turn = (uint64_t)pos * a.freq[p];
+    // [-1/2, 1/2) turns: 2^-31 makes half turns of the upper 32 bits
+    const float x = (float)(int32_t)(turn >> 32) * 4.656612873077393e-10f;
+    float s, c;
+    sincospif(x, &s, &c);
+    cs[j][p] = c * a.mscale;
+    sn[j][p] = s * a.mscale;
+  }
+  if ((int)threadIdx.x < nt)
+    slot_s[threadIdx.x] = a.slots ? a.slots[t0 + threadIdx.x]
+                                  : (int64_t)(t0 + threadIdx.x);
+  __syncthreads();
+  const int rows = a.H + a.n_kv + (a.v ? a.n_kv : 0);
+  if (kVec) {
+    const int per = a.d >> 4, rper = a.rot >> 4;     // items: row, rotated
+    const int tok_items = rows * per;
+    for (int i = threadIdx.x; i < nt * tok_items; i += kRotThreads) {
+      const int j = i / tok_items, w = i - j * tok_items;
+      const int row = w / per, c = w - row * per;
+      const char* src;
+      char* dst;
+      if (!rot_row(a, t0 + j, row, slot_s[j], &src, &dst)) continue;
+      const bool turn = row < a.H + a.n_kv && c < rper;
+      // byte offsets of the item's two 16-byte words
+      const int o0 = kHalf && turn ? c * 16 : c * 32;
+      const int o1 = kHalf && turn ? o0 + a.rot : o0 + 16;
+      uint4 x = *reinterpret_cast<const uint4*>(src + o0);
+      uint4 y = *reinterpret_cast<const uint4*>(src + o1);
+      if (turn) {
+        const float4* cp = reinterpret_cast<const float4*>(&cs[j][c * 8]);
+        const float4* sp = reinterpret_cast<const float4*>(&sn[j][c * 8]);
+        const float4 c0 = cp[0], c1 = cp[1], s0 = sp[0], s1 = sp[1];
+        const float cv[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+        const float sv[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+        uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+        if (kHalf) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 u = unpack2<kF16>(xw[e]), z = unpack2<kF16>(yw[e]);
+            const float ca = cv[2 * e], cb = cv[2 * e + 1];
+            const float sa = sv[2 * e], sb = sv[2 * e + 1];
+            xw[e] = pack2<kF16>(u.x * ca - z.x * sa, u.y * cb - z.y * sb);
+            yw[e] = pack2<kF16>(z.x * ca + u.x * sa, z.y * cb + u.y * sb);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 u = unpack2<kF16>(xw[e]), z = unpack2<kF16>(yw[e]);
+            xw[e] = pack2<kF16>(u.x * cv[e] - u.y * sv[e],
+                                u.y * cv[e] + u.x * sv[e]);
+            yw[e] = pack2<kF16>(z.x * cv[e + 4] - z.y * sv[e + 4],
+                                z.y * cv[e + 4] + z.x * sv[e + 4]);
+          }
+        }
+        x = make_uint4(xw[0], xw[1], xw[2], xw[3]);
+        y = make_uint4(yw[0], yw[1], yw[2], yw[3]);
+      }
+      *reinterpret_cast<uint4*>(dst + o0) = x;
+      *reinterpret_cast<uint4*>(dst + o1) = y;
+    }
+  } else {
+    // pair by pair: any even rotary_dim, strides and alignment
+    const int per = a.d >> 1, tok_items = rows * per;
+    for (int i = threadIdx.x; i < nt * tok_items; i += kRotThreads) {
+      const int j = i / tok_items, w = i - j * tok_items;
+      const int row = w / per, p = w - row * per;
+      const char* src;
+      char* dst;
+      if (!rot_row(a, t0 + j, row, slot_s[j], &src, &dst)) continue;
+      const bool turn = row < a.H + a.n_kv && p < half;
+      const int e0 = kHalf && turn ? p : 2 * p;
+      const int e1 = kHalf && turn ? p + half : 2 * p + 1;
+      if (turn) {
+        const float x = load1<kF16>(src + 2 * e0);
+        const float y = load1<kF16>(src + 2 * e1);
+        const float c = cs[j][p], s = sn[j][p];
+        store1<kF16>(dst + 2 * e0, x * c - y * s);
+        store1<kF16>(dst + 2 * e1, y * c + x * s);
+      } else {
+        const uint16_t x = *reinterpret_cast<const uint16_t*>(src + 2 * e0);
+        const uint16_t y = *reinterpret_cast<const uint16_t*>(src + 2 * e1);
+        *reinterpret_cast<uint16_t*>(dst + 2 * e0) = x;
+        *reinterpret_cast<uint16_t*>(dst + 2 * e1) = y;
+      }
+    }
+  }
+}
+
+template <bool kF16, bool kHalf>
+int rot_launch(const RotArgs& a, bool vec, cudaStream_t st) {
+  const dim3 grid((unsigned)((a.T + a.tok - 1) / a.tok));
+  return vec ? launch_pdl(rotary_write_kernel<kF16, kHalf, true>, grid,
+                          dim3(kRotThreads), 0, st, a)
+             : launch_pdl(rotary_write_kernel<kF16, kHalf, false>, grid,
+                          dim3(kRotThreads), 0, st, a);
+}
+
+}  // namespace
+}  // namespace amass
+
+extern "C" int amass_rotary_write(
+    const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st,
+    int64_t qo_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
+    int64_t v_st, int64_t v_sh, void* k_dst, int64_t kd_sb, int64_t kd_st,
+    int64_t kd_sh, void* v_dst, int64_t vd_sb, int64_t vd_st, int64_t vd_sh,
+    const int64_t* slot_mapping, int num_blocks, int page,
+    const void* positions, int pos64, const uint64_t* freq, float mscale,
+    int layout, int rotary_dim, int n_tokens, int H, int n_kv, int head_dim,
+    int dtype, void* stream) {
+  using namespace amass;
+  if (n_tokens < 0 || H < 0 || n_kv < 0 || head_dim <= 0 || rotary_dim <= 0 ||
+      rotary_dim > head_dim || num_blocks < 0 || page <= 0 ||
+      (n_tokens > 0 && (!positions || !freq)) || (!q) != (!q_out) ||
+      (!k) != (!k_dst) || (!v) != (!v_dst) || (v && !k) ||
+      (layout != AMASS_ROTARY_HALF && layout != AMASS_ROTARY_INTERLEAVED) ||
+      (dtype != AMASS_BF16 && dtype != AMASS_FP16))
+    return AMASS_ERR_ARG;
+  if (head_dim > kRotMaxDim || (head_dim & 1) || (rotary_dim & 1))
+    return AMASS_ERR_UNSUPPORTED;
+  RotArgs a = {};
+  a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v;
+  a.qo = (char*)q_out; a.kd = (char*)k_dst; a.vd = (char*)v_dst;
+  a.q_st = q_st; a.q_sh = q_sh; a.qo_st = qo_st; a.qo_sh = qo_sh;
+  a.k_st = k_st; a.k_sh = k_sh; a.v_st = v_st; a.v_sh = v_sh;
+  a.kd_sb = kd_sb; a.kd_st = kd_st; a.kd_sh = kd_sh;
+  a.vd_sb = vd_sb; a.vd_st = vd_st; a.vd_sh = vd_sh;
+  a.slots = slot_mapping; a.pos = positions; a.freq = freq;
+  a.page = slot_mapping ? page : 1;
+  a.n_slots = slot_mapping ? (int64_t)num_blocks * page : n_tokens;
+  a.mscale = mscale; a.pos64 = pos64; a.rot = rotary_dim; a.T = n_tokens;
+  a.H = q ? H : 0; a.n_kv = k ? n_kv : 0; a.d = head_dim;
+  if (n_tokens == 0 || a.H + a.n_kv == 0) return AMASS_OK;
+  // 16-byte items need whole items in the rotated part and in the rest, and
+  // 16-byte aligned rows; anything else goes pair by pair
+  const int64_t strides = q_st | q_sh | qo_st | qo_sh | k_st | k_sh | v_st |
+                          v_sh | kd_sb | kd_st | kd_sh | vd_sb | vd_st | vd_sh;
+  const uintptr_t base = (uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k |
+                         (uintptr_t)k_dst | (uintptr_t)v | (uintptr_t)v_dst;
+  const bool vec = !(head_dim & 15) && !(rotary_dim & 15) && !(strides & 7) &&
+                   !(base & 15);
+  // enough items per CTA that its angles and its one barrier are small
+  // beside its copies, while every SM still has several CTAs
+  const int64_t items = (int64_t)(a.H + a.n_kv * (v ? 2 : 1)) *
+                        (vec ? head_dim >> 4 : head_dim >> 1);
+  int64_t tok = (6ll * kRotThreads + items - 1) / items;
+  const int64_t spread = ((int64_t)n_tokens + 4 * num_sms() - 1) /
+                         (4 * num_sms());
+  if (tok > spread) tok = spread;
+  a.tok = (int)(tok < 1 ? 1 : tok > kRotMaxTok ? kRotMaxTok : tok);
+  const cudaStream_t st = (cudaStream_t)stream;
+  const bool half = layout == AMASS_ROTARY_HALF;
+  if (dtype == AMASS_FP16)
+    return half ? rot_launch<true, true>(a, vec, st)
+                : rot_launch<true, false>(a, vec, st);
+  return half ? rot_launch<false, true>(a, vec, st)
+              : rot_launch<false, false>(a, vec, st);
+}

@@ -537,6 +537,120 @@ int amass_tier_decode_install(
     float scale, int n_req, int n_kv, int G, int head_dim, int page,
     int max_pages, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Prefill side: page bookkeeping, rotary positions with the cache write,
+ * attention of a chunk of new tokens.  No counterpart in the reference, whose
+ * engine does these.
+ * ------------------------------------------------------------------------ */
+
+/* pages_begin -- one step's block allocation and token maps.  Request r in
+ * [0, n_req) grows by max(new_tokens[r], 0) tokens; with old = seq_lens[r] it
+ * needs ceil((old + new) / page) - ceil(old / page) blocks.  Requests are
+ * served in order: r is granted when it needs none or when the blocks needed
+ * up to and including r do not exceed free_top[0].  The k-th block granted is
+ * free_stack[top - 1 - k]; it is entered in block_table, free_top and
+ * seq_lens follow.  status[r]: 0 granted, 1 too few free blocks, 2 more than
+ * max_pages pages (then it counts as needing none); a refused request keeps
+ * its pages and length.  query_start_loc (n_req + 1): prefix sums of the new
+ * tokens, refused requests included.  For token t < n_tokens of request r:
+ * positions[t] = old + (t - query_start_loc[r]), slot_mapping[t] = block *
+ * page + offset, or -1 when refused; behind the last token 0 and -1.
+ * overflow[0] |= 1 (a status 1), 2 (a status 2), 4 (more than n_tokens new
+ * tokens: the maps end there).  ticket: int32, 0 before the first call, left
+ * 0.  One launch.  n_req <= 4096; the new tokens' sum fits int32. */
+int amass_pages_begin(const int32_t* new_tokens, int n_req,
+                      int32_t* block_table, int64_t bt_stride,
+                      int32_t* seq_lens, const int32_t* free_stack,
+                      int32_t* free_top, int num_blocks,
+                      int32_t* query_start_loc, int64_t* positions,
+                      int64_t* slot_mapping, int n_tokens, int32_t* status,
+                      int32_t* overflow, int32_t* ticket, int max_pages,
+                      int page, void* stream);
+
+/* pages_trim -- request r loses its last min(max(drop[r], 0), seq_lens[r])
+ * tokens (whole = 0), or all of them where drop[r] != 0 (whole = 1).  Pages
+ * left without a token return to free_stack and their table entries become
+ * -1.  They are pushed last request and last page first, so a trim of what a
+ * pages_begin granted restores the stack's order.  One launch.
+ * n_req <= 4096. */
+int amass_pages_trim(const int32_t* drop, int whole, int n_req,
+                     int32_t* block_table, int64_t bt_stride,
+                     int32_t* seq_lens, int32_t* free_stack,
+                     int32_t* free_top, int num_blocks, int32_t* ticket,
+                     int max_pages, int page, void* stream);
+
+/* slot_map -- positions and slots of a step whose block table and lengths
+ * exist: token t of request r (query_start_loc[r] <= t <
+ * query_start_loc[r + 1]) has position seq_lens[r] - (query_start_loc[r + 1]
+ * - t) and slot block_table[r][position / page] * page + position % page;
+ * slot -1 for a negative position, one beyond max_pages or a block < 0;
+ * tokens outside every request get 0 and -1.  n_req <= 4096. */
+int amass_slot_map(const int32_t* block_table, int64_t bt_stride,
+                   const int32_t* seq_lens, const int32_t* query_start_loc,
+                   int n_req, int64_t* positions, int64_t* slot_mapping,
+                   int n_tokens, int max_pages, int page, void* stream);
+
+/* element types of the prefill-side entry points */
+enum { AMASS_BF16 = 0, AMASS_FP16 = 1 };
+/* pairing of a head's rotated elements: (i, i + rotary_dim / 2) or
+ * (2i, 2i + 1) */
+enum { AMASS_ROTARY_HALF = 0, AMASS_ROTARY_INTERLEAVED = 1 };
+
+/* rotary_write -- turns pair i of every head of q and k by the angle
+ * positions[t] * f_i and scales it by mscale; elements from rotary_dim on
+ * pass unchanged.  q (n_tokens, H, d) goes to q_out (which may be q); k and
+ * v (n_tokens, n_kv, d) go to k_dst and v_dst at block slot / page, row
+ * slot % page (element strides *_sb, *_st, *_sh), slot = slot_mapping[t];
+ * slots outside [0, num_blocks * page) are skipped.  slot_mapping null:
+ * slot = t (page 1: a token-major destination, which may be k itself).
+ * Either of q and k may be null, v and v_dst may be null.  freq[i] =
+ * f_i / (2 pi) as a 64-bit binary fraction of a turn (rotary_dim / 2 values;
+ * the product with the position wraps, so no position is too far).
+ * positions are int64 (pos64 = 1) or int32.  Products in fp32, one rounding.
+ * head_dim <= 256 and rotary_dim <= head_dim, both even.  Two tokens must not
+ * share a slot. */
+int amass_rotary_write(const void* q, int64_t q_st, int64_t q_sh, void* q_out,
+                       int64_t qo_st, int64_t qo_sh, const void* k,
+                       int64_t k_st, int64_t k_sh, const void* v,
+                       int64_t v_st, int64_t v_sh, void* k_dst, int64_t kd_sb,
+                       int64_t kd_st, int64_t kd_sh, void* v_dst,
+                       int64_t vd_sb, int64_t vd_st, int64_t vd_sh,
+                       const int64_t* slot_mapping, int num_blocks, int page,
+                       const void* positions, int pos64, const uint64_t* freq,
+                       float mscale, int layout, int rotary_dim, int n_tokens,
+                       int H, int n_kv, int head_dim, int dtype,
+                       void* stream);
+
+/* paged_chunk -- dense attention of a step's new tokens over the paged cache
+ * (which already holds their keys and values): prefill chunks, single tokens
+ * and mixtures.  q (n_tokens, n_kv * G, d); request r owns the rows
+ * [query_start_loc[r], query_start_loc[r + 1]), the last of its seq_lens[r]
+ * tokens; row i has position seq_lens[r] - q_len + i and sees the keys
+ * max(0, position - window + 1) .. position (window 0: from 0).  K and V are
+ * addressed as in amass_sparse_decode.  out (n_tokens, n_kv * G, d): rows
+ * without a key become 0, rows outside every request are left as they are;
+ * lse (n_tokens, n_kv * G) fp32 or null: natural log of the row's sum of
+ * exp(scale q.k), -inf without a key.  Cache slots behind a request's last
+ * token may hold anything; block ids outside [0, num_blocks) read as zeros;
+ * seq_lens is cut at max_pages * page.  Scratch for n_ctas CTAs (one per SM):
+ * acc_part n_ctas * 2 * 256 * d fp32 and ml_part n_ctas * 2 * 256 * 2 fp32
+ * (both 16-byte aligned), meta n_ctas * 4 int32; none needs to be set.  Calls
+ * that overlap on the GPU need scratch of their own.  fault[0] becomes 1 when
+ * a CTA gave up a bounded wait (its rows are then incomplete).
+ * head_dim in {64, 128}, G <= 8, page = 16, n_req <= 4096, scale > 0; bases
+ * 16-byte aligned, strides positive multiples of 8 elements.  Two launches;
+ * the first call on a device sets a kernel attribute. */
+int amass_paged_chunk(
+    const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+    int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb,
+    int64_t v_st, int64_t v_sh, int num_blocks, const int32_t* block_table,
+    int64_t bt_stride, const int32_t* seq_lens,
+    const int32_t* query_start_loc, float* acc_part, float* ml_part,
+    int32_t* meta, int n_ctas, int32_t* fault, void* out, int64_t o_stride_t,
+    int64_t o_stride_h, float* lse, float scale, int window, int n_tokens,
+    int n_req, int n_kv, int G, int head_dim, int page, int max_pages,
+    int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,176 @@
+"""Calls the prefill-side entry points refuse, checked before any launch (no
+GPU needed)."""
+import ctypes
+
+import pytest
+import torch
+
+from amass_kv_b200 import _lib
+from amass_kv_b200.attention import paged_chunk_attention
+from amass_kv_b200.paging import BlockPool, build_slot_map
+from amass_kv_b200.rotary import Rotary, rotary_embed, rotary_write_kv
+
+CPU = torch.device("cpu")
+
+
+class Buf:
+    """What paged_chunk_attention reads of its buffers."""
+    device, n_kv, G, d = CPU, 2, 4, 64
+
+
+def chunk_args(**kw):
+    a = dict(q=torch.zeros(5, 8, 64, dtype=torch.bfloat16),
+             kv_cache=torch.zeros(4, 2, 16, 2, 64, dtype=torch.bfloat16),
+             block_table=torch.zeros(2, 3, dtype=torch.int32),
+             seq_lens=torch.ones(2, dtype=torch.int32),
+             query_start_loc=torch.zeros(3, dtype=torch.int32),
+             out=torch.zeros(5, 8, 64, dtype=torch.bfloat16), buf=Buf())
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(q=torch.zeros(5, 8, 64)), "bf16 or all fp16"),
+    (dict(out=torch.zeros(5, 8, 64, dtype=torch.float16)), "bf16 or all"),
+    (dict(out=torch.zeros(4, 8, 64, dtype=torch.bfloat16)), "same shape"),
+    (dict(kv_cache=torch.zeros(4, 1, 16, 2, 64, dtype=torch.bfloat16)),
+     "no V source"),
+    (dict(kv_cache=torch.zeros(4, 2, 16, 4, 64, dtype=torch.bfloat16)),
+     "do not fit"),
+    (dict(seq_lens=torch.ones(2, dtype=torch.int64)), "int32"),
+    (dict(seq_lens=torch.ones(3, dtype=torch.int32)), "cover"),
+    (dict(query_start_loc=torch.zeros(2, dtype=torch.int32)), "cover"),
+    (dict(block_table=torch.zeros(3, 2, dtype=torch.int32).t()),
+     "contiguous last"),
+    (dict(block_table=torch.zeros(2, 0, dtype=torch.int32)), "no columns"),
+    (dict(window=0), "window"), (dict(scale=0.0), "scale"),
+    (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
+    (dict(lse=torch.zeros(5, 4)), "lse"),
+    (dict(q=torch.zeros(5, 8, 65, dtype=torch.bfloat16)[..., 1:]),
+     "16-byte"),
+    (dict(q=torch.zeros(5, 8, 128, dtype=torch.bfloat16)[..., ::2]),
+     "contiguous head_dim"),
+])
+def test_chunk_refuses(kw, match):
+    with pytest.raises(ValueError, match=match):
+        paged_chunk_attention(**chunk_args(**kw))
+
+
+def test_chunk_c_entry_refuses():
+    lib = _lib.load()
+    one = ctypes.c_void_p(64)
+
+    def call(**kw):
+        a = dict(q=one, k=one, page=16, d=128, G=4, T=4, R=1, scale=0.1,
+                 window=0, dtype=0, ksh=128, nb=3, mp=4, fault=one)
+        a.update(kw)
+        return lib.amass_paged_chunk(
+            a["q"], 512, 128, a["k"], 4096, 256, a["ksh"], one, 4096, 256,
+            128, a["nb"], one, 4, one, one, one, one, one, 8, a["fault"], one,
+            512, 128, None, ctypes.c_float(a["scale"]), a["window"], a["T"],
+            a["R"], 2, a["G"], a["d"], a["page"], a["mp"], a["dtype"], None)
+    assert call(T=0) == 0 and call(R=0) == 0
+    for kw in (dict(q=None), dict(fault=None), dict(T=-1), dict(scale=0.0),
+               dict(scale=float("nan")), dict(window=-1), dict(dtype=2),
+               dict(ksh=100), dict(ksh=-128), dict(nb=0), dict(mp=0),
+               dict(k=ctypes.c_void_p(24))):
+        assert call(**kw) == 1, kw
+    for kw in (dict(d=96), dict(G=9), dict(page=32), dict(R=4097)):
+        assert call(**kw) == 2, kw
+
+
+def test_pool_refuses():
+    for kw in (dict(num_blocks=0), dict(max_reqs=0), dict(max_reqs=4097),
+               dict(max_pages=0), dict(max_tokens=0), dict(page=0),
+               dict(max_pages=1 << 28)):
+        a = dict(num_blocks=4, max_reqs=2, max_pages=3, max_tokens=9)
+        a.update(kw)
+        with pytest.raises(ValueError):
+            BlockPool(CPU, **a)
+    p = BlockPool(CPU, num_blocks=4, max_reqs=2, max_pages=3, max_tokens=9)
+    one = torch.ones(2, dtype=torch.int32)
+    for bad in (torch.ones(2), torch.ones(3, dtype=torch.int32),
+                torch.ones(2, 1, dtype=torch.int32),
+                torch.ones(4, dtype=torch.int32)[::2]):
+        for f in (p.begin_step, p.truncate, p.release):
+            with pytest.raises(ValueError):
+                f(bad)
+    for n in (-1, 10):
+        with pytest.raises(ValueError):
+            p.begin_step(one, n_tokens=n)
+    p.check()
+    p.overflow.fill_(6)
+    with pytest.raises(RuntimeError, match="outgrew.*n_tokens"):
+        p.check()
+    lib = _lib.load()
+    assert lib.amass_pages_trim(None, 0, 0, None, 0, None, ctypes.c_void_p(8),
+                                ctypes.c_void_p(8), 4, ctypes.c_void_p(8), 3,
+                                16, None) == 0
+    assert lib.amass_pages_trim(None, 0, 1, None, 0, None, ctypes.c_void_p(8),
+                                ctypes.c_void_p(8), 4, ctypes.c_void_p(8), 3,
+                                16, None) == 1
+
+
+def test_slot_map_refuses():
+    i32, i64 = torch.int32, torch.int64
+    a = dict(block_table=torch.zeros(2, 3, dtype=i32),
+             seq_lens=torch.ones(2, dtype=i32),
+             query_start_loc=torch.zeros(3, dtype=i32),
+             positions=torch.zeros(9, dtype=i64),
+             slot_mapping=torch.zeros(9, dtype=i64))
+    for kw in (dict(positions=torch.zeros(9, dtype=i32)),
+               dict(positions=torch.zeros(8, dtype=i64)),
+               dict(slot_mapping=torch.zeros(18, dtype=i64)[::2]),
+               dict(seq_lens=torch.ones(3, dtype=i32)), dict(page=0),
+               dict(seq_lens=torch.ones(2)), dict(n_tokens=10)):
+        with pytest.raises(ValueError):
+            build_slot_map(**{**a, **kw})
+
+
+@pytest.mark.parametrize("kw", [
+    dict(rotary_dim=3), dict(rotary_dim=0), dict(rotary_dim=258),
+    dict(layout="pairs"), dict(base=1.0), dict(scaling=dict(factor=2.0)),
+    dict(scaling=dict(type="linear")),
+    dict(scaling=dict(type="linear", factor=0.5)),
+    dict(scaling=dict(type="linear", factor=2.0, beta_fast=3)),
+    dict(scaling=dict(type="yarn", factor=2.0)),
+    dict(scaling=dict(type="yarn", factor=2.0, original_max_position=100,
+                      beta_fast=1, beta_slow=2)),
+    dict(scaling=dict(type="llama3", factor=2.0, low_freq_factor=4,
+                      high_freq_factor=1, original_max_position=100)),
+])
+def test_rotary_refuses(kw):
+    with pytest.raises(ValueError):
+        Rotary(CPU, **{**dict(rotary_dim=64), **kw})
+
+
+def test_rotary_calls_refuse():
+    rot = Rotary(CPU, rotary_dim=64)
+    bf = torch.bfloat16
+    a = dict(q=torch.zeros(5, 8, 64, dtype=bf),
+             k=torch.zeros(5, 2, 64, dtype=bf),
+             v=torch.zeros(5, 2, 64, dtype=bf), positions=torch.arange(5),
+             kv_cache=torch.zeros(4, 2, 16, 2, 64, dtype=bf),
+             slot_mapping=torch.arange(5))
+    for kw in (dict(q=torch.zeros(5, 8, 64)), dict(k=None), dict(v=None),
+               dict(q=None, q_out=a["q"]),
+               dict(positions=torch.arange(4)),
+               dict(positions=torch.arange(5.0)),
+               dict(slot_mapping=torch.arange(4)),
+               dict(slot_mapping=torch.arange(5, dtype=torch.int32)),
+               dict(slot_mapping=torch.arange(10)[::2]),
+               dict(kv_cache=torch.zeros(4, 2, 16, 2, 128, dtype=bf)),
+               dict(kv_cache=torch.zeros(4, 1, 16, 2, 64, dtype=bf)),
+               dict(q_out=torch.zeros(5, 4, 64, dtype=bf)),
+               dict(q_out=torch.zeros(4, 8, 64, dtype=bf)),
+               dict(k=torch.zeros(5, 4, 64, dtype=bf)),
+               dict(q=torch.zeros(5, 8, 32, dtype=bf)), dict(n_tokens=6),
+               dict(n_tokens=-1)):
+        with pytest.raises(ValueError):
+            rotary_write_kv(rot, **{**a, **kw})
+    with pytest.raises(ValueError):
+        rotary_embed(rot, None, None, torch.arange(5))
+    with pytest.raises(ValueError):
+        rotary_embed(rot, a["q"], None, torch.arange(5), k_out=a["k"])
+    with pytest.raises(ValueError):
+        rotary_embed(rot, a["q"][..., :32], None, torch.arange(5))
