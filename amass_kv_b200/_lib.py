@@ -8,7 +8,10 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
+
+import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libamass_b200.so")
@@ -27,6 +30,12 @@ class DmaRun(ctypes.Structure):
                 ("dpitch", ctypes.c_int64), ("spitch", ctypes.c_int64),
                 ("width", ctypes.c_int64), ("height", ctypes.c_int64)]
 
+
+# argument blocks of the prefill side (include/amass_b200.h), packed in one go:
+# converting three dozen ctypes arguments costs more than the launch
+PAGE_POOL = struct.Struct("10Pq6i")
+ROTARY = struct.Struct("9P14qf11i")
+CHUNK = struct.Struct("12P11qf11i")
 
 # name -> argtypes (restype is int status for every compute entry point)
 _SIGS = {
@@ -95,16 +104,11 @@ _SIGS = {
                                   _L, _L, _L, _P, _P, _P, _P, _P, _P, _I, _I,
                                   _I, _P, _L, _P, _P, _P, _P, _P, _P, _I, _I,
                                   _P, _L, _L, _F, _I, _I, _I, _I, _I, _I, _P],
-    "amass_pages_begin": [_P, _I, _P, _L, _P, _P, _P, _I, _P, _P, _P, _I, _P,
-                          _P, _P, _I, _I, _P],
-    "amass_pages_trim": [_P, _I, _I, _P, _L, _P, _P, _P, _I, _P, _I, _I, _P],
+    "amass_pages_begin": [_P, _P, _I, _I, _P],
+    "amass_pages_trim": [_P, _P, _I, _I, _P],
     "amass_slot_map": [_P, _L, _P, _P, _I, _P, _P, _I, _I, _I, _P],
-    "amass_rotary_write": [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L,
-                           _P, _L, _L, _L, _P, _L, _L, _L, _P, _I, _I, _P,
-                           _I, _P, _F, _I, _I, _I, _I, _I, _I, _I, _P],
-    "amass_paged_chunk": [_P, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _I, _P,
-                          _L, _P, _P, _P, _P, _P, _I, _P, _P, _L, _L, _P, _F,
-                          _I, _I, _I, _I, _I, _I, _I, _I, _I, _P],
+    "amass_rotary_write": [_P, _P],
+    "amass_paged_chunk": [_P, _P],
 }
 
 _lib = None
@@ -152,6 +156,27 @@ def call(name: str, *args) -> None:
     rc = getattr(lib, name)(*args)
     if rc != 0:
         raise RuntimeError(f"{name} failed: {status_string(rc)} (status {rc})")
+
+
+def launch(index: int, name: str, *args) -> None:
+    """``call`` with GPU ``index`` current and its current stream as the last
+    argument."""
+    fn = getattr(_lib or load(), name)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        raise RuntimeError(f"{name} failed: {status_string(rc)} (status {rc})")
+
+
+def device_of(device) -> torch.device:
+    """``device`` with its index (the current GPU's for plain "cuda")."""
+    dev = torch.device(device)
+    if dev.type == "cuda" and dev.index is None:
+        dev = torch.device("cuda", torch.cuda.current_device())
+    return dev
 
 
 def ptr(t) -> int:

@@ -119,15 +119,29 @@ sparse_paged_decode_batched = sparse_paged_decode_batched_cuda
 DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
 
-def check_i32(device, **tensors) -> None:
-    """int32 index tensors on ``device`` with a contiguous last dimension."""
-    for name, t in tensors.items():
-        if t.dtype != torch.int32:
-            raise ValueError(f"{name} must be int32, got {t.dtype}")
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
-        if t.dim() < 1 or (t.shape[-1] > 1 and t.stride(-1) != 1):
-            raise ValueError(f"{name} must have a contiguous last dimension")
+def check_i32(index: int, name: str, t, dim: int) -> None:
+    """An int32 tensor of ``dim`` dimensions on GPU ``index`` (-1: the host)
+    with a contiguous last one."""
+    if t.dtype != torch.int32 or t.get_device() != index or t.dim() != dim \
+            or (t.stride()[-1] != 1 and t.shape[-1] > 1):
+        raise ValueError(f"{name} must be int32, of {dim} dimensions, on GPU "
+                         f"{index} and contiguous in the last dimension; got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def cache_layout(kv_cache):
+    """(num_blocks, page, n_kv, d, (block, token, head stride), K address, V
+    address or 0) of the cache layouts of ``split_kv``, without making views;
+    ValueError when it is none of them."""
+    shape, s = kv_cache.shape, kv_cache.stride()
+    if len(shape) != 5 or (s[4] != 1 and shape[4] > 1):
+        raise ValueError("kv_cache must be (blocks, 1 or 2, page, n_kv, d) or "
+                         "(2, blocks, page, n_kv, d) with a contiguous "
+                         f"head_dim, got {tuple(shape)}")
+    p = kv_cache.data_ptr()
+    b, half = (1, 0) if shape[0] == 2 else (0, 1)
+    v = 0 if shape[half] == 1 else p + s[half] * kv_cache.element_size()
+    return (shape[b], shape[2], shape[3], shape[4], (s[b], s[2], s[3]), p, v)
 
 
 class ChunkBuffers:
@@ -143,10 +157,9 @@ class ChunkBuffers:
         if head_dim not in (64, 128) or not 1 <= G <= 8 or n_kv < 1:
             raise ValueError(f"no kernel for head_dim {head_dim}, G {G}, "
                              f"n_kv {n_kv}")
-        dev = torch.device(device)
-        if dev.index is None and dev.type == "cuda":
-            dev = torch.device("cuda", torch.cuda.current_device())
+        dev = _lib.device_of(device)
         self.device, self.n_kv, self.G, self.d = dev, n_kv, G, head_dim
+        self.index = dev.index
         n = torch.cuda.get_device_properties(dev).multi_processor_count
         self.n_ctas = n
         f32 = torch.float32
@@ -155,6 +168,8 @@ class ChunkBuffers:
         self.ml_part = torch.empty(n, 2, 256, 2, device=dev, dtype=f32)
         self.meta = torch.zeros(n, 4, device=dev, dtype=torch.int32)
         self.fault = torch.zeros(1, device=dev, dtype=torch.int32)
+        self.scratch = (ptr(self.acc_part), ptr(self.ml_part),
+                        ptr(self.meta), ptr(self.fault))
 
     def check(self) -> None:
         if int(self.fault.item()):
@@ -179,47 +194,56 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
     anything; a NaN or infinity at a position a request has reached may
     reach any row of its tile, as in a product over the whole tile.
     One pass, no allocation, no synchronisation."""
-    k, v = split_kv(kv_cache)
+    nb, page, n_kv, d, (k_sb, k_st, k_sh), k, v = cache_layout(kv_cache)
+    v_sb, v_st, v_sh = k_sb, k_st, k_sh
+    dtype, dev = q.dtype, buf.index
     if vsource is not None:
-        v = vsource.args()[0]
-    if v is None:
+        vt = vsource.args()[0]
+        if tuple(vt.shape) != (nb, page, n_kv, d) or vt.dtype != dtype or \
+                vt.get_device() != dev or vt.stride(3) != 1:
+            raise ValueError(f"the V source's {tuple(vt.shape)} {vt.dtype} "
+                             "does not match K")
+        v, (v_sb, v_st, v_sh, _) = vt.data_ptr(), vt.stride()
+    if not v:
         raise ValueError("no V source")
-    if q.dim() != 3 or out.shape != q.shape:
+    shape = q.shape
+    if len(shape) != 3 or out.shape != shape:
         raise ValueError("q and out must be (T, H, d) of the same shape")
-    if q.dtype not in DTYPES or k.dtype != q.dtype or v.dtype != q.dtype or \
-            out.dtype != q.dtype:
+    if dtype not in DTYPES or kv_cache.dtype != dtype or out.dtype != dtype:
         raise ValueError("q, kv_cache and out must all be bf16 or all fp16")
-    NB, page, n_kv, d = k.shape
-    T, H, dq = q.shape
-    if v.shape != k.shape:
-        raise ValueError(f"V {tuple(v.shape)} does not match K "
-                         f"{tuple(k.shape)}")
+    T, H, dq = shape
     if dq != d or H != n_kv * buf.G or d != buf.d or n_kv != buf.n_kv:
-        raise ValueError(f"q {tuple(q.shape)} and a cache of {n_kv} heads of "
+        raise ValueError(f"q {tuple(shape)} and a cache of {n_kv} heads of "
                          f"{d} do not fit buffers for {buf.n_kv} x {buf.G} "
                          f"heads of {buf.d}")
-    dev = buf.device
-    for name, t in (("q", q), ("kv_cache", k), ("V", v), ("out", out)):
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, not on {dev}")
-        if t.stride(-1) != 1:
-            raise ValueError(f"{name} must have a contiguous head_dim")
-        if t.data_ptr() % 16 or any(
-                n > 1 and (st <= 0 or st % 8)
-                for n, st in zip(t.shape[:-1], t.stride()[:-1])):
-            raise ValueError(f"{name} must be 16-byte aligned, with strides "
-                             "that are positive multiples of 8 elements")
-    check_i32(dev, block_table=block_table, seq_lens=seq_lens,
-              query_start_loc=query_start_loc)
+    q_st, q_sh, q_sd = q.stride()
+    o_st, o_sh, o_sd = out.stride()
+    if q_sd != 1 or o_sd != 1:
+        raise ValueError("q and out must have a contiguous head_dim")
+    if q.get_device() != dev or out.get_device() != dev or \
+            kv_cache.get_device() != dev:
+        raise ValueError(f"q, kv_cache and out must be on GPU {dev}")
+    qp, op = q.data_ptr(), out.data_ptr()
+    if (qp | op | k | v) % 16 or \
+            (T > 1 and (q_st <= 0 or q_st % 8 or o_st <= 0 or o_st % 8)) or \
+            (H > 1 and (q_sh <= 0 or q_sh % 8 or o_sh <= 0 or o_sh % 8)) or \
+            (k_sb | k_st | k_sh | v_sb | v_st | v_sh) % 8 or \
+            min(k_sb, k_st, k_sh, v_sb, v_st, v_sh) <= 0:
+        raise ValueError("q, kv_cache and out must be 16-byte aligned, with "
+                         "strides that are positive multiples of 8 elements")
+    check_i32(dev, "block_table", block_table, 2)
+    check_i32(dev, "seq_lens", seq_lens, 1)
+    check_i32(dev, "query_start_loc", query_start_loc, 1)
     n_req = seq_lens.shape[0]
-    if block_table.dim() != 2 or block_table.shape[0] < n_req or \
-            query_start_loc.shape[0] < n_req + 1:
-        raise ValueError(f"block_table {tuple(block_table.shape)} and "
+    rows, max_pages = block_table.shape
+    if rows < n_req or query_start_loc.shape[0] < n_req + 1 or max_pages < 1:
+        raise ValueError(f"block_table {(rows, max_pages)} and "
                          f"query_start_loc {tuple(query_start_loc.shape)} do "
                          f"not cover {n_req} requests")
     if window is not None and window < 1:
         raise ValueError(f"window must be at least 1, got {window}")
-    if lse is not None and (lse.dtype != torch.float32 or lse.device != dev or
+    if lse is not None and (lse.dtype != torch.float32 or
+                            lse.get_device() != dev or
                             tuple(lse.shape) != (T, H) or
                             not lse.is_contiguous()):
         raise ValueError(f"lse must be a contiguous fp32 ({T}, {H}) tensor")
@@ -227,16 +251,12 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
         scale = d ** -0.5
     if not 0 < scale < float("inf"):
         raise ValueError(f"scale must be positive, got {scale}")
-    if block_table.shape[1] == 0 and n_req:
-        raise ValueError("block_table has no columns")
-    with torch.cuda.device(dev):
-        _lib.call("amass_paged_chunk", ptr(q), q.stride(0), q.stride(1),
-                  ptr(k), k.stride(0), k.stride(1), k.stride(2), ptr(v),
-                  v.stride(0), v.stride(1), v.stride(2), int(NB),
-                  ptr(block_table), block_table.stride(0), ptr(seq_lens),
-                  ptr(query_start_loc), ptr(buf.acc_part), ptr(buf.ml_part),
-                  ptr(buf.meta), buf.n_ctas, ptr(buf.fault), ptr(out),
-                  out.stride(0), out.stride(1), ptr(lse), float(scale),
-                  int(window or 0), int(T), int(n_req), int(n_kv), buf.G,
-                  int(d), int(page), max(1, int(block_table.shape[1])),
-                  DTYPES[q.dtype], _lib.stream_of(dev))
+    if T == 0 or n_req == 0:
+        return
+    _lib.launch(dev, "amass_paged_chunk", _lib.CHUNK.pack(
+        qp, k, v, block_table.data_ptr(), seq_lens.data_ptr(),
+        query_start_loc.data_ptr(), *buf.scratch, op,
+        0 if lse is None else lse.data_ptr(), q_st, q_sh, k_sb, k_st, k_sh,
+        v_sb, v_st, v_sh, block_table.stride(0), o_st, o_sh, scale, nb,
+        buf.n_ctas, window or 0, T, n_req, n_kv, buf.G, d, page, max_pages,
+        DTYPES[dtype]))

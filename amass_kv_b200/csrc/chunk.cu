@@ -821,71 +821,67 @@ int chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk,
 }  // namespace
 }  // namespace amass
 
-extern "C" int amass_paged_chunk(
-    const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
-    int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb,
-    int64_t v_st, int64_t v_sh, int num_blocks, const int32_t* block_table,
-    int64_t bt_stride, const int32_t* seq_lens,
-    const int32_t* query_start_loc, float* acc_part, float* ml_part,
-    int32_t* meta, int n_ctas, int32_t* fault, void* out, int64_t o_stride_t,
-    int64_t o_stride_h, float* lse, float scale, int window, int n_tokens,
-    int n_req, int n_kv, int G, int head_dim, int page, int max_pages,
-    int dtype, void* stream) {
+extern "C" int amass_paged_chunk(const AmassChunk* args, void* stream) {
   using namespace amass;
-  if (n_tokens < 0 || n_req < 0 || n_kv <= 0 || G <= 0 || head_dim <= 0 ||
-      page <= 0 || max_pages <= 0 || num_blocks <= 0 || n_ctas <= 0 ||
-      window < 0 || !(scale > 0.f) || scale > 3e38f || bt_stride < 0 ||
-      (dtype != AMASS_BF16 && dtype != AMASS_FP16))
+  if (!args) return AMASS_ERR_ARG;
+  const AmassChunk& x = *args;
+  if (x.n_tokens < 0 || x.n_req < 0 || x.n_kv <= 0 || x.G <= 0 ||
+      x.head_dim <= 0 || x.page <= 0 || x.max_pages <= 0 ||
+      x.num_blocks <= 0 || x.n_ctas <= 0 || x.window < 0 ||
+      !(x.scale > 0.f) || x.scale > 3e38f || x.bt_stride < 0 ||
+      (x.dtype != AMASS_BF16 && x.dtype != AMASS_FP16))
     return AMASS_ERR_ARG;
-  if (n_tokens == 0 || n_req == 0) return AMASS_OK;
-  if (!q || !k || !v || !block_table || !seq_lens || !query_start_loc ||
-      !acc_part || !ml_part || !meta || !fault || !out)
+  if (x.n_tokens == 0 || x.n_req == 0) return AMASS_OK;
+  if (!x.q || !x.k || !x.v || !x.block_table || !x.seq_lens ||
+      !x.query_start_loc || !x.acc_part || !x.ml_part || !x.meta ||
+      !x.fault || !x.out)
     return AMASS_ERR_ARG;
-  if ((head_dim != 64 && head_dim != 128) || G > 8 || page != kPg ||
-      n_req > kChMaxReq || max_pages > (1 << 26))
+  if ((x.head_dim != 64 && x.head_dim != 128) || x.G > 8 || x.page != kPg ||
+      x.n_req > kChMaxReq || x.max_pages > (1 << 26))
     return AMASS_ERR_UNSUPPORTED;
   // TMA and 16-byte stores: 16-byte aligned bases and strides
-  const uintptr_t bases = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v |
-                          (uintptr_t)out | (uintptr_t)acc_part;
-  if ((bases & 15) || ((o_stride_t | o_stride_h) & 7)) return AMASS_ERR_ARG;
-  const int64_t qs[2] = {q_stride_h, q_stride_t};
-  const int64_t ks[6] = {k_sh, k_st, k_sb, v_sh, v_st, v_sb};
-  const int64_t qd[2] = {(int64_t)n_kv * G, n_tokens};
-  const int64_t kd[3] = {n_kv, kPg, num_blocks};
-  for (int i = 0; i < 2; ++i)
-    if (qd[i] > 1 && (qs[i] <= 0 || (qs[i] & 7))) return AMASS_ERR_ARG;
-  for (int i = 0; i < 6; ++i)
-    if (kd[i % 3] > 1 && (ks[i] <= 0 || (ks[i] & 7))) return AMASS_ERR_ARG;
+  const uintptr_t bases = (uintptr_t)x.q | (uintptr_t)x.k | (uintptr_t)x.v |
+                          (uintptr_t)x.out | (uintptr_t)x.acc_part |
+                          (uintptr_t)x.ml_part | (uintptr_t)x.meta;
+  if ((bases & 15) || ((x.o_st | x.o_sh) & 7)) return AMASS_ERR_ARG;
+  const uint64_t d = (uint64_t)x.head_dim;
+  const uint64_t qdim[3] = {d, (uint64_t)(x.n_kv * x.G),
+                            (uint64_t)x.n_tokens};
+  const uint64_t kdim[4] = {d, (uint64_t)x.n_kv, (uint64_t)kPg,
+                            (uint64_t)x.num_blocks};
+  const int64_t qstr[3] = {1, x.q_sh, x.q_st};
+  const int64_t kstr[4] = {1, x.k_sh, x.k_st, x.k_sb};
+  const int64_t vstr[4] = {1, x.v_sh, x.v_st, x.v_sb};
+  const auto bad = [](uint64_t n, int64_t s) {
+    return n > 1 && (s <= 0 || (s & 7));
+  };
+  for (int i = 1; i < 4; ++i)
+    if ((i < 3 && bad(qdim[i], qstr[i])) || bad(kdim[i], kstr[i]) ||
+        bad(kdim[i], vstr[i]))
+      return AMASS_ERR_ARG;
 
   ChunkArgs a = {};
-  a.bt = block_table; a.bt_stride = bt_stride; a.sl = seq_lens;
-  a.qsl = query_start_loc; a.out = out; a.o_st = o_stride_t;
-  a.o_sh = o_stride_h; a.lse = lse; a.acc = acc_part;
-  a.ml = reinterpret_cast<float2*>(ml_part);
-  a.meta = reinterpret_cast<int4*>(meta); a.fault = fault;
-  a.scale_log2 = scale * kLog2e;
-  a.n_req = n_req; a.n_kv = n_kv; a.G = G; a.T = n_tokens;
-  a.max_pages = max_pages; a.nb = num_blocks; a.window = window;
+  a.bt = x.block_table; a.bt_stride = x.bt_stride; a.sl = x.seq_lens;
+  a.qsl = x.query_start_loc; a.out = x.out; a.o_st = x.o_st; a.o_sh = x.o_sh;
+  a.lse = x.lse; a.acc = x.acc_part;
+  a.ml = reinterpret_cast<float2*>(x.ml_part);
+  a.meta = reinterpret_cast<int4*>(x.meta); a.fault = x.fault;
+  a.scale_log2 = x.scale * kLog2e;
+  a.n_req = x.n_req; a.n_kv = x.n_kv; a.G = x.G; a.T = x.n_tokens;
+  a.max_pages = x.max_pages; a.nb = x.num_blocks; a.window = x.window;
   // tokens of a row tile: the largest power of two whose G heads fit 128 rows
-  a.tm_log2 = G == 1 ? 7 : G == 2 ? 6 : G <= 4 ? 5 : 4;
-  const bool f16 = dtype == AMASS_FP16;
-  const uint64_t d = (uint64_t)head_dim;
-  CUtensorMap mq, mk, mv;
-  const uint64_t qdim[3] = {d, (uint64_t)(n_kv * G), (uint64_t)n_tokens};
-  const int64_t qstr[3] = {1, q_stride_h, q_stride_t};
-  const uint32_t qbox[3] = {64, (uint32_t)G, 1u << a.tm_log2};
-  const uint64_t kdim[4] = {d, (uint64_t)n_kv, (uint64_t)kPg,
-                            (uint64_t)num_blocks};
-  const int64_t kstr[4] = {1, k_sh, k_st, k_sb};
-  const int64_t vstr[4] = {1, v_sh, v_st, v_sb};
+  a.tm_log2 = x.G == 1 ? 7 : x.G == 2 ? 6 : x.G <= 4 ? 5 : 4;
+  const bool f16 = x.dtype == AMASS_FP16;
+  const uint32_t qbox[3] = {64, (uint32_t)x.G, 1u << a.tm_log2};
   const uint32_t kbox[4] = {64, 1, (uint32_t)kPg, 1};
-  int rc = make_map(&mq, f16, q, 3, qdim, qstr, qbox);
-  if (!rc) rc = make_map(&mk, f16, k, 4, kdim, kstr, kbox);
-  if (!rc) rc = make_map(&mv, f16, v, 4, kdim, vstr, kbox);
+  CUtensorMap mq, mk, mv;
+  int rc = make_map(&mq, f16, x.q, 3, qdim, qstr, qbox);
+  if (!rc) rc = make_map(&mk, f16, x.k, 4, kdim, kstr, kbox);
+  if (!rc) rc = make_map(&mv, f16, x.v, 4, kdim, vstr, kbox);
   if (rc) return rc;
-  const int ctas = n_ctas < num_sms() ? n_ctas : num_sms();
+  const int ctas = x.n_ctas < num_sms() ? x.n_ctas : num_sms();
   const cudaStream_t st = (cudaStream_t)stream;
-  if (head_dim == 128)
+  if (x.head_dim == 128)
     return f16 ? chunk_launch<128, true>(mq, mk, mv, a, ctas, st)
                : chunk_launch<128, false>(mq, mk, mv, a, ctas, st);
   return f16 ? chunk_launch<64, true>(mq, mk, mv, a, ctas, st)

@@ -28,8 +28,8 @@ namespace {
 constexpr int kPgThreads = 512;
 constexpr int kPgMaxReq = 4096;          // 32 KB of request sums
 
-AMASS_DEV int pages_of(int64_t tokens, int page) {
-  return (int)((tokens + page - 1) / page);
+AMASS_DEV int pages_of(int tokens, int page) {   // tokens + page < 2^32
+  return (int)(((unsigned)tokens + (unsigned)page - 1u) / (unsigned)page);
 }
 
 // exclusive prefix of (a, b) over the CTA's threads; *ta, *tb the totals
@@ -71,6 +71,10 @@ AMASS_DEV int find_start(const int* start, int n, int t) {
 // true in every thread of the CTA that finishes last; its ticket is reset
 AMASS_DEV bool last_cta(int32_t* ticket) {
   __shared__ int last;
+  if (gridDim.x == 1) {
+    __syncthreads();
+    return true;
+  }
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -83,57 +87,54 @@ AMASS_DEV bool last_cta(int32_t* ticket) {
 }
 
 __global__ void __launch_bounds__(kPgThreads)
-pages_begin_kernel(const int32_t* __restrict__ new_tokens, int n_req,
-                   int32_t* block_table, int64_t bt_stride, int32_t* seq_lens,
-                   const int32_t* __restrict__ free_stack, int32_t* free_top,
-                   int num_blocks, int32_t* query_start_loc,
-                   int64_t* positions, int64_t* slot_mapping, int n_tokens,
-                   int32_t* status, int32_t* overflow, int32_t* ticket,
-                   int max_pages, int page) {
+pages_begin_kernel(const __grid_constant__ AmassPagePool p,
+                   const int32_t* __restrict__ new_tokens, int n_req,
+                   int n_tokens) {
   grid_dep_wait();
   grid_dep_launch();
   extern __shared__ int sm[];
   int* start = sm;                       // n_req + 1: first token
   int* pre = sm + n_req + 1;             // n_req: first new block, -1 refused
-  const int tid = threadIdx.x;
-  const int top = min(max(*free_top, 0), num_blocks);
+  __shared__ int used;                   // blocks granted
+  const int tid = threadIdx.x, most = p.max_pages * p.page;
+  if (tid == 0) used = 0;                // set before scan2's barriers
+  const int top = min(max(*p.free_top, 0), p.num_blocks);
   const int per = (n_req + kPgThreads - 1) / kPgThreads;
   const int r0 = min(n_req, tid * per), r1 = min(n_req, r0 + per);
   int sn = 0, sd = 0;
   for (int r = r0; r < r1; ++r) {
-    const int nw = max(new_tokens[r], 0), old = max(seq_lens[r], 0);
+    const int nw = max(new_tokens[r], 0), old = max(p.seq_lens[r], 0);
     const int64_t want = (int64_t)old + nw;
     sn += nw;
-    if (want <= (int64_t)max_pages * page)
-      sd += pages_of(want, page) - pages_of(old, page);
+    if (want <= most) sd += pages_of((int)want, p.page) - pages_of(old, p.page);
   }
   int total, need_all;
   scan2(sn, sd, &total, &need_all);
-  int flags = 0, taken = 0;
+  int flags = 0;
   for (int r = r0; r < r1; ++r) {
-    const int nw = max(new_tokens[r], 0), old = max(seq_lens[r], 0);
+    const int nw = max(new_tokens[r], 0), old = max(p.seq_lens[r], 0);
     const int64_t want = (int64_t)old + nw;
     start[r] = sn;
     sn += nw;
     int st = 0, need = 0;
-    if (want > (int64_t)max_pages * page) {
+    if (want > most) {
       st = 2;
     } else {
-      need = pages_of(want, page) - pages_of(old, page);
+      need = pages_of((int)want, p.page) - pages_of(old, p.page);
       if (need > 0 && sd + need > top) st = 1;
     }
     pre[r] = st ? -1 : sd;
     sd += need;
     flags |= st;
-    if (st == 0) taken += need;
+    if (st == 0 && need > 0) atomicMax(&used, sd);   // granted: a prefix
     if (blockIdx.x == 0) {
-      status[r] = st;
-      query_start_loc[r] = start[r];
+      p.status[r] = st;
+      p.query_start_loc[r] = start[r];
     }
   }
   if (tid == 0) {
     start[n_req] = total;
-    if (blockIdx.x == 0) query_start_loc[n_req] = total;
+    if (blockIdx.x == 0) p.query_start_loc[n_req] = total;
   }
   __syncthreads();
 
@@ -143,54 +144,50 @@ pages_begin_kernel(const int32_t* __restrict__ new_tokens, int n_req,
     int64_t pos = 0, slot = -1;
     if (t < total) {
       const int r = find_start(start, n_req, (int)t);
-      const int old = max(seq_lens[r], 0);   // committed after the ticket
-      pos = old + (t - start[r]);
-      const int64_t pg = pos / page;
-      const int off = (int)(pos - pg * page);
-      if (pre[r] >= 0 && pg < max_pages) {
-        const int have = pages_of(old, page);
-        int32_t* e = block_table + (int64_t)r * bt_stride + pg;
+      const int old = max(p.seq_lens[r], 0);   // committed after the ticket
+      pos = (int64_t)old + (t - start[r]);
+      const int pg = (int)((unsigned)pos / (unsigned)p.page);
+      const int off = (int)pos - pg * p.page;
+      if (pre[r] >= 0 && pg < p.max_pages) {
+        const int have = pages_of(old, p.page);
+        int32_t* e = p.block_table + (int64_t)r * p.bt_stride + pg;
         int b = -1;
         if (pg < have) {
           b = *e;
         } else {
-          const int k = top - 1 - (pre[r] + (int)pg - have);
+          const int k = top - 1 - (pre[r] + pg - have);
           if (k >= 0) {
-            b = free_stack[k];
+            b = p.free_stack[k];
             if (off == 0) *e = b;
           }
         }
-        if (b >= 0) slot = (int64_t)b * page + off;
+        if (b >= 0) slot = (int64_t)b * p.page + off;
       }
     }
     if (t < n_tokens) {
-      positions[t] = pos;
-      slot_mapping[t] = slot;
+      p.positions[t] = pos;
+      p.slot_mapping[t] = slot;
     }
   }
   const int short_f = __syncthreads_or(flags & 1);
   const int long_f = __syncthreads_or(flags & 2);
-  if (!last_cta(ticket)) return;
-  int zero = 0, used, z;
-  scan2(taken, zero, &used, &z);
+  if (!last_cta(p.ticket)) return;
   for (int r = r0; r < r1; ++r) {
     if (pre[r] < 0) continue;
     const int nx = r + 1 < n_req ? start[r + 1] : total;
-    seq_lens[r] = max(seq_lens[r], 0) + (nx - start[r]);
+    p.seq_lens[r] = max(p.seq_lens[r], 0) + (nx - start[r]);
   }
   if (tid == 0) {
-    *free_top = top - used;
+    *p.free_top = top - used;
     const int f = (short_f ? 1 : 0) | (long_f ? 2 : 0) |
                   (total > n_tokens ? 4 : 0);
-    if (f) *overflow |= f;
+    if (f) *p.overflow |= f;
   }
 }
 
 __global__ void __launch_bounds__(kPgThreads)
-pages_trim_kernel(const int32_t* __restrict__ drop, int whole, int n_req,
-                  int32_t* block_table, int64_t bt_stride, int32_t* seq_lens,
-                  int32_t* free_stack, int32_t* free_top, int num_blocks,
-                  int32_t* ticket, int max_pages, int page) {
+pages_trim_kernel(const __grid_constant__ AmassPagePool p,
+                  const int32_t* __restrict__ drop, int n_req, int whole) {
   grid_dep_wait();
   grid_dep_launch();
   extern __shared__ int sm[];
@@ -198,22 +195,21 @@ pages_trim_kernel(const int32_t* __restrict__ drop, int whole, int n_req,
                                          // order of descending request
   int* left = sm + n_req + 1;            // n_req: tokens kept, by request
   const int tid = threadIdx.x;
-  const int top = min(max(*free_top, 0), num_blocks);
+  const int top = min(max(*p.free_top, 0), p.num_blocks);
   const int per = (n_req + kPgThreads - 1) / kPgThreads;
   const int i0 = min(n_req, tid * per), i1 = min(n_req, i0 + per);
   const auto kept = [&](int r, int* have) {
-    const int old = (int)min((int64_t)max(seq_lens[r], 0),
-                             (int64_t)max_pages * page);
+    const int old = min(max(p.seq_lens[r], 0), p.max_pages * p.page);
     const int d = whole ? (drop[r] != 0 ? old : 0)
                         : min(max(drop[r], 0), old);
-    *have = pages_of(old, page);
+    *have = pages_of(old, p.page);
     return old - d;
   };
   int s = 0, zero = 0, total, z;
   for (int i = i0; i < i1; ++i) {
     int have;
     const int k = kept(n_req - 1 - i, &have);
-    s += have - pages_of(k, page);
+    s += have - pages_of(k, p.page);
   }
   scan2(s, zero, &total, &z);
   for (int i = i0; i < i1; ++i) {
@@ -221,7 +217,7 @@ pages_trim_kernel(const int32_t* __restrict__ drop, int whole, int n_req,
     int have;
     left[r] = kept(r, &have);
     start[i] = s;
-    s += have - pages_of(left[r], page);
+    s += have - pages_of(left[r], p.page);
   }
   if (tid == 0) start[n_req] = total;
   __syncthreads();
@@ -230,14 +226,14 @@ pages_trim_kernel(const int32_t* __restrict__ drop, int whole, int n_req,
     const int i = find_start(start, n_req, k), r = n_req - 1 - i;
     // the request's freed pages are keep .. keep + n - 1, last one first
     const int n = start[i + 1] - start[i];
-    const int pg = pages_of(left[r], page) + n - 1 - (k - start[i]);
-    int32_t* e = block_table + (int64_t)r * bt_stride + pg;
-    if (top + k < num_blocks) free_stack[top + k] = *e;
+    const int pg = pages_of(left[r], p.page) + n - 1 - (k - start[i]);
+    int32_t* e = p.block_table + (int64_t)r * p.bt_stride + pg;
+    if (top + k < p.num_blocks) p.free_stack[top + k] = *e;
     *e = -1;
   }
-  if (!last_cta(ticket)) return;
-  for (int i = i0; i < i1; ++i) seq_lens[n_req - 1 - i] = left[n_req - 1 - i];
-  if (tid == 0) *free_top = min(top + total, num_blocks);
+  if (!last_cta(p.ticket)) return;
+  for (int i = i0; i < i1; ++i) p.seq_lens[n_req - 1 - i] = left[n_req - 1 - i];
+  if (tid == 0) *p.free_top = min(top + total, p.num_blocks);
 }
 
 __global__ void __launch_bounds__(kPgThreads)
@@ -259,10 +255,10 @@ slot_map_kernel(const int32_t* __restrict__ block_table, int64_t bt_stride,
     if (t >= sm[0] && t < sm[n_req]) {
       const int r = find_start(sm, n_req, (int)t);
       pos = (int64_t)seq_lens[r] - (sm[r + 1] - t);
-      const int64_t pg = pos / page;
+      const int pg = (int)((unsigned)pos / (unsigned)page);
       if (pos >= 0 && pg < max_pages) {
         const int b = block_table[(int64_t)r * bt_stride + pg];
-        if (b >= 0) slot = (int64_t)b * page + (pos - pg * page);
+        if (b >= 0) slot = (int64_t)b * page + ((int)pos - pg * page);
       }
     }
     positions[t] = pos;
@@ -278,53 +274,41 @@ int grid_for(int64_t items, int per_cta) {
 }  // namespace
 }  // namespace amass
 
-extern "C" int amass_pages_begin(const int32_t* new_tokens, int n_req,
-                                 int32_t* block_table, int64_t bt_stride,
-                                 int32_t* seq_lens, const int32_t* free_stack,
-                                 int32_t* free_top, int num_blocks,
-                                 int32_t* query_start_loc, int64_t* positions,
-                                 int64_t* slot_mapping, int n_tokens,
-                                 int32_t* status, int32_t* overflow,
-                                 int32_t* ticket, int max_pages, int page,
-                                 void* stream) {
+static bool pool_ok(const AmassPagePool* p) {
+  return p && p->block_table && p->seq_lens && p->free_stack && p->free_top &&
+         p->query_start_loc && p->positions && p->slot_mapping && p->status &&
+         p->overflow && p->ticket && p->bt_stride >= 0 && p->num_blocks > 0 &&
+         p->max_reqs > 0 && p->max_pages > 0 && p->max_tokens > 0 &&
+         p->page > 0 && (int64_t)p->max_pages * p->page < (1ll << 31);
+}
+
+extern "C" int amass_pages_begin(const AmassPagePool* pool,
+                                 const int32_t* new_tokens, int n_req,
+                                 int n_tokens, void* stream) {
   using namespace amass;
-  if (n_req < 0 || n_tokens < 0 || num_blocks < 0 || max_pages <= 0 ||
-      page <= 0 || bt_stride < 0 || !free_top || !query_start_loc ||
-      !overflow || !ticket || (num_blocks > 0 && !free_stack) ||
-      (n_tokens > 0 && (!positions || !slot_mapping)) ||
-      (n_req > 0 && (!new_tokens || !block_table || !seq_lens || !status)))
+  if (!pool_ok(pool) || n_req < 0 || n_req > pool->max_reqs || n_tokens < 0 ||
+      n_tokens > pool->max_tokens || (n_req > 0 && !new_tokens))
     return AMASS_ERR_ARG;
   if (n_req > kPgMaxReq) return AMASS_ERR_UNSUPPORTED;
   return launch_pdl(pages_begin_kernel, dim3(grid_for(n_tokens, kPgThreads)),
                     dim3(kPgThreads), (2 * n_req + 1) * sizeof(int),
-                    (cudaStream_t)stream, new_tokens, n_req, block_table,
-                    bt_stride, seq_lens, free_stack, free_top, num_blocks,
-                    query_start_loc, positions, slot_mapping, n_tokens,
-                    status, overflow, ticket, max_pages, page);
+                    (cudaStream_t)stream, *pool, new_tokens, n_req, n_tokens);
 }
 
-extern "C" int amass_pages_trim(const int32_t* drop, int whole, int n_req,
-                                int32_t* block_table, int64_t bt_stride,
-                                int32_t* seq_lens, int32_t* free_stack,
-                                int32_t* free_top, int num_blocks,
-                                int32_t* ticket, int max_pages, int page,
-                                void* stream) {
+extern "C" int amass_pages_trim(const AmassPagePool* pool, const int32_t* drop,
+                                int n_req, int whole, void* stream) {
   using namespace amass;
-  if (n_req < 0 || num_blocks < 0 || max_pages <= 0 || page <= 0 ||
-      bt_stride < 0 || !free_top || !ticket ||
-      (num_blocks > 0 && !free_stack) ||
-      (n_req > 0 && (!drop || !block_table || !seq_lens)))
+  if (!pool_ok(pool) || n_req < 0 || n_req > pool->max_reqs ||
+      (n_req > 0 && !drop))
     return AMASS_ERR_ARG;
   if (n_req > kPgMaxReq) return AMASS_ERR_UNSUPPORTED;
   if (n_req == 0) return AMASS_OK;
   // the number of pages that return is known on the device only: a whole
   // release may free every row, a truncation mostly a page or two per request
-  const int64_t most = whole ? (int64_t)n_req * max_pages : 4ll * n_req;
+  const int64_t most = whole ? (int64_t)n_req * pool->max_pages : 4ll * n_req;
   return launch_pdl(pages_trim_kernel, dim3(grid_for(most, 4 * kPgThreads)),
                     dim3(kPgThreads), (2 * n_req + 1) * sizeof(int),
-                    (cudaStream_t)stream, drop, whole, n_req, block_table,
-                    bt_stride, seq_lens, free_stack, free_top, num_blocks,
-                    ticket, max_pages, page);
+                    (cudaStream_t)stream, *pool, drop, n_req, whole);
 }
 
 extern "C" int amass_slot_map(const int32_t* block_table, int64_t bt_stride,

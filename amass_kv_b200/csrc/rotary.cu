@@ -196,49 +196,49 @@ int rot_launch(const RotArgs& a, bool vec, cudaStream_t st) {
 }  // namespace
 }  // namespace amass
 
-extern "C" int amass_rotary_write(
-    const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st,
-    int64_t qo_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
-    int64_t v_st, int64_t v_sh, void* k_dst, int64_t kd_sb, int64_t kd_st,
-    int64_t kd_sh, void* v_dst, int64_t vd_sb, int64_t vd_st, int64_t vd_sh,
-    const int64_t* slot_mapping, int num_blocks, int page,
-    const void* positions, int pos64, const uint64_t* freq, float mscale,
-    int layout, int rotary_dim, int n_tokens, int H, int n_kv, int head_dim,
-    int dtype, void* stream) {
+extern "C" int amass_rotary_write(const AmassRotary* args, void* stream) {
   using namespace amass;
-  if (n_tokens < 0 || H < 0 || n_kv < 0 || head_dim <= 0 || rotary_dim <= 0 ||
-      rotary_dim > head_dim || num_blocks < 0 || page <= 0 ||
-      (n_tokens > 0 && (!positions || !freq)) || (!q) != (!q_out) ||
-      (!k) != (!k_dst) || (!v) != (!v_dst) || (v && !k) ||
-      (layout != AMASS_ROTARY_HALF && layout != AMASS_ROTARY_INTERLEAVED) ||
-      (dtype != AMASS_BF16 && dtype != AMASS_FP16))
+  if (!args) return AMASS_ERR_ARG;
+  const AmassRotary& x = *args;
+  if (x.n_tokens < 0 || x.H < 0 || x.n_kv < 0 || x.head_dim <= 0 ||
+      x.rotary_dim <= 0 || x.rotary_dim > x.head_dim || x.num_blocks < 0 ||
+      x.page <= 0 || (x.n_tokens > 0 && (!x.positions || !x.freq)) ||
+      (!x.q) != (!x.q_out) || (!x.k) != (!x.k_dst) || (!x.v) != (!x.v_dst) ||
+      (x.v && !x.k) ||
+      (x.layout != AMASS_ROTARY_HALF &&
+       x.layout != AMASS_ROTARY_INTERLEAVED) ||
+      (x.dtype != AMASS_BF16 && x.dtype != AMASS_FP16))
     return AMASS_ERR_ARG;
-  if (head_dim > kRotMaxDim || (head_dim & 1) || (rotary_dim & 1))
+  if (x.head_dim > kRotMaxDim || (x.head_dim & 1) || (x.rotary_dim & 1))
     return AMASS_ERR_UNSUPPORTED;
   RotArgs a = {};
-  a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v;
-  a.qo = (char*)q_out; a.kd = (char*)k_dst; a.vd = (char*)v_dst;
-  a.q_st = q_st; a.q_sh = q_sh; a.qo_st = qo_st; a.qo_sh = qo_sh;
-  a.k_st = k_st; a.k_sh = k_sh; a.v_st = v_st; a.v_sh = v_sh;
-  a.kd_sb = kd_sb; a.kd_st = kd_st; a.kd_sh = kd_sh;
-  a.vd_sb = vd_sb; a.vd_st = vd_st; a.vd_sh = vd_sh;
-  a.slots = slot_mapping; a.pos = positions; a.freq = freq;
-  a.page = slot_mapping ? page : 1;
-  a.n_slots = slot_mapping ? (int64_t)num_blocks * page : n_tokens;
-  a.mscale = mscale; a.pos64 = pos64; a.rot = rotary_dim; a.T = n_tokens;
-  a.H = q ? H : 0; a.n_kv = k ? n_kv : 0; a.d = head_dim;
+  a.q = (const char*)x.q; a.k = (const char*)x.k; a.v = (const char*)x.v;
+  a.qo = (char*)x.q_out; a.kd = (char*)x.k_dst; a.vd = (char*)x.v_dst;
+  a.q_st = x.q_st; a.q_sh = x.q_sh; a.qo_st = x.qo_st; a.qo_sh = x.qo_sh;
+  a.k_st = x.k_st; a.k_sh = x.k_sh; a.v_st = x.v_st; a.v_sh = x.v_sh;
+  a.kd_sb = x.kd_sb; a.kd_st = x.kd_st; a.kd_sh = x.kd_sh;
+  a.vd_sb = x.vd_sb; a.vd_st = x.vd_st; a.vd_sh = x.vd_sh;
+  a.slots = x.slot_mapping; a.pos = x.positions; a.freq = x.freq;
+  a.page = x.slot_mapping ? x.page : 1;
+  a.n_slots = x.slot_mapping ? (int64_t)x.num_blocks * x.page : x.n_tokens;
+  a.mscale = x.mscale; a.pos64 = x.pos64; a.rot = x.rotary_dim;
+  a.T = x.n_tokens; a.H = x.q ? x.H : 0; a.n_kv = x.k ? x.n_kv : 0;
+  a.d = x.head_dim;
+  const int head_dim = x.head_dim, rotary_dim = x.rotary_dim;
+  const int n_tokens = x.n_tokens;
   if (n_tokens == 0 || a.H + a.n_kv == 0) return AMASS_OK;
   // 16-byte items need whole items in the rotated part and in the rest, and
   // 16-byte aligned rows; anything else goes pair by pair
-  const int64_t strides = q_st | q_sh | qo_st | qo_sh | k_st | k_sh | v_st |
-                          v_sh | kd_sb | kd_st | kd_sh | vd_sb | vd_st | vd_sh;
-  const uintptr_t base = (uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k |
-                         (uintptr_t)k_dst | (uintptr_t)v | (uintptr_t)v_dst;
+  const int64_t strides = a.q_st | a.q_sh | a.qo_st | a.qo_sh | a.k_st |
+                          a.k_sh | a.v_st | a.v_sh | a.kd_sb | a.kd_st |
+                          a.kd_sh | a.vd_sb | a.vd_st | a.vd_sh;
+  const uintptr_t base = (uintptr_t)a.q | (uintptr_t)a.qo | (uintptr_t)a.k |
+                         (uintptr_t)a.kd | (uintptr_t)a.v | (uintptr_t)a.vd;
   const bool vec = !(head_dim & 15) && !(rotary_dim & 15) && !(strides & 7) &&
                    !(base & 15);
   // enough items per CTA that its angles and its one barrier are small
   // beside its copies, while every SM still has several CTAs
-  const int64_t items = (int64_t)(a.H + a.n_kv * (v ? 2 : 1)) *
+  const int64_t items = (int64_t)(a.H + a.n_kv * (a.v ? 2 : 1)) *
                         (vec ? head_dim >> 4 : head_dim >> 1);
   int64_t tok = (6ll * kRotThreads + items - 1) / items;
   const int64_t spread = ((int64_t)n_tokens + 4 * num_sms() - 1) /
@@ -246,8 +246,8 @@ extern "C" int amass_rotary_write(
   if (tok > spread) tok = spread;
   a.tok = (int)(tok < 1 ? 1 : tok > kRotMaxTok ? kRotMaxTok : tok);
   const cudaStream_t st = (cudaStream_t)stream;
-  const bool half = layout == AMASS_ROTARY_HALF;
-  if (dtype == AMASS_FP16)
+  const bool half = x.layout == AMASS_ROTARY_HALF;
+  if (x.dtype == AMASS_FP16)
     return half ? rot_launch<true, true>(a, vec, st)
                 : rot_launch<true, false>(a, vec, st);
   return half ? rot_launch<false, true>(a, vec, st)

@@ -19,7 +19,6 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import ptr
 from .attention import check_i32
 
 MAX_REQS = 4096
@@ -54,9 +53,7 @@ class BlockPool:
                              f"{max_reqs}")
         if max_pages * page >= 1 << 31:
             raise ValueError("max_pages * page must fit int32")
-        dev = torch.device(device)
-        if dev.index is None and dev.type == "cuda":
-            dev = torch.device("cuda", torch.cuda.current_device())
+        dev = _lib.device_of(device)
         self.device, self.NB, self.R = dev, num_blocks, max_reqs
         self.MP, self.max_tokens, self.page = max_pages, max_tokens, page
         kw = dict(dtype=torch.int32, device=dev)
@@ -73,13 +70,30 @@ class BlockPool:
         self.slot_mapping = torch.full((max_tokens,), -1, dtype=torch.int64,
                                        device=dev)
 
+        self._index = -1 if dev.index is None else dev.index
+        # the C side's view of the buffers: fill them in place, they are not
+        # to be replaced
+        self._pool = _lib.PAGE_POOL.pack(
+            *(t.data_ptr() for t in (
+                self.block_table, self.seq_lens, self.free_stack,
+                self.free_top, self.query_start_loc, self.positions,
+                self.slot_mapping, self.status, self.overflow, self.ticket)),
+            self.block_table.stride(0), num_blocks, max_reqs, max_pages,
+            max_tokens, page, 0)
+        self._fixed = True
+
+    def __setattr__(self, name, value):
+        if getattr(self, "_fixed", False):
+            raise AttributeError(f"BlockPool.{name} is fixed: fill the "
+                                 "buffers in place")
+        object.__setattr__(self, name, value)
+
     def _rows(self, t, name: str) -> int:
-        check_i32(self.device, **{name: t})
-        if t.dim() != 1 or t.shape[0] > self.R or \
-                (t.shape[0] > 1 and t.stride(0) != 1):
-            raise ValueError(f"{name} must be a contiguous vector of at most "
-                             f"{self.R} rows, got {tuple(t.shape)}")
-        return int(t.shape[0])
+        check_i32(self._index, name, t, 1)
+        n = t.shape[0]
+        if n > self.R:
+            raise ValueError(f"{name} has {n} rows, the pool {self.R}")
+        return n
 
     def begin_step(self, new_tokens, n_tokens: int | None = None) -> None:
         """Rows 0 .. len(new_tokens) - 1 grow by ``new_tokens`` (int32, < 0
@@ -91,35 +105,24 @@ class BlockPool:
         nt = self.max_tokens if n_tokens is None else int(n_tokens)
         if not 0 <= nt <= self.max_tokens:
             raise ValueError(f"n_tokens {nt} outside 0 .. {self.max_tokens}")
-        with torch.cuda.device(self.device):
-            _lib.call("amass_pages_begin", ptr(new_tokens), n,
-                      ptr(self.block_table), self.block_table.stride(0),
-                      ptr(self.seq_lens), ptr(self.free_stack),
-                      ptr(self.free_top), self.NB, ptr(self.query_start_loc),
-                      ptr(self.positions), ptr(self.slot_mapping), nt,
-                      ptr(self.status), ptr(self.overflow), ptr(self.ticket),
-                      self.MP, self.page, _lib.stream_of(self.device))
-
-    def _trim(self, rows, whole: int) -> None:
-        n = self._rows(rows, "done" if whole else "drop")
-        with torch.cuda.device(self.device):
-            _lib.call("amass_pages_trim", ptr(rows), whole, n,
-                      ptr(self.block_table), self.block_table.stride(0),
-                      ptr(self.seq_lens), ptr(self.free_stack),
-                      ptr(self.free_top), self.NB, ptr(self.ticket), self.MP,
-                      self.page, _lib.stream_of(self.device))
+        _lib.launch(self._index, "amass_pages_begin", self._pool,
+                    new_tokens.data_ptr(), n, nt)
 
     def truncate(self, drop) -> None:
         """Row r loses its last ``drop[r]`` tokens (int32; clipped to what it
         has).  Pages left empty go back to the free stack, last row and last
         page first: dropping all that a ``begin_step`` granted restores the
         stack's order."""
-        self._trim(drop, 0)
+        n = self._rows(drop, "drop")
+        _lib.launch(self._index, "amass_pages_trim", self._pool,
+                    drop.data_ptr(), n, 0)
 
     def release(self, done) -> None:
         """Rows with ``done[r] != 0`` (int32) give back all their pages and
         become idle."""
-        self._trim(done, 1)
+        n = self._rows(done, "done")
+        _lib.launch(self._index, "amass_pages_trim", self._pool,
+                    done.data_ptr(), n, 1)
 
     def check(self) -> None:
         f = int(self.overflow.item())
@@ -139,30 +142,31 @@ def build_slot_map(block_table, seq_lens, query_start_loc, positions,
     query_start_loc[r] <= t < query_start_loc[r + 1], is one of the last of
     its ``seq_lens[r]``.  Slot -1 for a position without a block (< 0, beyond
     the table's row, block < 0); tokens of no request get 0 and -1."""
-    dev = block_table.device
-    check_i32(dev, block_table=block_table, seq_lens=seq_lens,
-              query_start_loc=query_start_loc)
+    dev = block_table.get_device()
+    check_i32(dev, "block_table", block_table, 2)
+    check_i32(dev, "seq_lens", seq_lens, 1)
+    check_i32(dev, "query_start_loc", query_start_loc, 1)
     n = seq_lens.shape[0]
-    if block_table.dim() != 2 or block_table.shape[0] < n or \
-            block_table.shape[1] < 1 or query_start_loc.shape[0] < n + 1:
-        raise ValueError(f"block_table {tuple(block_table.shape)} and "
+    rows, max_pages = block_table.shape
+    if rows < n or max_pages < 1 or query_start_loc.shape[0] < n + 1:
+        raise ValueError(f"block_table {(rows, max_pages)} and "
                          f"query_start_loc {tuple(query_start_loc.shape)} do "
                          f"not cover {n} requests")
     if n > MAX_REQS:
         raise ValueError(f"{n} requests > {MAX_REQS}")
-    if page < 1:
-        raise ValueError(f"page must be at least 1, got {page}")
+    if page < 1 or page * max_pages >= 1 << 31:
+        raise ValueError(f"page must be at least 1 and a row's tokens fit "
+                         f"int32, got {page} x {max_pages}")
     nt = slot_mapping.shape[0] if n_tokens is None else int(n_tokens)
     for name, t in (("positions", positions), ("slot_mapping", slot_mapping)):
-        if t.dtype != torch.int64 or t.device != dev or t.dim() != 1 or \
-                not t.is_contiguous() or not 0 <= nt <= t.shape[0]:
+        if t.dtype != torch.int64 or t.get_device() != dev or t.dim() != 1 \
+                or not t.is_contiguous() or not 0 <= nt <= t.shape[0]:
             raise ValueError(f"{name} must be a contiguous int64 vector of "
-                             f"at least {nt} tokens on {dev}")
-    with torch.cuda.device(dev):
-        _lib.call("amass_slot_map", ptr(block_table), block_table.stride(0),
-                  ptr(seq_lens), ptr(query_start_loc), int(n),
-                  ptr(positions), ptr(slot_mapping), nt,
-                  int(block_table.shape[1]), int(page), _lib.stream_of(dev))
+                             f"at least {nt} tokens on GPU {dev}")
+    _lib.launch(dev, "amass_slot_map", block_table.data_ptr(),
+                block_table.stride(0), seq_lens.data_ptr(),
+                query_start_loc.data_ptr(), n, positions.data_ptr(),
+                slot_mapping.data_ptr(), nt, max_pages, page)
 
 
 __all__ = ["BlockPool", "build_slot_map"]

@@ -17,8 +17,7 @@ import math
 import torch
 
 from . import _lib
-from ._lib import ptr
-from .attention import DTYPES, split_kv
+from .attention import DTYPES, cache_layout
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 
@@ -109,9 +108,8 @@ class Rotary:
                              f"{rotary_dim}")
         if not 1.0 < base < float("inf"):
             raise ValueError(f"base must be above 1, got {base}")
-        dev = torch.device(device)
-        if dev.index is None and dev.type == "cuda":
-            dev = torch.device("cuda", torch.cuda.current_device())
+        dev = _lib.device_of(device)
+        self.index = -1 if dev.index is None else dev.index
         self.device, self.rotary_dim, self.layout = dev, rotary_dim, layout
         self.inv_freq, self.mscale = rotary_frequencies(rotary_dim, base,
                                                         scaling)
@@ -119,88 +117,89 @@ class Rotary:
         turns = [round(x / (2 * math.pi) * 2.0 ** 64)
                  for x in self.inv_freq.tolist()]
         self.freq = torch.tensor(turns, dtype=torch.int64, device=dev)
+        self._freq = self.freq.data_ptr()
 
 
-def _rows(name, t, dev, dtype, T, d):
-    if t.dim() != 3 or t.shape[0] < T or t.shape[2] != d:
-        raise ValueError(f"{name} must be (>= {T} tokens, heads, {d}), got "
-                         f"{tuple(t.shape)}")
-    if t.dtype != dtype or t.device != dev:
-        raise ValueError(f"{name} must be {dtype} on {dev}, got {t.dtype} on "
-                         f"{t.device}")
-    if t.stride(2) != 1:
-        raise ValueError(f"{name} must have a contiguous head_dim")
+_NONE = (0, 0, 0, 0)                     # pointer, token / head stride, heads
 
 
-def _launch(rot, q, q_out, k, v, k_dst, v_dst, slot_mapping, nb, page,
-            positions, n_tokens):
-    dev = rot.device
-    x = q if q is not None else k
-    if x is None:
-        raise ValueError("nothing to turn: q and k are both None")
-    if x.dim() != 3:
-        raise ValueError(f"q and k must be (T, heads, d), got "
+def _rows(rot, name, t, dtype, T, d):
+    """(address, token stride, head stride, heads) of (>= T, heads, d)."""
+    shape, s = t.shape, t.stride()
+    if len(shape) != 3 or shape[0] < T or shape[2] != d or s[2] != 1 or \
+            t.dtype != dtype or t.get_device() != rot.index:
+        raise ValueError(f"{name} must be (>= {T} tokens, heads, {d}) {dtype} "
+                         f"on GPU {rot.index} with a contiguous head_dim, got "
+                         f"{tuple(shape)} {t.dtype} on {t.device}")
+    return t.data_ptr(), s[0], s[1], shape[1]
+
+
+def _vector(rot, name, t, T, dtypes):
+    if t.dtype not in dtypes or t.get_device() != rot.index or \
+            t.dim() != 1 or t.shape[0] < T or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous vector of at least "
+                         f"{T} tokens, {' or '.join(map(str, dtypes))}, on "
+                         f"GPU {rot.index}")
+    return t.data_ptr()
+
+
+_INDEX = (torch.int64, torch.int32)
+
+
+def _launch(rot, x, q, q_out, k, v, k_dst, kd, v_dst, vd, slots, nb, page,
+            positions, T):
+    dtype, d = x.dtype, x.shape[-1]
+    if dtype not in DTYPES:
+        raise ValueError(f"q, k and v must be bf16 or fp16, got {dtype}")
+    if x.dim() != 3 or not 0 <= T <= x.shape[0]:
+        raise ValueError(f"n_tokens {T} outside the tokens of "
                          f"{tuple(x.shape)}")
-    T = x.shape[0] if n_tokens is None else int(n_tokens)
-    d = x.shape[2]
-    if x.dtype not in DTYPES:
-        raise ValueError(f"q, k and v must be bf16 or fp16, got {x.dtype}")
-    if T < 0 or T > x.shape[0]:
-        raise ValueError(f"n_tokens {T} outside 0 .. {x.shape[0]}")
     if rot.rotary_dim > d or d > 256 or d % 2:
         raise ValueError(f"no kernel for head_dim {d} with rotary_dim "
                          f"{rot.rotary_dim}")
-    for name, t in (("q", q), ("q_out", q_out), ("k", k), ("v", v)):
-        if t is not None:
-            _rows(name, t, dev, x.dtype, T, d)
-    if q is not None and q_out.shape[1] != q.shape[1]:
+    qp, q_st, q_sh, H = o = _NONE if q is None else \
+        _rows(rot, "q", q, dtype, T, d)
+    if q_out is not q:
+        o = _rows(rot, "q_out", q_out, dtype, T, d)
+    if o[3] != H:
         raise ValueError("q_out must have q's heads")
-    if v is not None and v.shape[1] != k.shape[1]:
+    kp, k_st, k_sh, n_kv = _NONE if k is None else \
+        _rows(rot, "k", k, dtype, T, d)
+    vp, v_st, v_sh, nv = _NONE if v is None else \
+        _rows(rot, "v", v, dtype, T, d)
+    if v is not None and nv != n_kv:
         raise ValueError("v must have k's heads")
-    if positions.dtype not in (torch.int32, torch.int64) or \
-            positions.device != dev or positions.dim() != 1 or \
-            positions.shape[0] < T or \
-            (positions.shape[0] > 1 and positions.stride(0) != 1):
-        raise ValueError(f"positions must be a contiguous int32 or int64 "
-                         f"vector of at least {T} tokens on {dev}")
-
-    def st(t, n):
-        return [0] * n if t is None else list(t.stride()[:n])
-    with torch.cuda.device(dev):
-        _lib.call("amass_rotary_write", ptr(q), *st(q, 2), ptr(q_out),
-                  *st(q_out, 2), ptr(k), *st(k, 2), ptr(v), *st(v, 2),
-                  ptr(k_dst), *(st(k_dst, 3) if slot_mapping is not None
-                                else _token_major(k_dst)),
-                  ptr(v_dst), *st(v_dst, 3), ptr(slot_mapping), int(nb),
-                  int(page), ptr(positions),
-                  1 if positions.dtype == torch.int64 else 0, ptr(rot.freq),
-                  float(rot.mscale), LAYOUTS[rot.layout], rot.rotary_dim,
-                  int(T), int(q.shape[1]) if q is not None else 0,
-                  int(k.shape[1]) if k is not None else 0, int(d),
-                  DTYPES[x.dtype], _lib.stream_of(dev))
-
-
-def _token_major(t):
-    return [0, 0, 0] if t is None else [t.stride(0), 0, t.stride(1)]
+    pos = _vector(rot, "positions", positions, T, _INDEX)
+    if T == 0:
+        return
+    _lib.launch(rot.index, "amass_rotary_write", _lib.ROTARY.pack(
+        qp, o[0], kp, vp, k_dst, v_dst, slots, pos, rot._freq, q_st, q_sh,
+        o[1], o[2], k_st, k_sh, v_st, v_sh, *kd, *vd, rot.mscale, nb, page,
+        positions.dtype == torch.int64, LAYOUTS[rot.layout], rot.rotary_dim,
+        T, H, n_kv, d, DTYPES[dtype], 0))
 
 
 def rotary_embed(rot, q, k, positions, *, q_out=None, k_out=None,
                  n_tokens=None) -> None:
     """Turn q (T, H, d) into ``q_out`` and k (T, n_kv, d) into ``k_out``
     (defaults: in place) for the first ``n_tokens`` tokens (default: all).
-    Either of q and k may be None."""
-    if q is None and q_out is not None or k is None and k_out is not None:
-        raise ValueError("an output without its input")
-    if q is not None and q_out is None:
-        q_out = q
+    Either of q and k may be None.  An output may be its input itself, but
+    must not overlap it in another way."""
+    x = q if q is not None else k
+    if x is None or (q is None and q_out is not None) or \
+            (k is None and k_out is not None):
+        raise ValueError("an output needs its input, and q or k must be given")
+    T = x.shape[0] if n_tokens is None else int(n_tokens)
+    kd, dst = (0, 0, 0), 0
     if k is not None:
-        if k_out is None:
-            k_out = k
-        if k_out.shape != k.shape or k_out.dtype != k.dtype or \
-                k_out.device != k.device or k_out.stride(-1) != 1:
-            raise ValueError("k_out must match k")
-    _launch(rot, q, q_out, k, None, k_out, None, None, 1, 1, positions,
-            n_tokens)
+        k_out = k if k_out is None else k_out
+        dst, st, sh, heads = _rows(rot, "k_out", k_out, x.dtype, T,
+                                   x.shape[-1])
+        if heads != k.shape[1]:
+            raise ValueError("k_out must have k's heads")
+        kd = (st, 0, sh)                 # one token a block, no slot mapping
+    _launch(rot, x, q, q if q_out is None else q_out, k, None, dst, kd, 0,
+            (0, 0, 0), 0, 1, 1, positions, T)
 
 
 def rotary_write_kv(rot, q, k, v, positions, kv_cache, slot_mapping, *,
@@ -210,31 +209,24 @@ def rotary_write_kv(rot, q, k, v, positions, kv_cache, slot_mapping, *,
     and copy v into the V half of ``kv_cache`` (either layout of
     ``attention.split_kv``; a K-only cache takes ``v=None``) at
     ``slot_mapping`` (int64, block * page + offset; slots outside the cache
-    are skipped).  k itself is left as it is.  Two tokens must not share a
-    slot.  bf16 or fp16, the cache's type."""
-    kc, vc = split_kv(kv_cache)
+    are skipped) for the first ``n_tokens`` tokens (default: all of k).  k
+    itself is left as it is.  Two tokens must not share a slot.  bf16 or
+    fp16, the cache's type."""
     if k is None:
         raise ValueError("rotary_write_kv needs k")
-    if (v is None) != (vc is None):
+    nb, page, n_kv, d, st, kc, vc = cache_layout(kv_cache)
+    if (v is None) != (not vc):
         raise ValueError("v and the cache's V half go together")
-    if kc.dtype != k.dtype or kc.device != rot.device or \
-            kc.stride(3) != 1 or kc.shape[2] != k.shape[1] or \
-            kc.shape[3] != k.shape[2]:
+    if kv_cache.dtype != k.dtype or kv_cache.get_device() != rot.index or \
+            k.shape[1:] != (n_kv, d):
         raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not fit the "
                          f"cache {tuple(kv_cache.shape)} {kv_cache.dtype}")
-    if q is not None and q_out is None:
-        q_out = q
     if q is None and q_out is not None:
         raise ValueError("q_out without q")
     T = k.shape[0] if n_tokens is None else int(n_tokens)
-    if slot_mapping.dtype != torch.int64 or \
-            slot_mapping.device != rot.device or slot_mapping.dim() != 1 or \
-            slot_mapping.shape[0] < T or \
-            (slot_mapping.shape[0] > 1 and slot_mapping.stride(0) != 1):
-        raise ValueError(f"slot_mapping must be a contiguous int64 vector of "
-                         f"at least {T} tokens on {rot.device}")
-    _launch(rot, q, q_out, k, v, kc, vc, slot_mapping, kc.shape[0],
-            kc.shape[1], positions, T)
+    slots = _vector(rot, "slot_mapping", slot_mapping, T, _INDEX[:1])
+    _launch(rot, k, q, q if q_out is None else q_out, k, v, kc, st, vc,
+            st if vc else (0, 0, 0), slots, nb, page, positions, T)
 
 
 __all__ = ["Rotary", "rotary_embed", "rotary_write_kv", "rotary_frequencies"]

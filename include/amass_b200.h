@@ -543,6 +543,23 @@ int amass_tier_decode_install(
  * engine does these.
  * ------------------------------------------------------------------------ */
 
+/* The buffers of a page pool of max_reqs rows (all device memory).  ticket
+ * must be 0 before the first call; the calls leave it 0. */
+typedef struct AmassPagePool {
+  int32_t* block_table;      /* (max_reqs, max_pages), rows bt_stride apart */
+  int32_t* seq_lens;         /* (max_reqs,) tokens of each row             */
+  int32_t* free_stack;       /* (num_blocks,)                              */
+  int32_t* free_top;         /* (1,) free blocks on the stack              */
+  int32_t* query_start_loc;  /* (max_reqs + 1,)                            */
+  int64_t* positions;        /* (max_tokens,)                              */
+  int64_t* slot_mapping;     /* (max_tokens,)                              */
+  int32_t* status;           /* (max_reqs,)                                */
+  int32_t* overflow;         /* (1,) latch                                 */
+  int32_t* ticket;           /* (1,)                                       */
+  int64_t bt_stride;
+  int32_t num_blocks, max_reqs, max_pages, max_tokens, page, reserved;
+} AmassPagePool;
+
 /* pages_begin -- one step's block allocation and token maps.  Request r in
  * [0, n_req) grows by max(new_tokens[r], 0) tokens; with old = seq_lens[r] it
  * needs ceil((old + new) / page) - ceil(old / page) blocks.  Requests are
@@ -556,28 +573,18 @@ int amass_tier_decode_install(
  * positions[t] = old + (t - query_start_loc[r]), slot_mapping[t] = block *
  * page + offset, or -1 when refused; behind the last token 0 and -1.
  * overflow[0] |= 1 (a status 1), 2 (a status 2), 4 (more than n_tokens new
- * tokens: the maps end there).  ticket: int32, 0 before the first call, left
- * 0.  One launch.  n_req <= 4096; the new tokens' sum fits int32. */
-int amass_pages_begin(const int32_t* new_tokens, int n_req,
-                      int32_t* block_table, int64_t bt_stride,
-                      int32_t* seq_lens, const int32_t* free_stack,
-                      int32_t* free_top, int num_blocks,
-                      int32_t* query_start_loc, int64_t* positions,
-                      int64_t* slot_mapping, int n_tokens, int32_t* status,
-                      int32_t* overflow, int32_t* ticket, int max_pages,
-                      int page, void* stream);
+ * tokens: the maps end there).  One launch.  max_reqs <= 4096; the new
+ * tokens' sum fits int32. */
+int amass_pages_begin(const AmassPagePool* pool, const int32_t* new_tokens,
+                      int n_req, int n_tokens, void* stream);
 
 /* pages_trim -- request r loses its last min(max(drop[r], 0), seq_lens[r])
  * tokens (whole = 0), or all of them where drop[r] != 0 (whole = 1).  Pages
  * left without a token return to free_stack and their table entries become
  * -1.  They are pushed last request and last page first, so a trim of what a
- * pages_begin granted restores the stack's order.  One launch.
- * n_req <= 4096. */
-int amass_pages_trim(const int32_t* drop, int whole, int n_req,
-                     int32_t* block_table, int64_t bt_stride,
-                     int32_t* seq_lens, int32_t* free_stack,
-                     int32_t* free_top, int num_blocks, int32_t* ticket,
-                     int max_pages, int page, void* stream);
+ * pages_begin granted restores the stack's order.  One launch. */
+int amass_pages_trim(const AmassPagePool* pool, const int32_t* drop,
+                     int n_req, int whole, void* stream);
 
 /* slot_map -- positions and slots of a step whose block table and lengths
  * exist: token t of request r (query_start_loc[r] <= t <
@@ -596,30 +603,55 @@ enum { AMASS_BF16 = 0, AMASS_FP16 = 1 };
  * (2i, 2i + 1) */
 enum { AMASS_ROTARY_HALF = 0, AMASS_ROTARY_INTERLEAVED = 1 };
 
+/* Arguments of amass_rotary_write; strides in elements. */
+typedef struct AmassRotary {
+  const void* q;             /* (n_tokens, H, d) or null                   */
+  void* q_out;               /* may be q                                   */
+  const void* k;             /* (n_tokens, n_kv, d) or null                */
+  const void* v;             /* (n_tokens, n_kv, d) or null                */
+  void* k_dst;               /* cache halves: block, row, head strides     */
+  void* v_dst;
+  const int64_t* slot_mapping;
+  const void* positions;     /* int64 (pos64 = 1) or int32                 */
+  const uint64_t* freq;      /* (rotary_dim / 2,)                          */
+  int64_t q_st, q_sh, qo_st, qo_sh, k_st, k_sh, v_st, v_sh;
+  int64_t kd_sb, kd_st, kd_sh, vd_sb, vd_st, vd_sh;
+  float mscale;
+  int32_t num_blocks, page, pos64, layout, rotary_dim, n_tokens, H, n_kv;
+  int32_t head_dim, dtype, reserved;
+} AmassRotary;
+
 /* rotary_write -- turns pair i of every head of q and k by the angle
  * positions[t] * f_i and scales it by mscale; elements from rotary_dim on
- * pass unchanged.  q (n_tokens, H, d) goes to q_out (which may be q); k and
- * v (n_tokens, n_kv, d) go to k_dst and v_dst at block slot / page, row
- * slot % page (element strides *_sb, *_st, *_sh), slot = slot_mapping[t];
- * slots outside [0, num_blocks * page) are skipped.  slot_mapping null:
- * slot = t (page 1: a token-major destination, which may be k itself).
- * Either of q and k may be null, v and v_dst may be null.  freq[i] =
- * f_i / (2 pi) as a 64-bit binary fraction of a turn (rotary_dim / 2 values;
- * the product with the position wraps, so no position is too far).
- * positions are int64 (pos64 = 1) or int32.  Products in fp32, one rounding.
- * head_dim <= 256 and rotary_dim <= head_dim, both even.  Two tokens must not
- * share a slot. */
-int amass_rotary_write(const void* q, int64_t q_st, int64_t q_sh, void* q_out,
-                       int64_t qo_st, int64_t qo_sh, const void* k,
-                       int64_t k_st, int64_t k_sh, const void* v,
-                       int64_t v_st, int64_t v_sh, void* k_dst, int64_t kd_sb,
-                       int64_t kd_st, int64_t kd_sh, void* v_dst,
-                       int64_t vd_sb, int64_t vd_st, int64_t vd_sh,
-                       const int64_t* slot_mapping, int num_blocks, int page,
-                       const void* positions, int pos64, const uint64_t* freq,
-                       float mscale, int layout, int rotary_dim, int n_tokens,
-                       int H, int n_kv, int head_dim, int dtype,
-                       void* stream);
+ * pass unchanged.  q goes to q_out; k and v go to k_dst and v_dst at block
+ * slot / page, row slot % page, slot = slot_mapping[t]; slots outside
+ * [0, num_blocks * page) are skipped.  slot_mapping null: slot = t (page 1: a
+ * token-major destination, which may be k itself).  freq[i] = f_i / (2 pi) as
+ * a 64-bit binary fraction of a turn (the product with the position wraps, so
+ * no position is too far).  Products in fp32, one rounding.  head_dim <= 256
+ * and rotary_dim <= head_dim, both even.  Two tokens must not share a slot. */
+int amass_rotary_write(const AmassRotary* args, void* stream);
+
+/* Arguments of amass_paged_chunk; strides in elements. */
+typedef struct AmassChunk {
+  const void* q;             /* (n_tokens, n_kv * G, d)                    */
+  const void* k;             /* block, token, head strides                 */
+  const void* v;
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  const int32_t* query_start_loc;
+  float* acc_part;           /* n_ctas * 2 * 256 * d, 16-byte aligned      */
+  float* ml_part;            /* n_ctas * 2 * 256 * 2, 16-byte aligned      */
+  int32_t* meta;             /* n_ctas * 4, 16-byte aligned                */
+  int32_t* fault;            /* (1,)                                       */
+  void* out;                 /* (n_tokens, n_kv * G, d)                    */
+  float* lse;                /* (n_tokens, n_kv * G) or null               */
+  int64_t q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+  int64_t bt_stride, o_st, o_sh;
+  float scale;
+  int32_t num_blocks, n_ctas, window, n_tokens, n_req, n_kv, G, head_dim;
+  int32_t page, max_pages, dtype;
+} AmassChunk;
 
 /* paged_chunk -- dense attention of a step's new tokens over the paged cache
  * (which already holds their keys and values): prefill chunks, single tokens
@@ -632,24 +664,14 @@ int amass_rotary_write(const void* q, int64_t q_st, int64_t q_sh, void* q_out,
  * lse (n_tokens, n_kv * G) fp32 or null: natural log of the row's sum of
  * exp(scale q.k), -inf without a key.  Cache slots behind a request's last
  * token may hold anything; block ids outside [0, num_blocks) read as zeros;
- * seq_lens is cut at max_pages * page.  Scratch for n_ctas CTAs (one per SM):
- * acc_part n_ctas * 2 * 256 * d fp32 and ml_part n_ctas * 2 * 256 * 2 fp32
- * (both 16-byte aligned), meta n_ctas * 4 int32; none needs to be set.  Calls
- * that overlap on the GPU need scratch of their own.  fault[0] becomes 1 when
- * a CTA gave up a bounded wait (its rows are then incomplete).
- * head_dim in {64, 128}, G <= 8, page = 16, n_req <= 4096, scale > 0; bases
- * 16-byte aligned, strides positive multiples of 8 elements.  Two launches;
- * the first call on a device sets a kernel attribute. */
-int amass_paged_chunk(
-    const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
-    int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb,
-    int64_t v_st, int64_t v_sh, int num_blocks, const int32_t* block_table,
-    int64_t bt_stride, const int32_t* seq_lens,
-    const int32_t* query_start_loc, float* acc_part, float* ml_part,
-    int32_t* meta, int n_ctas, int32_t* fault, void* out, int64_t o_stride_t,
-    int64_t o_stride_h, float* lse, float scale, int window, int n_tokens,
-    int n_req, int n_kv, int G, int head_dim, int page, int max_pages,
-    int dtype, void* stream);
+ * seq_lens is cut at max_pages * page.  The scratch (acc_part, ml_part, meta;
+ * n_ctas = the GPU's SM count) need not be set; calls that overlap on the GPU
+ * need scratch of their own.  fault[0] becomes 1 when a CTA gave up a bounded
+ * wait (its rows are then incomplete).  head_dim in {64, 128}, G <= 8, page =
+ * 16, n_req <= 4096, scale > 0; bases 16-byte aligned, strides positive
+ * multiples of 8 elements.  Two launches; the first call on a device sets a
+ * kernel attribute. */
+int amass_paged_chunk(const AmassChunk* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,7 +15,7 @@ CPU = torch.device("cpu")
 
 class Buf:
     """What paged_chunk_attention reads of its buffers."""
-    device, n_kv, G, d = CPU, 2, 4, 64
+    index, n_kv, G, d = -1, 2, 4, 64
 
 
 def chunk_args(**kw):
@@ -41,8 +41,8 @@ def chunk_args(**kw):
     (dict(seq_lens=torch.ones(3, dtype=torch.int32)), "cover"),
     (dict(query_start_loc=torch.zeros(2, dtype=torch.int32)), "cover"),
     (dict(block_table=torch.zeros(3, 2, dtype=torch.int32).t()),
-     "contiguous last"),
-    (dict(block_table=torch.zeros(2, 0, dtype=torch.int32)), "no columns"),
+     "contiguous in the last"),
+    (dict(block_table=torch.zeros(2, 0, dtype=torch.int32)), "cover"),
     (dict(window=0), "window"), (dict(scale=0.0), "scale"),
     (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
     (dict(lse=torch.zeros(5, 4)), "lse"),
@@ -58,22 +58,23 @@ def test_chunk_refuses(kw, match):
 
 def test_chunk_c_entry_refuses():
     lib = _lib.load()
-    one = ctypes.c_void_p(64)
 
     def call(**kw):
-        a = dict(q=one, k=one, page=16, d=128, G=4, T=4, R=1, scale=0.1,
-                 window=0, dtype=0, ksh=128, nb=3, mp=4, fault=one)
+        a = dict(q=64, k=64, page=16, d=128, G=4, T=4, R=1, scale=0.1,
+                 window=0, dtype=0, ksh=128, nb=3, mp=4, fault=64)
         a.update(kw)
-        return lib.amass_paged_chunk(
-            a["q"], 512, 128, a["k"], 4096, 256, a["ksh"], one, 4096, 256,
-            128, a["nb"], one, 4, one, one, one, one, one, 8, a["fault"], one,
-            512, 128, None, ctypes.c_float(a["scale"]), a["window"], a["T"],
-            a["R"], 2, a["G"], a["d"], a["page"], a["mp"], a["dtype"], None)
+        return lib.amass_paged_chunk(_lib.CHUNK.pack(
+            a["q"], a["k"], 64, 64, 64, 64, 64, 64, 64, a["fault"], 64, 0,
+            1024, 128, 4096, 256, a["ksh"], 4096, 256, 128, 4, 1024, 128,
+            a["scale"], a["nb"], 8, a["window"], a["T"], a["R"], 2, a["G"],
+            a["d"], a["page"], a["mp"], a["dtype"]), None)
+    assert lib.amass_paged_chunk(None, None) == 1
+    assert lib.amass_rotary_write(None, None) == 1
     assert call(T=0) == 0 and call(R=0) == 0
-    for kw in (dict(q=None), dict(fault=None), dict(T=-1), dict(scale=0.0),
+    for kw in (dict(q=0), dict(fault=0), dict(T=-1), dict(scale=0.0),
                dict(scale=float("nan")), dict(window=-1), dict(dtype=2),
                dict(ksh=100), dict(ksh=-128), dict(nb=0), dict(mp=0),
-               dict(k=ctypes.c_void_p(24))):
+               dict(k=24)):
         assert call(**kw) == 1, kw
     for kw in (dict(d=96), dict(G=9), dict(page=32), dict(R=4097)):
         assert call(**kw) == 2, kw
@@ -103,12 +104,14 @@ def test_pool_refuses():
     with pytest.raises(RuntimeError, match="outgrew.*n_tokens"):
         p.check()
     lib = _lib.load()
-    assert lib.amass_pages_trim(None, 0, 0, None, 0, None, ctypes.c_void_p(8),
-                                ctypes.c_void_p(8), 4, ctypes.c_void_p(8), 3,
-                                16, None) == 0
-    assert lib.amass_pages_trim(None, 0, 1, None, 0, None, ctypes.c_void_p(8),
-                                ctypes.c_void_p(8), 4, ctypes.c_void_p(8), 3,
-                                16, None) == 1
+    assert lib.amass_pages_begin(None, None, 0, 0, None) == 1
+    assert lib.amass_pages_trim(None, None, 0, 0, None) == 1
+    assert lib.amass_pages_trim(p._pool, None, 0, 0, None) == 0
+    assert lib.amass_pages_trim(p._pool, None, 1, 0, None) == 1
+    assert lib.amass_pages_begin(p._pool, ctypes.c_void_p(8), 3, 0, None) == 1
+    assert lib.amass_pages_begin(p._pool, None, 0, 10, None) == 1
+    with pytest.raises(AttributeError, match="fixed"):
+        p.block_table = torch.zeros(2, 3, dtype=torch.int32)
 
 
 def test_slot_map_refuses():
