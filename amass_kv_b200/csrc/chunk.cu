@@ -44,6 +44,7 @@ constexpr int kPg = 16;                  // tokens of a page
 constexpr int kChMaxReq = 4096;
 constexpr int kMinUnits = 2;             // key tiles a run has at least
 constexpr float kRescaleLog2 = 8.f;
+constexpr int kPart = 96;                // keys whose weights go to O first
 
 struct ChunkArgs {
   const int32_t* bt;
@@ -131,6 +132,49 @@ AMASS_DEV void tc_st32(uint32_t t, const uint32_t* r) {
          "r"(r[31])
       : "memory");
 }
+AMASS_DEV void tc_ld16(uint32_t* r, uint32_t t) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]),
+        "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15])
+      : "r"(t));
+}
+AMASS_DEV void tc_st16(uint32_t t, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      :: "r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+         "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// two fp32 lanes at once
+AMASS_DEV uint64_t f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+AMASS_DEV void f2_get(uint64_t x, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
+}
+AMASS_DEV uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+AMASS_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+AMASS_DEV uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 AMASS_DEV void tma_3d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x,
                       int y, int z) {
   asm volatile(
@@ -216,13 +260,52 @@ struct ChSeg {
   int r, h, q0, tok0, ntok, off, sl, t0, n, left;
   bool first, last;
 };
-// walks the segments of a CTA's run; every role keeps its own copy
-struct ChWalk {
-  int r, h, i, uoff;
-  int rem;
+struct ChPlan {
   ChReq q;
-  AMASS_DEV bool next(const ChunkArgs& a, ChSeg& s) {
-    if (rem <= 0 || r >= a.n_req) return false;
+  int r, h, i, uoff, rem, share;
+  long long u1;
+};
+
+// Walks the segments of a CTA's run; every role keeps its own copy.  A first
+// segment that starts inside its item goes last: then every CTA starts at its
+// item's first key tile, and since the runs are equally long the late pieces
+// of one head's items meet at the same key tiles again.  CTAs of a head so
+// stream its K and V together and read them from L2 (2048 rows behind 64K
+// tokens: DRAM would have to deliver 64 KB per CTA and unit otherwise).
+struct ChWalk {
+  ChReq q;
+  int r, h, i, uoff, rem, late;          // late: units of the deferred segment
+  AMASS_DEV void start(const ChunkArgs& a, const ChPlan& p) {
+    q = p.q; r = p.r; h = p.h; i = p.i; uoff = p.uoff; rem = p.rem;
+    late = 0;
+    if (uoff > 0 && rem > 0) {
+      int lo;
+      const int n = min(rem, ch_tiles(a, q, i, &lo) - uoff);
+      if (n < rem) {
+        late = n;
+        rem -= n;
+        uoff = 0;
+        step(a);
+      }
+    }
+  }
+  AMASS_DEV void step(const ChunkArgs& a) {
+    if (++i < q.nt) return;
+    i = 0;
+    if (++h < a.n_kv) return;
+    h = 0;
+    if (rem <= 0) return;
+    do {
+      if (++r >= a.n_req) break;
+      q = ch_req(a, r);
+    } while (q.nt == 0);
+  }
+  AMASS_DEV bool next(const ChunkArgs& a, const ChPlan& p, ChSeg& s) {
+    if (rem <= 0 || r >= a.n_req) {
+      if (late == 0) return false;
+      q = p.q; r = p.r; h = p.h; i = p.i; uoff = p.uoff; rem = late;
+      late = 0;
+    }
     const int tl = a.tm_log2 + 1;
     int lo;
     const int nu = ch_tiles(a, q, i, &lo);
@@ -236,25 +319,9 @@ struct ChWalk {
     s.last = s.left == 0;
     rem -= s.n;
     uoff = 0;
-    if (++i >= q.nt) {
-      i = 0;
-      if (++h >= a.n_kv) {
-        h = 0;
-        if (rem > 0) {
-          do {
-            if (++r >= a.n_req) break;
-            q = ch_req(a, r);
-          } while (q.nt == 0);
-        }
-      }
-    }
+    step(a);
     return true;
   }
-};
-
-struct ChPlan {
-  int r, h, i, uoff, rem, share;
-  long long u1;
 };
 
 // this CTA's run of the flat unit list
@@ -263,10 +330,12 @@ AMASS_DEV void ch_plan(const ChunkArgs& a, ChPlan* out) {
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int per = (a.n_req + kChThreads - 1) / kChThreads;
   const int r0 = min(a.n_req, tid * per), r1 = min(a.n_req, r0 + per);
-  long long mine = 0;
+  long long mine = 0, units = 0;
+  ChReq q;
   for (int r = r0; r < r1; ++r) {
-    const ChReq q = ch_req(a, r);
-    mine += ch_units(a, q, q.nt) * a.n_kv;
+    q = ch_req(a, r);
+    units = ch_units(a, q, q.nt);
+    mine += units * a.n_kv;
   }
   long long incl = mine;
 #pragma unroll
@@ -290,19 +359,24 @@ AMASS_DEV void ch_plan(const ChunkArgs& a, ChPlan* out) {
   if (u0 >= before && u0 < before + mine) {
     u0 -= before;
     for (int r = r0; r < r1; ++r) {
-      const ChReq q = ch_req(a, r);
-      const long long s = ch_units(a, q, q.nt);
-      if (u0 >= s * a.n_kv) {
-        u0 -= s * a.n_kv;
+      if (per > 1) {                     // one request: still in registers
+        q = ch_req(a, r);
+        units = ch_units(a, q, q.nt);
+      }
+      const long long all = units * a.n_kv;
+      if (u0 >= all) {
+        u0 -= all;
         continue;
       }
-      const int h = (int)(u0 / s);
-      u0 -= h * s;
+      const int h = all >> 32 ? (int)(u0 / units)
+                              : (int)((uint32_t)u0 / (uint32_t)units);
+      u0 -= h * units;
       int lo = 0, hi = q.nt;             // last item that starts at or before
       while (hi - lo > 1) {
         const int m = (lo + hi) >> 1;
         if (ch_units(a, q, m) <= u0) lo = m; else hi = m;
       }
+      out->q = q;
       out->r = r;
       out->h = h;
       out->i = lo;
@@ -335,16 +409,11 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   using X = ChShape<D>;
   constexpr int NS = X::kStages;
   extern __shared__ uint8_t dyn[];
-  __shared__ __align__(8) uint64_t bars[2 * NS + 10];
+  __shared__ __align__(8) uint64_t bars[2 * NS + 14];
+  __shared__ float2 ml_s[128];           // warpgroup 1's (m, l), one-tile items
   __shared__ ChPlan plan;
   __shared__ uint32_t tmem_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-  grid_dep_wait();
-  grid_dep_launch();
-  ch_plan(a, &plan);
-  if (tid == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-  if (plan.rem <= 0) return;
 
   const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
   const uint32_t q_s = base, ring = base + 2 * X::kTile;
@@ -353,7 +422,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   const auto empty = [&](int s) { return b0 + 8u * (NS + s); };
   const uint32_t q_full = b0 + 8u * (2 * NS), q_empty = q_full + 8;
   const uint32_t s_full = q_full + 16, p_full = q_full + 32;   // two each
-  const uint32_t o_full = q_full + 48, v_tmp = q_full + 64, drain = v_tmp + 8;
+  const uint32_t o_full = q_full + 48, p_part = q_full + 64;   // two each
+  const uint32_t v_tmp = q_full + 80, drain = v_tmp + 8;
+  const uint32_t pair = v_tmp + 16, pair_done = v_tmp + 24;
 
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
@@ -364,11 +435,14 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
     mbar_init(q_empty, 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full + 8 * t, 1);
+      mbar_init(p_part + 8 * t, 4);
       mbar_init(p_full + 8 * t, 4);
       mbar_init(o_full + 8 * t, 1);
     }
     mbar_init(v_tmp, 1);
     mbar_init(drain, 1);
+    mbar_init(pair, 4);
+    mbar_init(pair_done, 4);
     mbar_init_fence();
   }
   if (warp == 9) {
@@ -377,10 +451,14 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
         :: "r"(smem_u32(&tmem_s)), "r"(X::kCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  // the predecessor's memory is read from here on
+  grid_dep_wait();
+  grid_dep_launch();
   tc_before();
-  __syncthreads();
+  ch_plan(a, &plan);                     // ends with a barrier
   tc_after();
   const uint32_t tmem = tmem_s;
+  if (tid == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
 
   // bounded wait: after about a second the CTA records the fault and unwinds
   const auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
@@ -394,9 +472,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   };
 
   ChWalk wk;
-  wk.r = plan.r; wk.h = plan.h; wk.i = plan.i; wk.uoff = plan.uoff;
-  wk.rem = plan.rem;
-  wk.q = ch_req(a, plan.r);
+  wk.start(a, plan);
   ChSeg sg;
 
   // a softmax thread holds a row of 128 scores: 384 * 168 registers at launch
@@ -406,23 +482,23 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
     // ------------------------------------------------------------- softmax
     const int t = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + t * 128 + lanes, to = tmem + X::kO + t * D +
-                                                     lanes;
-    const int tok = row / a.G, g = row - tok * a.G;
+    const uint32_t ts = tmem + t * 128 + lanes;
+    const uint32_t to = tmem + X::kO + t * D + lanes;
+    const int tok = row / a.G, g = row - tok * a.G, tm = 1 << a.tm_log2;
     const float sl2 = a.scale_log2;
-    uint32_t sph = 0, oph = 0;
+    const uint64_t sl2x2 = f2(sl2, sl2);
+    uint32_t sph = 0, oph = 0, cph = 0;
     bool ok = true;
-    while (ok && wk.next(a, sg)) {
-      const int tm = 1 << a.tm_log2;
-      if (t == 1 && sg.ntok <= tm) continue;
-      const int it = t * tm + tok;               // token within the item
+    while (ok && wk.next(a, plan, sg)) {
+      const bool two = sg.ntok > tm;
+      const int it = (two ? t * tm : 0) + tok;   // token within the item
       const bool valid = tok < tm && it < sg.ntok;
       const int pos = sg.off + sg.tok0 + it;
       const int khi = valid ? max(pos + 1, 0) : 0;
       const int klo = a.window ? max(pos - a.window + 1, 0) : 0;
       const bool live = __any_sync(~0u, valid);
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < sg.n; ++j) {
+      for (int j = two ? 0 : t; j < sg.n; j += two ? 1 : 2) {
         if (!(ok = wait_warp(s_full + 8 * t, sph))) break;
         sph ^= 1;
         tc_after();
@@ -438,96 +514,163 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
             for (int c = 0; c < 128; ++c)
               if (c >= e || c < b) s[c] = 0xff800000u;
           }
-          float mx = __uint_as_float(s[0]);
+          float x4[4];
 #pragma unroll
-          for (int c = 1; c < 128; ++c)
-            mx = fmaxf(mx, __uint_as_float(s[c]));
-          if (j == 0) {
+          for (int c = 0; c < 4; ++c) x4[c] = __uint_as_float(s[c]);
+#pragma unroll
+          for (int c = 4; c < 124; c += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              x4[e] = fmaxf(fmaxf(x4[e], __uint_as_float(s[c + e])),
+                            __uint_as_float(s[c + 4 + e]));
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            x4[c] = fmaxf(x4[c], __uint_as_float(s[124 + c]));
+          const float mx = fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3]));
+          if (j < 2 - (two ? 1 : 0)) {           // this warpgroup's first tile
             m = mx;
           } else if (__any_sync(~0u, (mx - m) * sl2 > kRescaleLog2)) {
             const float mn = fmaxf(m, mx);
             const float f = m == -INFINITY ? 0.f : ex2_approx((m - mn) * sl2);
             l *= f;
             m = mn;
-#pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tc_ld32(o, to + c);
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tc_ld16(o, to + c);
               tc_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
+              for (int e = 0; e < 16; ++e)
                 o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tc_st32(to + c, o);
+              tc_st16(to + c, o);
             }
           }
           const float nm = m == -INFINITY ? 0.f : -m * sl2;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t nm2 = f2(nm, nm);
+          uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
           for (int c = 0; c < 128; c += 2) {
-            const float p0 = ex2_approx(fmaf(__uint_as_float(s[c]), sl2, nm));
-            const float p1 =
-                ex2_approx(fmaf(__uint_as_float(s[c + 1]), sl2, nm));
-            sum[(c >> 1) & 3] += p0 + p1;
+            float p0, p1;
+            f2_get(f2_fma(f2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])),
+                          sl2x2, nm2), p0, p1);
+            p0 = ex2_approx(p0);
+            p1 = ex2_approx(p1);
+            sum[(c >> 1) & 1] = f2_add(sum[(c >> 1) & 1], f2(p0, p1));
             s[c >> 1] = kF16 ? pack_h2(p0, p1) : pack_bf2(p0, p1);
+            if (c + 2 == kPart) {                // the MMA may start
+              tc_st32(ts, s);
+              tc_st16(ts + 32, s + 32);
+              tc_wait_st();
+              tc_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(p_part + 8 * t);
+            }
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tc_st32(ts, s);
-          tc_st32(ts + 32, s + 32);
+          tc_st16(ts + kPart / 2, s + kPart / 2);
+          float a0, a1;
+          f2_get(f2_add(sum[0], sum[1]), a0, a1);
+          l += a0 + a1;
           tc_wait_st();
+        } else if (lane == 0) {
+          mbar_arrive(p_part + 8 * t);
         }
         tc_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + 8 * t);
       }
       if (!ok) break;
-      if (!(ok = wait_warp(o_full + 8 * t, oph))) break;
-      oph ^= 1;
-      tc_after();
-      if (!live) continue;
+      const bool paired = !two && sg.n > 1;      // both hold part of the rows
+      if (t == 0 || two || paired) {
+        if (!(ok = wait_warp(o_full + 8 * t, oph))) break;
+        oph ^= 1;
+        tc_after();
+      }
+      if (!two && t == 1) {
+        if (!paired) continue;
+        ml_s[row] = make_float2(m, l);
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pair);
+        // warpgroup 0 reads O_1 and ml_s until then
+        if (!(ok = wait_warp(pair_done, cph))) break;
+        cph ^= 1;
+        continue;
+      }
+      float f0 = 1.f, f1 = 0.f;
+      if (paired) {
+        if (!(ok = wait_warp(pair, cph))) break;
+        cph ^= 1;
+        tc_after();
+        const float2 o = ml_s[row];
+        const float mn = fmaxf(m, o.x), ref = mn == -INFINITY ? 0.f : mn;
+        f0 = ex2_approx((m - ref) * sl2);
+        f1 = ex2_approx((o.x - ref) * sl2);
+        l = l * f0 + o.y * f1;
+        m = mn;
+      }
       const bool whole = sg.first && sg.last;
       const int slot = sg.first ? 1 : 0;
       const int64_t part = (int64_t)blockIdx.x * 2 + slot;
-      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      const bool some = l > 0.f || l != l;
+      const float inv = !whole ? 1.f : some ? 1.f / l : 0.f;
+      f0 *= inv;
+      f1 *= inv;
       const int token = sg.q0 + sg.tok0 + it;
       char* orow = (char*)a.out + 2 * ((int64_t)token * a.o_st +
                                        (int64_t)(sg.h * a.G + g) * a.o_sh);
+      float4* prow = reinterpret_cast<float4*>(a.acc) + part * (D / 4) * 256 +
+                     (two ? t : 0) * 128 + row;
+      if (live) {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          uint32_t o[16];
+          tc_ld16(o, to + c);
+          tc_wait_ld();
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
-        uint32_t o[32];
-        tc_ld32(o, to + c);
-        tc_wait_ld();
-        if (!valid) continue;
-        if (whole) {
+          for (int e = 0; e < 16; ++e)
+            o[e] = __float_as_uint(__uint_as_float(o[e]) * f0);
+          if (paired) {
+            uint32_t o1[16];
+            tc_ld16(o1, to + D + c);
+            tc_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint32_t w[4];
+            for (int e = 0; e < 16; ++e)
+              o[e] = __float_as_uint(fmaf(__uint_as_float(o1[e]), f1,
+                                          __uint_as_float(o[e])));
+          }
+          if (valid && whole) {
+            uint32_t w[8];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float lo = __uint_as_float(o[e + 2 * x]) * inv;
-              const float hi = __uint_as_float(o[e + 2 * x + 1]) * inv;
+            for (int x = 0; x < 8; ++x) {
+              const float lo = __uint_as_float(o[2 * x]);
+              const float hi = __uint_as_float(o[2 * x + 1]);
               w[x] = kF16 ? pack_h2(lo, hi) : pack_bf2(lo, hi);
             }
-            *reinterpret_cast<uint4*>(orow + 2 * (c + e)) =
-                make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        } else {
-          float4* p = reinterpret_cast<float4*>(a.acc) +
-                      (part * (D / 4) + c / 4) * 256 + t * 128 + row;
+            uint4* d = reinterpret_cast<uint4*>(orow + 2 * c);
+            d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          } else if (valid) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            p[(e / 4) * 256] = make_float4(
-                __uint_as_float(o[e]), __uint_as_float(o[e + 1]),
-                __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+            for (int e = 0; e < 16; e += 4)
+              prow[(c + e) / 4 * 256] = make_float4(
+                  __uint_as_float(o[e]), __uint_as_float(o[e + 1]),
+                  __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+          }
+          __syncwarp();
+        }
+        if (valid) {
+          const float ms = m == -INFINITY ? m : m * sl2;
+          if (!whole)
+            a.ml[part * 256 + (two ? t : 0) * 128 + row] = make_float2(ms, l);
+          else if (a.lse)
+            a.lse[(int64_t)token * (a.n_kv * a.G) + sg.h * a.G + g] =
+                some ? (ms + log2f(l)) * 0.6931471805599453f : -INFINITY;
         }
       }
-      if (valid) {
-        const float ms = m == -INFINITY ? m : m * sl2;
-        if (!whole)
-          a.ml[part * 256 + t * 128 + row] = make_float2(ms, l);
-        else if (a.lse)
-          a.lse[(int64_t)token * (a.n_kv * a.G) + sg.h * a.G + g] =
-              l > 0.f || l != l ? (ms + log2f(l)) * 0.6931471805599453f
-                                : -INFINITY;
+      if (paired) {
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pair_done);
       }
       if (!whole && sg.first && tid == 0) {
         // the CTAs behind this one that hold the rest of the item
@@ -544,7 +687,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       int st = 0, issued = 0;
       uint32_t ph = 1, qph = 1;
       bool ok = true;
-      while (ok && wk.next(a, sg)) {
+      while (ok && wk.next(a, plan, sg)) {
         const int tm = 1 << a.tm_log2;
         if (!(ok = wait_warp(q_empty, qph))) break;
         qph ^= 1;
@@ -614,71 +757,96 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       if (lane == 0) {
         constexpr uint32_t id_s = mma_idesc(kF16, false, kKeys);
         constexpr uint32_t id_o = mma_idesc(kF16, true, D);
-        int st = 0;
-        uint32_t ph = 0, qph = 0, pph = 0;
+        uint32_t seq = 0, qph = 0, pph = 0;
         bool ok = true;
-        const auto scores = [&](int t, int s) {
-          const uint32_t qa = q_s + t * X::kTile, ka = ring + s * X::kTile;
-  #pragma unroll
+        // K of tile j is the ring's entry seq + 2 j, V the one behind it
+        const auto stage = [&](uint32_t n) { return (int)(n % NS); };
+        const auto arrived = [&](uint32_t n) {
+          return wait(full(stage(n)), (n / NS) & 1);
+        };
+        const auto scores = [&](int t, int qt, uint32_t n) {
+          const uint32_t qa = q_s + qt * X::kTile;
+          const uint32_t ka = ring + stage(n) * X::kTile;
+#pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t o = (k >> 2) * X::kPanel + (k & 3) * 32;
             mma_ss(tmem + t * 128, smem_desc(qa + o, 16, 1024),
                    smem_desc(ka + o, 16, 1024), id_s, k > 0);
           }
+          mma_commit(s_full + 8 * t);
         };
-        const auto product = [&](int t, int s, bool acc) {
-          const uint32_t va = ring + s * X::kTile;
-  #pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
+        // O_t += P_t V, the first keys of the tile as soon as their weights
+        // are there
+        const auto product = [&](int t, uint32_t n, bool acc) -> bool {
+          const uint32_t va = ring + stage(n) * X::kTile, p = (pph >> t) & 1;
+          pph ^= 1u << t;
+          if (!wait(p_part + 8 * t, p)) return false;
+          tc_after();
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k) {
+            if (k == kPart / 16) {
+              if (!wait(p_full + 8 * t, p)) return false;
+              tc_after();
+            }
             mma_ts(tmem + X::kO + t * D, tmem + t * 128 + k * 8,
                    smem_desc(va + k * 2048, X::kPanel, 1024), id_o,
                    acc || k > 0);
+          }
+          return true;
         };
-        const auto step = [&](int& s, uint32_t& p) {
-          if (++s == NS) { s = 0; p ^= 1; }
-        };
-        while (ok && wk.next(a, sg)) {
-          const int nt = sg.ntok > (1 << a.tm_log2) ? 2 : 1;
+        while (ok && wk.next(a, plan, sg)) {
+          const bool two = sg.ntok > (1 << a.tm_log2);
+          const int n = sg.n;
           if (!(ok = wait(q_full, qph))) break;
           qph ^= 1;
-          if (!(ok = wait(full(st), ph))) break;
+          if (!(ok = arrived(seq))) break;
           tc_after();
-          for (int t = 0; t < nt; ++t) {
-            scores(t, st);
-            mma_commit(s_full + 8 * t);
-          }
-          mma_commit(empty(st));
-          if (sg.n == 1) mma_commit(q_empty);
-          step(st, ph);
-          for (int j = 0; ok && j < sg.n; ++j) {
-            const int sv = st;
-            if (!(ok = wait(full(st), ph))) break;
-            step(st, ph);
-            const int sk = st;
-            const bool more = j + 1 < sg.n;
-            if (more) {
-              if (!(ok = wait(full(st), ph))) break;
-              step(st, ph);
+          scores(0, 0, seq);
+          if (two) scores(1, 1, seq);
+          mma_commit(empty(stage(seq)));
+          if (two) {
+            if (n == 1) mma_commit(q_empty);
+            for (int j = 0; ok && j < n; ++j) {
+              const uint32_t v = seq + 2 * j + 1, k = v + 1;
+              const bool more = j + 1 < n;
+              ok = arrived(v) && (!more || arrived(k));
+              for (int t = 0; ok && t < 2; ++t) {
+                if (!(ok = product(t, v, j > 0))) break;
+                if (more) scores(t, t, k);
+                else mma_commit(o_full + 8 * t);
+              }
+              if (!ok) break;
+              mma_commit(empty(stage(v)));
+              if (more) mma_commit(empty(stage(k)));
+              if (j + 2 == n) mma_commit(q_empty);
             }
-            for (int t = 0; t < nt; ++t) {
-              if (!(ok = wait(p_full + 8 * t, (pph >> t) & 1))) break;
-              pph ^= 1u << t;
+          } else {
+            // one row tile: the two warpgroups take its key tiles in turn
+            if (n > 1) {
+              if (!(ok = arrived(seq + 2))) break;
               tc_after();
-              product(t, sv, j > 0);
+              scores(1, 0, seq + 2);
+              mma_commit(empty(stage(seq + 2)));
+            }
+            if (n <= 2) mma_commit(q_empty);
+            for (int j = 0; j < n; ++j) {
+              const uint32_t v = seq + 2 * j + 1, k = v + 3;
+              const int t = j & 1;
+              const bool more = j + 2 < n;
+              ok = arrived(v) && (!more || arrived(k)) &&
+                   product(t, v, j > 1);
+              if (!ok) break;
+              mma_commit(empty(stage(v)));
               if (more) {
-                scores(t, sk);
-                mma_commit(s_full + 8 * t);
+                scores(t, 0, k);
+                mma_commit(empty(stage(k)));
               } else {
                 mma_commit(o_full + 8 * t);
               }
-            }
-            if (!ok) break;
-            mma_commit(empty(sv));
-            if (more) {
-              mma_commit(empty(sk));
-              if (j + 2 == sg.n) mma_commit(q_empty);
+              if (j + 3 == n) mma_commit(q_empty);
             }
           }
+          seq += 2 * n;
         }
         // every MMA and its arrivals end before the CTA does
         mma_commit(drain);
