@@ -231,6 +231,11 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
             min(k_sb, k_st, k_sh, v_sb, v_st, v_sh) <= 0:
         raise ValueError("q, kv_cache and out must be 16-byte aligned, with "
                          "strides that are positive multiples of 8 elements")
+    if n_kv > 1 and nb > 1 and (
+            k_sb % k_sh or v_sb % v_sh or k_sb // k_sh != v_sb // v_sh or
+            k_sb < n_kv * k_sh):
+        raise ValueError("kv_cache needs block strides that are multiples of "
+                         "the head strides, the same for K and V")
     check_i32(dev, "block_table", block_table, 2)
     check_i32(dev, "seq_lens", seq_lens, 1)
     check_i32(dev, "query_start_loc", query_start_loc, 1)

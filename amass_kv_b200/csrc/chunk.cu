@@ -11,8 +11,10 @@
 // -- two softmax warpgroups, one tile each -- against 128-key tiles.
 //
 //   warps 0-3, 4-7  softmax of row tile 0, 1: one thread per row
-//   warp 8          TMA producer: Q, then K and V tiles page by page (a 16-row
-//                   box per page and 64-column panel) into a ring
+//   warp 8          TMA producer: Q, then K and V tiles into a ring, one copy
+//                   a page (a copy takes some 80-100 cycles of the TMA unit
+//                   whatever its size: at one per page and 64 columns K and V
+//                   came at 26 bytes a cycle, the tensor core wants 32)
 //   warp 9          issues the tcgen05 MMAs: S = Q K^T (both operands in
 //                   shared memory, fp32 S in TMEM), O += P V (P in TMEM over
 //                   S's columns, V as a column-major operand, fp32 O in TMEM)
@@ -42,7 +44,10 @@ constexpr int kChThreads = 384;          // three warpgroups (two idle warps)
 constexpr int kKeys = 128;               // keys of a tile
 constexpr int kPg = 16;                  // tokens of a page
 constexpr int kChMaxReq = 4096;
-constexpr int kMinUnits = 2;             // key tiles a run has at least
+// cost of an item, for equal runs: a key tile of two row tiles (3300 cycles,
+// softmax bound), of one row tile (2100, its loads), and what an item adds
+// (query load, first scores, output)
+constexpr int kCost2 = 3, kCost1 = 2, kCostItem = 6, kMinRun = 4;
 constexpr float kRescaleLog2 = 8.f;
 constexpr int kPart = 96;                // keys whose weights go to O first
 
@@ -60,6 +65,7 @@ struct ChunkArgs {
   int32_t* fault;
   float scale_log2;
   int n_req, n_kv, G, T, max_pages, nb, window, tm_log2;
+  int bh;                                // head rows from block to block
 };
 
 // ------------------------------------------------------------ tcgen05 / TMA
@@ -151,6 +157,11 @@ AMASS_DEV void tc_st16(uint32_t t, const uint32_t* r) {
          "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+AMASS_DEV float fmax_nan(float a, float b) {   // NaN when either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 // two fp32 lanes at once
 AMASS_DEV uint64_t f2(float lo, float hi) {
   uint64_t r;
@@ -170,11 +181,6 @@ AMASS_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-AMASS_DEV uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 AMASS_DEV void tma_3d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x,
                       int y, int z) {
   asm volatile(
@@ -182,13 +188,12 @@ AMASS_DEV void tma_3d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x,
       "complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
       :: "r"(dst), "l"(m), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
-AMASS_DEV void tma_4d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x,
-                      int y, int z, int w) {
+AMASS_DEV void tma_5d(uint32_t dst, const CUtensorMap* m, uint32_t bar,
+                      int w) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::"
-      "complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-      :: "r"(dst), "l"(m), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
-      : "memory");
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::"
+      "complete_tx::bytes [%0], [%1, {%2, %2, %2, %2, %3}], [%4];"
+      :: "r"(dst), "l"(m), "r"(0), "r"(w), "r"(bar) : "memory");
 }
 
 // ------------------------------------------------------------- work list ---
@@ -236,106 +241,118 @@ AMASS_DEV int64_t floor_sum(int64_t b, int64_t i0, int64_t i1, int tl) {
   const int64_t c = b >> tl;
   return shift_sum(i1 + c, 7 - tl) - shift_sum(i0 + c, 7 - tl);
 }
-// units of items 0 .. m - 1 of the request (closed form of ch_tiles' sum)
-AMASS_DEV int64_t ch_units(const ChunkArgs& a, const ChReq& q, int m) {
+// cost of one key tile of item i
+AMASS_DEV int ch_weight(const ChunkArgs& a, const ChReq& q, int i) {
+  return q.ql - (i << (a.tm_log2 + 1)) > (1 << a.tm_log2) ? kCost2 : kCost1;
+}
+// cost of items 0 .. m - 1 of the request (closed form of ch_tiles' sum)
+AMASS_DEV int64_t ch_cost(const ChunkArgs& a, const ChReq& q, int m) {
   const int tl = a.tm_log2 + 1;
   if (m <= 0) return 0;
-  int64_t s = 0;
+  int64_t s = (int64_t)m * kCostItem;
   int full = m;
   if (m == q.nt) {                       // the last item may be short
     int lo;
-    s = ch_tiles(a, q, m - 1, &lo);
+    s += (int64_t)ch_tiles(a, q, m - 1, &lo) * ch_weight(a, q, m - 1);
     full = m - 1;
   }
   // items whose last position is negative visit one (empty) tile
   const int none = q.off < 0 ? min(full, (-q.off) >> tl) : 0;
-  s += none;
-  s += floor_sum((int64_t)q.off + (1 << tl) + kKeys - 1, none, full, tl);
+  int64_t u = none + floor_sum((int64_t)q.off + (1 << tl) + kKeys - 1, none,
+                               full, tl);
   if (a.window)
-    s -= floor_sum((int64_t)q.off - a.window + 1, none, full, tl);
-  return s;
+    u -= floor_sum((int64_t)q.off - a.window + 1, none, full, tl);
+  return s + u * kCost2;
 }
 
 struct ChSeg {
-  int r, h, q0, tok0, ntok, off, sl, t0, n, left;
+  int r, h, q0, tok0, ntok, off, sl, t0, n, parts;
   bool first, last;
 };
 struct ChPlan {
   ChReq q;
-  int r, h, i, uoff, rem, share;
-  long long u1;
+  int r, h, i, from, to, share;          // run [from, to) from item i's start
+  long long end;                         // its end in the whole list
 };
 
-// Walks the segments of a CTA's run; every role keeps its own copy.  A first
-// segment that starts inside its item goes last: then every CTA starts at its
-// item's first key tile, and since the runs are equally long the late pieces
-// of one head's items meet at the same key tiles again.  CTAs of a head so
-// stream its K and V together and read them from L2 (2048 rows behind 64K
-// tokens: DRAM would have to deliver 64 KB per CTA and unit otherwise).
+// Walks the segments of a CTA's run; every role keeps its own copy.  Key tile
+// k of an item belongs to the CTA whose run holds its place, item start + k *
+// weight.  A first segment that starts inside its item goes last: then every
+// CTA starts at its item's first key tile, and since the runs are equally
+// long the late pieces of one head's items meet at the same key tiles again.
+// CTAs of a head so stream its K and V together and find them in L2 (2048
+// rows behind 64K tokens: 2290 -> 1920 us).
 struct ChWalk {
   ChReq q;
-  int r, h, i, uoff, rem, late;          // late: units of the deferred segment
+  int r, h, i, from, to;
+  bool late;                             // the first segment is still to come
   AMASS_DEV void start(const ChunkArgs& a, const ChPlan& p) {
-    q = p.q; r = p.r; h = p.h; i = p.i; uoff = p.uoff; rem = p.rem;
-    late = 0;
-    if (uoff > 0 && rem > 0) {
+    q = p.q; r = p.r; h = p.h; i = p.i; from = p.from; to = p.to;
+    late = false;
+    if (from > 0 && to > 0) {
       int lo;
-      const int n = min(rem, ch_tiles(a, q, i, &lo) - uoff);
-      if (n < rem) {
-        late = n;
-        rem -= n;
-        uoff = 0;
-        step(a);
+      const int w = ch_weight(a, q, i), n = ch_tiles(a, q, i, &lo);
+      if (to > n * w + kCostItem) {      // the run goes on behind this item
+        late = from <= (n - 1) * w;      // no tile of it: its overhead only
+        step(a, n * w + kCostItem);
       }
     }
   }
-  AMASS_DEV void step(const ChunkArgs& a) {
+  AMASS_DEV void step(const ChunkArgs& a, int cost) {
+    from = 0;
+    to -= cost;
     if (++i < q.nt) return;
     i = 0;
     if (++h < a.n_kv) return;
     h = 0;
-    if (rem <= 0) return;
+    if (to <= 0) return;
     do {
-      if (++r >= a.n_req) break;
+      if (++r >= a.n_req) { to = 0; return; }
       q = ch_req(a, r);
     } while (q.nt == 0);
   }
   AMASS_DEV bool next(const ChunkArgs& a, const ChPlan& p, ChSeg& s) {
-    if (rem <= 0 || r >= a.n_req) {
-      if (late == 0) return false;
-      q = p.q; r = p.r; h = p.h; i = p.i; uoff = p.uoff; rem = late;
-      late = 0;
+    bool only = false;
+    if (to <= 0) {
+      if (!late) return false;
+      late = false;
+      only = true;
+      q = p.q; r = p.r; h = p.h; i = p.i; from = p.from; to = p.to;
     }
-    const int tl = a.tm_log2 + 1;
+    const int tl = a.tm_log2 + 1, w = ch_weight(a, q, i);
     int lo;
     const int nu = ch_tiles(a, q, i, &lo);
+    const int k0 = (from + w - 1) / w;
+    const int k1 = to >= nu * w ? nu : (to + w - 1) / w;
+    if (k0 >= k1) return false;          // a run inside an item's overhead
     s.r = r; s.h = h; s.q0 = q.q0; s.off = q.off; s.sl = q.sl;
     s.tok0 = i << tl;
     s.ntok = min(1 << tl, q.ql - s.tok0);
-    s.t0 = lo + uoff;
-    s.n = min(rem, nu - uoff);
-    s.first = uoff == 0;
-    s.left = nu - uoff - s.n;
-    s.last = s.left == 0;
-    rem -= s.n;
-    uoff = 0;
-    step(a);
+    s.t0 = lo + k0;
+    s.n = k1 - k0;
+    s.first = k0 == 0;
+    s.last = k1 == nu;
+    // CTAs behind this one that hold the rest of the item
+    s.parts = s.last ? 0 : (int)((p.end - to + (int64_t)(nu - 1) * w) /
+                                 p.share) - (int)blockIdx.x;
+    if (only) to = 0;
+    else step(a, nu * w + kCostItem);
     return true;
   }
 };
 
-// this CTA's run of the flat unit list
+// this CTA's run of the flat list of items
 AMASS_DEV void ch_plan(const ChunkArgs& a, ChPlan* out) {
   __shared__ long long wsum[kChThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int per = (a.n_req + kChThreads - 1) / kChThreads;
   const int r0 = min(a.n_req, tid * per), r1 = min(a.n_req, r0 + per);
-  long long mine = 0, units = 0;
+  long long mine = 0, cost = 0;
   ChReq q;
   for (int r = r0; r < r1; ++r) {
     q = ch_req(a, r);
-    units = ch_units(a, q, q.nt);
-    mine += units * a.n_kv;
+    cost = ch_cost(a, q, q.nt);
+    mine += cost * a.n_kv;
   }
   long long incl = mine;
 #pragma unroll
@@ -344,7 +361,7 @@ AMASS_DEV void ch_plan(const ChunkArgs& a, ChPlan* out) {
     if (lane >= o) incl += x;
   }
   if (lane == 31) wsum[w] = incl;
-  if (tid == 0) out->rem = 0;
+  if (tid == 0) out->to = 0;
   __syncthreads();
   long long before = incl - mine, total = 0;
 #pragma unroll
@@ -353,37 +370,38 @@ AMASS_DEV void ch_plan(const ChunkArgs& a, ChPlan* out) {
     total += wsum[i];
   }
   long long share = (total + gridDim.x - 1) / gridDim.x;
-  if (share < kMinUnits) share = kMinUnits;
-  long long u0 = share * blockIdx.x;
-  const long long u1 = min(total, u0 + share);
-  if (u0 >= before && u0 < before + mine) {
-    u0 -= before;
+  if (share < kMinRun) share = kMinRun;
+  const long long begin = share * blockIdx.x;
+  const long long end = min(total, begin + share);
+  if (begin >= before && begin < before + mine) {
+    long long u = begin - before;
     for (int r = r0; r < r1; ++r) {
       if (per > 1) {                     // one request: still in registers
         q = ch_req(a, r);
-        units = ch_units(a, q, q.nt);
+        cost = ch_cost(a, q, q.nt);
       }
-      const long long all = units * a.n_kv;
-      if (u0 >= all) {
-        u0 -= all;
+      const long long all = cost * a.n_kv;
+      if (u >= all) {
+        u -= all;
         continue;
       }
-      const int h = all >> 32 ? (int)(u0 / units)
-                              : (int)((uint32_t)u0 / (uint32_t)units);
-      u0 -= h * units;
+      const int h = all >> 32 ? (int)(u / cost)
+                              : (int)((uint32_t)u / (uint32_t)cost);
+      u -= h * cost;
       int lo = 0, hi = q.nt;             // last item that starts at or before
       while (hi - lo > 1) {
         const int m = (lo + hi) >> 1;
-        if (ch_units(a, q, m) <= u0) lo = m; else hi = m;
+        if (ch_cost(a, q, m) <= u) lo = m; else hi = m;
       }
+      u -= ch_cost(a, q, lo);
       out->q = q;
       out->r = r;
       out->h = h;
       out->i = lo;
-      out->uoff = (int)(u0 - ch_units(a, q, lo));
-      out->rem = (int)(u1 - share * blockIdx.x);
+      out->from = (int)u;
+      out->to = (int)(u + end - begin);
       out->share = (int)share;
-      out->u1 = u1;
+      out->end = end;
       break;
     }
   }
@@ -394,7 +412,11 @@ template <int D>
 struct ChShape {
   static constexpr int kPanels = D / 64;
   static constexpr int kTile = kKeys * D * 2;        // bytes of a K or V tile
-  static constexpr int kPanel = kKeys * 128;         // bytes of a panel
+  static constexpr int kPanel = kKeys * 128;         // Q: 128 rows x 64
+  // K and V: 8 rows x 64 columns are one kilobyte, the panels of 8 rows side
+  // by side, so that one copy brings a whole page
+  static constexpr int kRows8 = kPanels * 1024;
+  static constexpr int kPage = 2 * kRows8;
   static constexpr int kStages = 163840 / kTile;     // 160 KB of ring
   static constexpr int kSmem = 2 * kTile + kStages * kTile + 1024;
   static constexpr uint32_t kCols = 512;             // 2 S/P + 2 O
@@ -409,7 +431,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   using X = ChShape<D>;
   constexpr int NS = X::kStages;
   extern __shared__ uint8_t dyn[];
-  __shared__ __align__(8) uint64_t bars[2 * NS + 14];
+  __shared__ __align__(8) uint64_t bars[2 * NS + 16];
   __shared__ float2 ml_s[128];           // warpgroup 1's (m, l), one-tile items
   __shared__ ChPlan plan;
   __shared__ uint32_t tmem_s;
@@ -420,10 +442,11 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   const uint32_t b0 = smem_u32(bars);
   const auto full = [&](int s) { return b0 + 8u * s; };
   const auto empty = [&](int s) { return b0 + 8u * (NS + s); };
-  const uint32_t q_full = b0 + 8u * (2 * NS), q_empty = q_full + 8;
-  const uint32_t s_full = q_full + 16, p_full = q_full + 32;   // two each
-  const uint32_t o_full = q_full + 48, p_part = q_full + 64;   // two each
-  const uint32_t v_tmp = q_full + 80, drain = v_tmp + 8;
+  // one of each per row tile
+  const uint32_t q_full = b0 + 8u * (2 * NS), q_empty = q_full + 16;
+  const uint32_t s_full = q_full + 32, p_part = q_full + 48;
+  const uint32_t p_full = q_full + 64, o_full = q_full + 80;
+  const uint32_t v_tmp = q_full + 96, drain = v_tmp + 8;
   const uint32_t pair = v_tmp + 16, pair_done = v_tmp + 24;
 
   if (tid == 0) {
@@ -431,9 +454,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
     }
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
     for (int t = 0; t < 2; ++t) {
+      mbar_init(q_full + 8 * t, 1);
+      mbar_init(q_empty + 8 * t, 1);
       mbar_init(s_full + 8 * t, 1);
       mbar_init(p_part + 8 * t, 4);
       mbar_init(p_full + 8 * t, 4);
@@ -476,9 +499,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   ChSeg sg;
 
   // a softmax thread holds a row of 128 scores: 384 * 168 registers at launch
-  // = 128 * (2 * 208 + 88)
+  // = 128 * (2 * 192 + 120)
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     // ------------------------------------------------------------- softmax
     const int t = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -494,11 +517,13 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       const int it = (two ? t * tm : 0) + tok;   // token within the item
       const bool valid = tok < tm && it < sg.ntok;
       const int pos = sg.off + sg.tok0 + it;
-      const int khi = valid ? max(pos + 1, 0) : 0;
-      const int klo = a.window ? max(pos - a.window + 1, 0) : 0;
+      // rows of nobody compute on whatever Q's buffer holds, unmasked
+      const int khi = valid ? max(pos + 1, 0) : 0x7fffffff;
+      const int klo = valid && a.window ? max(pos - a.window + 1, 0) : 0;
       const bool live = __any_sync(~0u, valid);
+      const int by = two ? 1 : 2;
       float m = -INFINITY, l = 0.f;
-      for (int j = two ? 0 : t; j < sg.n; j += two ? 1 : 2) {
+      for (int j = two ? 0 : t; j < sg.n; j += by) {
         if (!(ok = wait_warp(s_full + 8 * t, sph))) break;
         sph ^= 1;
         tc_after();
@@ -508,7 +533,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
           for (int c = 0; c < 4; ++c) tc_ld32(s + 32 * c, ts + 32 * c);
           tc_wait_ld();
           const int k0 = (sg.t0 + j) * kKeys;
-          if (__any_sync(~0u, k0 + kKeys > khi || k0 < klo)) {
+          if (__any_sync(~0u, khi - k0 < kKeys || k0 < klo)) {
             const int e = khi - k0, b = klo - k0;
 #pragma unroll
             for (int c = 0; c < 128; ++c)
@@ -521,16 +546,17 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
           for (int c = 4; c < 124; c += 8)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              x4[e] = fmaxf(fmaxf(x4[e], __uint_as_float(s[c + e])),
-                            __uint_as_float(s[c + 4 + e]));
+              x4[e] = fmax_nan(fmax_nan(x4[e], __uint_as_float(s[c + e])),
+                               __uint_as_float(s[c + 4 + e]));
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            x4[c] = fmaxf(x4[c], __uint_as_float(s[124 + c]));
-          const float mx = fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3]));
-          if (j < 2 - (two ? 1 : 0)) {           // this warpgroup's first tile
+            x4[c] = fmax_nan(x4[c], __uint_as_float(s[124 + c]));
+          const float mx = fmax_nan(fmax_nan(x4[0], x4[1]),
+                                    fmax_nan(x4[2], x4[3]));
+          if (j < by) {                  // this warpgroup's first tile
             m = mx;
-          } else if (__any_sync(~0u, (mx - m) * sl2 > kRescaleLog2)) {
-            const float mn = fmaxf(m, mx);
+          } else if (__any_sync(~0u, valid && !((mx - m) * sl2 <= kRescaleLog2))) {
+            const float mn = fmax_nan(m, mx);
             const float f = m == -INFINITY ? 0.f : ex2_approx((m - mn) * sl2);
             l *= f;
             m = mn;
@@ -545,7 +571,8 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
               tc_st16(to + c, o);
             }
           }
-          const float nm = m == -INFINITY ? 0.f : -m * sl2;
+          // an infinite or NaN score makes the row NaN, as the formula does
+          const float nm = m == -INFINITY ? 0.f : fmaf(0.f, m, -m * sl2);
           const uint64_t nm2 = f2(nm, nm);
           uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
@@ -602,7 +629,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
         cph ^= 1;
         tc_after();
         const float2 o = ml_s[row];
-        const float mn = fmaxf(m, o.x), ref = mn == -INFINITY ? 0.f : mn;
+        const float mn = fmax_nan(m, o.x), ref = mn == -INFINITY ? 0.f : mn;
         f0 = ex2_approx((m - ref) * sl2);
         f1 = ex2_approx((o.x - ref) * sl2);
         l = l * f0 + o.y * f1;
@@ -673,33 +700,30 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
         if (lane == 0) mbar_arrive(pair_done);
       }
       if (!whole && sg.first && tid == 0) {
-        // the CTAs behind this one that hold the rest of the item
-        const long long end = plan.u1 + sg.left;
         a.meta[blockIdx.x] =
-            make_int4((int)((end - 1) / plan.share) - (int)blockIdx.x,
-                      sg.q0 + sg.tok0, sg.ntok, sg.h);
+            make_int4(sg.parts, sg.q0 + sg.tok0, sg.ntok, sg.h);
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
     if (warp == 8) {
       // ------------------------------------------------------------ producer
-      int st = 0, issued = 0;
-      uint32_t ph = 1, qph = 1;
+      int st = 0;
+      uint32_t ph = 1, qph = 3, vph = 0;
       bool ok = true;
       while (ok && wk.next(a, plan, sg)) {
         const int tm = 1 << a.tm_log2;
-        if (!(ok = wait_warp(q_empty, qph))) break;
-        qph ^= 1;
-        if (lane == 0) {
-          const int halves = sg.ntok > tm ? 2 : 1;
-          mbar_arrive_expect_tx(q_full,
-                                halves * X::kPanels * 128u * a.G * tm);
-          for (int t = 0; t < halves; ++t)
+        for (int t = 0; ok && t < (sg.ntok > tm ? 2 : 1); ++t) {
+          if (!(ok = wait_warp(q_empty + 8 * t, (qph >> t) & 1))) break;
+          qph ^= 1u << t;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(q_full + 8 * t, X::kPanels * 128u * a.G * tm);
             for (int p = 0; p < X::kPanels; ++p)
-              tma_3d(q_s + t * X::kTile + p * X::kPanel, &mq, q_full, p * 64,
-                     sg.h * a.G, sg.q0 + sg.tok0 + t * tm);
+              tma_3d(q_s + t * X::kTile + p * X::kPanel, &mq, q_full + 8 * t,
+                     p * 64, sg.h * a.G, sg.q0 + sg.tok0 + t * tm);
+          }
         }
+        if (!ok) break;
         const int npg = (sg.sl + kPg - 1) / kPg;
         const int32_t* row = a.bt + (int64_t)sg.r * a.bt_stride;
         // block of the tile's page (lane & 7); pages that are not the
@@ -710,41 +734,54 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
           if (p < npg) b = row[p];
           return b < 0 || b >= a.nb ? a.nb : b;
         };
-        int blk = block_of(sg.t0);
-        for (int j = 0; ok && j < sg.n; ++j) {
-          const int tile = sg.t0 + j;
-          const int nxt = j + 1 < sg.n ? block_of(tile + 1) : 0;
-          const bool part = (sg.sl & (kPg - 1)) && tile == (sg.sl - 1) >> 7;
-          for (int kv = 0; kv < 2; ++kv) {
-            if (!(ok = wait_warp(empty(st), ph))) break;
-            const uint32_t dst = ring + st * X::kTile;
-            const uint32_t bar = kv && part ? v_tmp : full(st);
-            if (lane == 0) mbar_arrive_expect_tx(bar, X::kTile);
-            __syncwarp();
-            if (lane < 8 * X::kPanels)
-              tma_4d(dst + (lane >> 3) * X::kPanel + (lane & 7) * (kPg * 128),
-                     kv ? &mv : &mk, bar, (lane >> 3) * 64, sg.h, 0, blk);
-            if (kv && part) {
-              // rows behind the last token: whatever they hold, 0 * it must
-              // be 0 in P V
-              if (!(ok = wait_warp(v_tmp, (issued >> 16) & 1))) break;
-              const int r0 = sg.sl & (kPg - 1);
-              const int at = (((sg.sl - 1) & (kKeys - 1)) & ~(kPg - 1)) + r0;
-              const int words = (kPg - r0) * 8 * X::kPanels;
-              for (int i = lane; i < words; i += 32) {
-                const int p = i / ((kPg - r0) * 8), x = i - p * (kPg - r0) * 8;
-                const uint32_t d = dst + p * X::kPanel + at * 128 + x * 16;
-                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};"
-                             :: "r"(d), "r"(0) : "memory");
-              }
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              __syncwarp();
-              if (lane == 0) mbar_arrive(full(st));
-              issued ^= 1 << 16;
+        const auto load = [&](bool is_v, int tile, int blk) -> bool {
+          if (!wait_warp(empty(st), ph)) return false;
+          const bool part = is_v && (sg.sl & (kPg - 1)) &&
+                            tile == (sg.sl - 1) >> 7;
+          const uint32_t dst = ring + st * X::kTile;
+          const uint32_t bar = part ? v_tmp : full(st);
+          if (lane == 0) mbar_arrive_expect_tx(bar, X::kTile);
+          __syncwarp();
+          if (lane < 8)
+            tma_5d(dst + lane * X::kPage, is_v ? &mv : &mk, bar,
+                   blk * a.bh + sg.h);
+          if (part) {
+            // rows behind the last token: whatever they hold, 0 * it must be
+            // 0 in P V
+            if (!wait_warp(v_tmp, vph)) return false;
+            vph ^= 1;
+            constexpr int kWords = 8 * X::kPanels;
+            const int r0 = sg.sl & (kPg - 1);
+            const uint32_t pg =
+                dst + ((sg.sl - 1) & (kKeys - 1)) / kPg * X::kPage;
+            for (int i = lane; i < (kPg - r0) * kWords; i += 32) {
+              const int c = i % kWords, r = r0 + i / kWords;
+              const uint32_t d = pg + (r >> 3) * X::kRows8 + (c >> 3) * 1024 +
+                                 (r & 7) * 128 + (c & 7) * 16;
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};"
+                           :: "r"(d), "r"(0) : "memory");
             }
-            if (++st == NS) { st = 0; ph ^= 1; }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full(st));
           }
-          blk = nxt;
+          if (++st == NS) { st = 0; ph ^= 1; }
+          return true;
+        };
+        // in the order of use, `lead` tiles of K before the first of V: the
+        // ring then covers the same time for both
+        const int lead = sg.ntok > tm ? 1 : 2;
+        int b0 = block_of(sg.t0);
+        int b1 = sg.n > 1 ? block_of(sg.t0 + 1) : 0;
+        ok = load(false, sg.t0, b0);
+        if (ok && lead == 2 && sg.n > 1) ok = load(false, sg.t0 + 1, b1);
+        for (int j = 0; ok && j < sg.n; ++j) {
+          const int b2 = j + 2 < sg.n ? block_of(sg.t0 + j + 2) : 0;
+          ok = load(true, sg.t0 + j, b0) &&
+               (j + lead >= sg.n ||
+                load(false, sg.t0 + j + lead, lead == 1 ? b1 : b2));
+          b0 = b1;
+          b1 = b2;
         }
       }
       if (!ok) {
@@ -753,106 +790,140 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
           (void)mbar_wait(full(s), s < st ? (ph ^ 1) & 1 : ph & 1);
       }
     } else if (warp == 9) {
-      // ----------------------------------------------------------------- MMA
-      if (lane == 0) {
-        constexpr uint32_t id_s = mma_idesc(kF16, false, kKeys);
-        constexpr uint32_t id_o = mma_idesc(kF16, true, D);
-        uint32_t seq = 0, qph = 0, pph = 0;
-        bool ok = true;
-        // K of tile j is the ring's entry seq + 2 j, V the one behind it
-        const auto stage = [&](uint32_t n) { return (int)(n % NS); };
-        const auto arrived = [&](uint32_t n) {
-          return wait(full(stage(n)), (n / NS) & 1);
-        };
-        const auto scores = [&](int t, int qt, uint32_t n) {
-          const uint32_t qa = q_s + qt * X::kTile;
-          const uint32_t ka = ring + stage(n) * X::kTile;
+      // --------------------------------------------------------------- MMA
+      // The tensor core takes the next MMA about when the last one starts, so
+      // what this warp does between two MMAs is time lost.  It looks for the V
+      // tile and the next K tile while it would wait for weights anyway, and
+      // the whole warp walks while one elected lane issues (with a lane's own branch around it the
+      // compiler moves every descriptor to uniform registers one by one: 48
+      // cycles a small MMA instead of 37).  Two issuing warps, one per row
+      // tile, were slower: alternating MMAs of two accumulators do not
+      // overlap (2048 rows behind 64K: 1900 -> 2490 us).
+      constexpr uint32_t id_s = mma_idesc(kF16, false, kKeys);
+      constexpr uint32_t id_o = mma_idesc(kF16, true, D);
+      constexpr uint32_t kStep = X::kTile >> 4;
+      const uint64_t qd = smem_desc(q_s, 16, 1024);
+      const uint64_t kd = smem_desc(ring, 16, X::kRows8);
+      const uint64_t vd = smem_desc(ring, 1024, X::kRows8);
+      int st = 0;                        // the next ring entry and its phase
+      uint32_t ph = 0, qph = 0, pph = 0;
+      bool ok = true;
+      const auto score = [&](int t, uint64_t q0, uint64_t k0, int k) {
+        mma_ss(tmem + t * 128, q0 + (((k >> 2) * X::kPanel + (k & 3) * 32) >> 4),
+               k0 + (((k >> 2) * 1024 + (k & 3) * 32) >> 4), id_s, k > 0);
+      };
+      // S_t of ring entry e, which then is free when `done`
+      const auto scores = [&](int t, uint64_t q0, int e, bool done) {
+        const uint64_t k0 = kd + (uint32_t)e * kStep;
+        if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t o = (k >> 2) * X::kPanel + (k & 3) * 32;
-            mma_ss(tmem + t * 128, smem_desc(qa + o, 16, 1024),
-                   smem_desc(ka + o, 16, 1024), id_s, k > 0);
-          }
+          for (int k = 0; k < D / 16; ++k) score(t, q0, k0, k);
           mma_commit(s_full + 8 * t);
-        };
-        // O_t += P_t V, the first keys of the tile as soon as their weights
-        // are there
-        const auto product = [&](int t, uint32_t n, bool acc) -> bool {
-          const uint32_t va = ring + stage(n) * X::kTile, p = (pph >> t) & 1;
-          pph ^= 1u << t;
-          if (!wait(p_part + 8 * t, p)) return false;
-          tc_after();
-#pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k) {
-            if (k == kPart / 16) {
-              if (!wait(p_full + 8 * t, p)) return false;
-              tc_after();
-            }
-            mma_ts(tmem + X::kO + t * D, tmem + t * 128 + k * 8,
-                   smem_desc(va + k * 2048, X::kPanel, 1024), id_o,
-                   acc || k > 0);
-          }
-          return true;
-        };
-        while (ok && wk.next(a, plan, sg)) {
-          const bool two = sg.ntok > (1 << a.tm_log2);
-          const int n = sg.n;
-          if (!(ok = wait(q_full, qph))) break;
-          qph ^= 1;
-          if (!(ok = arrived(seq))) break;
-          tc_after();
-          scores(0, 0, seq);
-          if (two) scores(1, 1, seq);
-          mma_commit(empty(stage(seq)));
-          if (two) {
-            if (n == 1) mma_commit(q_empty);
-            for (int j = 0; ok && j < n; ++j) {
-              const uint32_t v = seq + 2 * j + 1, k = v + 1;
-              const bool more = j + 1 < n;
-              ok = arrived(v) && (!more || arrived(k));
-              for (int t = 0; ok && t < 2; ++t) {
-                if (!(ok = product(t, v, j > 0))) break;
-                if (more) scores(t, t, k);
-                else mma_commit(o_full + 8 * t);
-              }
-              if (!ok) break;
-              mma_commit(empty(stage(v)));
-              if (more) mma_commit(empty(stage(k)));
-              if (j + 2 == n) mma_commit(q_empty);
-            }
-          } else {
-            // one row tile: the two warpgroups take its key tiles in turn
-            if (n > 1) {
-              if (!(ok = arrived(seq + 2))) break;
-              tc_after();
-              scores(1, 0, seq + 2);
-              mma_commit(empty(stage(seq + 2)));
-            }
-            if (n <= 2) mma_commit(q_empty);
-            for (int j = 0; j < n; ++j) {
-              const uint32_t v = seq + 2 * j + 1, k = v + 3;
-              const int t = j & 1;
-              const bool more = j + 2 < n;
-              ok = arrived(v) && (!more || arrived(k)) &&
-                   product(t, v, j > 1);
-              if (!ok) break;
-              mma_commit(empty(stage(v)));
-              if (more) {
-                scores(t, 0, k);
-                mma_commit(empty(stage(k)));
-              } else {
-                mma_commit(o_full + 8 * t);
-              }
-              if (j + 3 == n) mma_commit(q_empty);
-            }
-          }
-          seq += 2 * n;
+          if (done) mma_commit(empty(e));
         }
-        // every MMA and its arrivals end before the CTA does
-        mma_commit(drain);
-        (void)mbar_wait(drain, 0);
+        __syncwarp();
+      };
+      // the next entry in the order of use: its index, + NS in odd phases
+      const auto take = [&]() {
+        const int e = st + (ph ? NS : 0);
+        if (++st == NS) { st = 0; ph ^= 1; }
+        return e;
+      };
+      const auto arrived = [&](int e) {
+        return wait_warp(full(e >= NS ? e - NS : e), e >= NS);
+      };
+      const auto commit = [&](uint32_t bar) {
+        if (elect_one()) mma_commit(bar);
+        __syncwarp();
+      };
+      // O_t += P_t V of entry ve, the first keys of the tile as soon as their
+      // weights are there, then S_t of entry ke (-1: none).  look: the entries
+      // have not been seen yet (2: K may wait until P V is issued), done:
+      // nothing else needs them
+      const auto turn = [&](int t, int ve, bool acc, uint64_t q0, int ke,
+                            int look, bool done) -> bool {
+        const int v = ve >= NS ? ve - NS : ve, kn = ke >= NS ? ke - NS : ke;
+        const uint64_t v0 = vd + (uint32_t)v * kStep;
+        const uint64_t k0 = kd + (uint32_t)kn * kStep;
+        const uint32_t p = tmem + t * 128, o = tmem + X::kO + t * D;
+        const uint32_t par = (pph >> t) & 1;
+        pph ^= 1u << t;
+        if (look && !arrived(ve)) return false;
+        if (look == 1 && ke >= 0 && !arrived(ke)) return false;
+        if (!wait_warp(p_part + 8 * t, par)) return false;
+        tc_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < kPart / 16; ++k)
+            mma_ts(o, p + k * 8, v0 + k * (X::kPage >> 4), id_o, acc || k > 0);
+        }
+        __syncwarp();
+        if (!wait_warp(p_full + 8 * t, par)) return false;
+        if (look == 2 && ke >= 0 && !arrived(ke)) return false;
+        tc_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = kPart / 16; k < kKeys / 16; ++k)
+            mma_ts(o, p + k * 8, v0 + k * (X::kPage >> 4), id_o, true);
+          if (ke >= 0) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) score(t, q0, k0, k);
+            mma_commit(s_full + 8 * t);
+            if (done) mma_commit(empty(kn));
+          } else {
+            mma_commit(o_full + 8 * t);
+          }
+          if (done) mma_commit(empty(v));
+        }
+        __syncwarp();
+        return true;
+      };
+      const auto scores_of = [&](int t, uint64_t q0, int e, bool done) {
+        scores(t, q0, e >= NS ? e - NS : e, done);
+      };
+      while (ok && wk.next(a, plan, sg)) {
+        const int n = sg.n;
+        const bool two = sg.ntok > (1 << a.tm_log2);
+        const int k0 = take();
+        if (!(ok = wait_warp(q_full, qph & 1) && arrived(k0))) break;
+        tc_after();
+        scores_of(0, qd, k0, !two);
+        if (two) {
+          if (!(ok = wait_warp(q_full + 8, (qph >> 1) & 1))) break;
+          qph ^= 3;
+          tc_after();
+          scores_of(1, qd + kStep, k0, true);
+          if (n == 1) {
+            commit(q_empty);
+            commit(q_empty + 8);
+          }
+          for (int j = 0; j < n; ++j) {
+            const int v = take(), k = j + 1 < n ? take() : -1;
+            if (!(ok = turn(0, v, j > 0, qd, k, 1, false))) break;
+            if (j + 2 == n) commit(q_empty);
+            if (!(ok = turn(1, v, j > 0, qd + kStep, k, 0, true))) break;
+            if (j + 2 == n) commit(q_empty + 8);
+          }
+        } else {
+          // one row tile: the two warpgroups take its key tiles in turn
+          qph ^= 1;
+          if (n > 1) {
+            const int k1 = take();
+            if (!(ok = arrived(k1))) break;
+            tc_after();
+            scores_of(1, qd, k1, true);
+          }
+          if (n <= 2) commit(q_empty);
+          for (int j = 0; j < n; ++j) {
+            const int v = take(), k = j + 2 < n ? take() : -1;
+            if (!(ok = turn(j & 1, v, j > 1, qd, k, 2, true))) break;
+            if (j + 3 == n) commit(q_empty);
+          }
+        }
       }
-      __syncwarp();
+      // every MMA and its arrivals end before the CTA does
+      commit(drain);
+      (void)wait_warp(drain, 0);
     }
   }
   tc_before();
@@ -950,8 +1021,8 @@ int make_map(CUtensorMap* m, bool f16, const void* p, int rank,
              const uint64_t* dim, const int64_t* stride, const uint32_t* box) {
   const EncodeFn fn = encode_fn();
   if (!fn) return AMASS_ERR_CUDA;
-  cuuint64_t gd[4], gs[3];
-  cuuint32_t bx[4], es[4];
+  cuuint64_t gd[5], gs[4];
+  cuuint32_t bx[5], es[5];
   for (int i = 0; i < rank; ++i) {
     gd[i] = dim[i];
     bx[i] = box[i];
@@ -1015,18 +1086,33 @@ extern "C" int amass_paged_chunk(const AmassChunk* args, void* stream) {
   const uint64_t d = (uint64_t)x.head_dim;
   const uint64_t qdim[3] = {d, (uint64_t)(x.n_kv * x.G),
                             (uint64_t)x.n_tokens};
-  const uint64_t kdim[4] = {d, (uint64_t)x.n_kv, (uint64_t)kPg,
-                            (uint64_t)x.num_blocks};
   const int64_t qstr[3] = {1, x.q_sh, x.q_st};
-  const int64_t kstr[4] = {1, x.k_sh, x.k_st, x.k_sb};
-  const int64_t vstr[4] = {1, x.v_sh, x.v_st, x.v_sb};
-  const auto bad = [](uint64_t n, int64_t s) {
-    return n > 1 && (s <= 0 || (s & 7));
+  // K and V, page by page: 64 columns, 8 tokens, the panels, the page's two
+  // halves, and (block, head) as one dimension of head strides
+  const int panels = x.head_dim / 64;
+  const auto rows = [&](int64_t sb, int64_t sh) {
+    return x.n_kv == 1 ? 1 : x.num_blocks == 1 ? x.n_kv : sb / sh;
   };
-  for (int i = 1; i < 4; ++i)
-    if ((i < 3 && bad(qdim[i], qstr[i])) || bad(kdim[i], kstr[i]) ||
-        bad(kdim[i], vstr[i]))
-      return AMASS_ERR_ARG;
+  const auto bad = [](bool used, int64_t s) {
+    return used && (s <= 0 || (s & 7));
+  };
+  if (bad(x.n_kv * x.G > 1, x.q_sh) || bad(x.n_tokens > 1, x.q_st) ||
+      bad(true, x.k_st) || bad(true, x.v_st) || bad(x.n_kv > 1, x.k_sh) ||
+      bad(x.n_kv > 1, x.v_sh) || bad(x.num_blocks > 1, x.k_sb) ||
+      bad(x.num_blocks > 1, x.v_sb))
+    return AMASS_ERR_ARG;
+  const int64_t bh = rows(x.k_sb, x.k_sh);
+  if (x.n_kv > 1 && x.num_blocks > 1 &&
+      (x.k_sb % x.k_sh || x.v_sb % x.v_sh || x.k_sb < x.n_kv * x.k_sh ||
+       rows(x.v_sb, x.v_sh) != bh))
+    return AMASS_ERR_UNSUPPORTED;
+  if ((x.num_blocks + 1ll) * bh >= (1ll << 31)) return AMASS_ERR_UNSUPPORTED;
+  const uint64_t kdim[5] = {64, 8, (uint64_t)panels, 2,
+                            (uint64_t)((x.num_blocks - 1) * bh + x.n_kv)};
+  const int64_t kstr[5] = {1, x.k_st, 64, 8 * x.k_st,
+                           x.n_kv > 1 ? x.k_sh : x.k_sb};
+  const int64_t vstr[5] = {1, x.v_st, 64, 8 * x.v_st,
+                           x.n_kv > 1 ? x.v_sh : x.v_sb};
 
   ChunkArgs a = {};
   a.bt = x.block_table; a.bt_stride = x.bt_stride; a.sl = x.seq_lens;
@@ -1036,16 +1122,16 @@ extern "C" int amass_paged_chunk(const AmassChunk* args, void* stream) {
   a.meta = reinterpret_cast<int4*>(x.meta); a.fault = x.fault;
   a.scale_log2 = x.scale * kLog2e;
   a.n_req = x.n_req; a.n_kv = x.n_kv; a.G = x.G; a.T = x.n_tokens;
-  a.max_pages = x.max_pages; a.nb = x.num_blocks; a.window = x.window;
+  a.bh = (int)bh; a.max_pages = x.max_pages; a.nb = x.num_blocks; a.window = x.window;
   // tokens of a row tile: the largest power of two whose G heads fit 128 rows
   a.tm_log2 = x.G == 1 ? 7 : x.G == 2 ? 6 : x.G <= 4 ? 5 : 4;
   const bool f16 = x.dtype == AMASS_FP16;
   const uint32_t qbox[3] = {64, (uint32_t)x.G, 1u << a.tm_log2};
-  const uint32_t kbox[4] = {64, 1, (uint32_t)kPg, 1};
+  const uint32_t kbox[5] = {64, 8, (uint32_t)panels, 2, 1};
   CUtensorMap mq, mk, mv;
   int rc = make_map(&mq, f16, x.q, 3, qdim, qstr, qbox);
-  if (!rc) rc = make_map(&mk, f16, x.k, 4, kdim, kstr, kbox);
-  if (!rc) rc = make_map(&mv, f16, x.v, 4, kdim, vstr, kbox);
+  if (!rc) rc = make_map(&mk, f16, x.k, 5, kdim, kstr, kbox);
+  if (!rc) rc = make_map(&mv, f16, x.v, 5, kdim, vstr, kbox);
   if (rc) return rc;
   const int ctas = x.n_ctas < num_sms() ? x.n_ctas : num_sms();
   const cudaStream_t st = (cudaStream_t)stream;

@@ -252,6 +252,14 @@ AMASS_DEV bool mbar_try_wait(uint32_t bar, uint32_t parity) {
       : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
+// true in one lane of a converged warp
+AMASS_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n"
+      " selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
 AMASS_DEV uint64_t global_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));

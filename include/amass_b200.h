@@ -669,7 +669,8 @@ typedef struct AmassChunk {
  * need scratch of their own.  fault[0] becomes 1 when a CTA gave up a bounded
  * wait (its rows are then incomplete).  head_dim in {64, 128}, G <= 8, page =
  * 16, n_req <= 4096, scale > 0; bases 16-byte aligned, strides positive
- * multiples of 8 elements.  Two launches; the first call on a device sets a
+ * multiples of 8 elements, block strides multiples of the head strides, with
+ * the same quotient for K and V.  Two launches; the first call on a device sets a
  * kernel attribute. */
 int amass_paged_chunk(const AmassChunk* args, void* stream);
 
