@@ -151,7 +151,8 @@ class ChunkBuffers:
     captured graphs replayed at once -- need a ``ChunkBuffers`` each.
 
     ``fault`` (1,) int32 latches 1 when a kernel gave up a bounded wait;
-    ``check()`` reads it (synchronises) and raises."""
+    ``check()`` reads it (synchronises) and raises: the buffers are then to be
+    replaced."""
 
     def __init__(self, device, *, n_kv: int, G: int, head_dim: int):
         if head_dim not in (64, 128) or not 1 <= G <= 8 or n_kv < 1:
@@ -166,10 +167,10 @@ class ChunkBuffers:
         self.acc_part = torch.empty(n, 2, head_dim // 4, 256, 4, device=dev,
                                     dtype=f32)
         self.ml_part = torch.empty(n, 2, 256, 2, device=dev, dtype=f32)
-        self.meta = torch.zeros(n, 4, device=dev, dtype=torch.int32)
+        self.tickets = torch.zeros(n, 8, device=dev, dtype=torch.int32)
         self.fault = torch.zeros(1, device=dev, dtype=torch.int32)
         self.scratch = (ptr(self.acc_part), ptr(self.ml_part),
-                        ptr(self.meta), ptr(self.fault))
+                        ptr(self.tickets), ptr(self.fault))
 
     def check(self) -> None:
         if int(self.fault.item()):

@@ -27,7 +27,9 @@
 // Work split: the (item, key tile) units of the whole batch form one flat
 // list; every CTA takes an equal run of it.  Lengths live on the device, so
 // each CTA scans the requests and finds its own run.  Items cut by a run's
-// end leave unnormalised partials that the merge kernel joins.  This serves a
+// end leave unnormalised partials; the CTA that finishes the last one of a
+// warp's rows joins them (a second kernel for that took 9 us of 20 at one
+// token).  This serves a
 // single token over a long context (all SMs read one request's cache) and a
 // large prefill (no tail of uneven causal tiles) with one rule.
 //
@@ -61,7 +63,7 @@ struct ChunkArgs {
   float* lse;                            // (T, H) or null
   float* acc;                            // [cta][2][D / 4][256][4]
   float2* ml;                            // [cta][2][256]
-  int4* meta;                            // [cta]: parts, token, tokens, head
+  int32_t* tickets;                      // [cta][8], 0 between calls
   int32_t* fault;
   float scale_log2;
   int n_req, n_kv, G, T, max_pages, nb, window, tm_log2;
@@ -266,13 +268,13 @@ AMASS_DEV int64_t ch_cost(const ChunkArgs& a, const ChReq& q, int m) {
 }
 
 struct ChSeg {
-  int r, h, q0, tok0, ntok, off, sl, t0, n, parts;
+  int r, h, q0, tok0, ntok, off, sl, t0, n;
+  int cta0, parts;                       // a cut item's CTAs
   bool first, last;
 };
 struct ChPlan {
   ChReq q;
   int r, h, i, from, to, share;          // run [from, to) from item i's start
-  long long end;                         // its end in the whole list
 };
 
 // Walks the segments of a CTA's run; every role keeps its own copy.  Key tile
@@ -284,11 +286,12 @@ struct ChPlan {
 // rows behind 64K tokens: 2290 -> 1920 us).
 struct ChWalk {
   ChReq q;
-  int r, h, i, from, to;
+  int r, h, i, from, to, at;             // at: the item's start in the run
   bool late;                             // the first segment is still to come
   AMASS_DEV void start(const ChunkArgs& a, const ChPlan& p) {
     q = p.q; r = p.r; h = p.h; i = p.i; from = p.from; to = p.to;
     late = false;
+    at = -from;
     if (from > 0 && to > 0) {
       int lo;
       const int w = ch_weight(a, q, i), n = ch_tiles(a, q, i, &lo);
@@ -301,6 +304,7 @@ struct ChWalk {
   AMASS_DEV void step(const ChunkArgs& a, int cost) {
     from = 0;
     to -= cost;
+    at += cost;
     if (++i < q.nt) return;
     i = 0;
     if (++h < a.n_kv) return;
@@ -318,12 +322,15 @@ struct ChWalk {
       late = false;
       only = true;
       q = p.q; r = p.r; h = p.h; i = p.i; from = p.from; to = p.to;
+      at = -from;
     }
     const int tl = a.tm_log2 + 1, w = ch_weight(a, q, i);
     int lo;
     const int nu = ch_tiles(a, q, i, &lo);
-    const int k0 = (from + w - 1) / w;
-    const int k1 = to >= nu * w ? nu : (to + w - 1) / w;
+    const auto tiles = [&](int c) {      // ceil(c / w)
+      return w == kCost2 ? (c + kCost2 - 1) / kCost2 : (c + kCost1 - 1) / kCost1;
+    };
+    const int k0 = tiles(from), k1 = to >= nu * w ? nu : tiles(to);
     if (k0 >= k1) return false;          // a run inside an item's overhead
     s.r = r; s.h = h; s.q0 = q.q0; s.off = q.off; s.sl = q.sl;
     s.tok0 = i << tl;
@@ -332,9 +339,12 @@ struct ChWalk {
     s.n = k1 - k0;
     s.first = k0 == 0;
     s.last = k1 == nu;
-    // CTAs behind this one that hold the rest of the item
-    s.parts = s.last ? 0 : (int)((p.end - to + (int64_t)(nu - 1) * w) /
-                                 p.share) - (int)blockIdx.x;
+    if (!(s.first && s.last)) {          // floor divisions by the run length
+      const int b = at < 0 ? -((p.share - 1 - at) / p.share) : 0;
+      s.cta0 = (int)blockIdx.x + b;
+      const int e = at + (nu - 1) * w;
+      s.parts = (e < 0 ? -((p.share - 1 - e) / p.share) : e / p.share) - b + 1;
+    }
     if (only) to = 0;
     else step(a, nu * w + kCostItem);
     return true;
@@ -369,7 +379,9 @@ AMASS_DEV void ch_plan(const ChunkArgs& a, ChPlan* out) {
     if (i < w) before += wsum[i];
     total += wsum[i];
   }
-  long long share = (total + gridDim.x - 1) / gridDim.x;
+  const long long over = total + gridDim.x - 1;
+  long long share = over >> 32 ? over / gridDim.x
+                               : (long long)((uint32_t)over / gridDim.x);
   if (share < kMinRun) share = kMinRun;
   const long long begin = share * blockIdx.x;
   const long long end = min(total, begin + share);
@@ -388,12 +400,15 @@ AMASS_DEV void ch_plan(const ChunkArgs& a, ChPlan* out) {
       const int h = all >> 32 ? (int)(u / cost)
                               : (int)((uint32_t)u / (uint32_t)cost);
       u -= h * cost;
-      int lo = 0, hi = q.nt;             // last item that starts at or before
-      while (hi - lo > 1) {
-        const int m = (lo + hi) >> 1;
-        if (ch_cost(a, q, m) <= u) lo = m; else hi = m;
+      int lo = 0;                        // last item that starts at or before
+      if (q.nt > 1) {
+        int hi = q.nt;
+        while (hi - lo > 1) {
+          const int m = (lo + hi) >> 1;
+          if (ch_cost(a, q, m) <= u) lo = m; else hi = m;
+        }
+        u -= ch_cost(a, q, lo);
       }
-      u -= ch_cost(a, q, lo);
       out->q = q;
       out->r = r;
       out->h = h;
@@ -401,7 +416,6 @@ AMASS_DEV void ch_plan(const ChunkArgs& a, ChPlan* out) {
       out->from = (int)u;
       out->to = (int)(u + end - begin);
       out->share = (int)share;
-      out->end = end;
       break;
     }
   }
@@ -423,6 +437,81 @@ struct ChShape {
   static constexpr uint32_t kO = 256;
 };
 
+// The rows of one warp of a cut item whose last partial was written here.
+struct ChJob {
+  int cta0, parts, h;                    // the item's CTAs, its kv head
+  int n, row0, tok0;                     // rows, first of the item's 256, token
+};                                       // of its row tile's row 0
+
+// out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over the item's CTAs in
+// order (the same result whichever CTA finishes last), by one warp: lanes are
+// spread over 2^sh >= n rows, then over groups of 4 columns; NC such blocks
+// from cg on, NP partials' loads in flight for each.
+template <int D, bool kF16, int NC, int NP>
+AMASS_DEV void ch_join(const ChunkArgs& a, const ChJob& b, int sh, int cg) {
+  const int lane = threadIdx.x & 31, r = lane & ((1 << sh) - 1);
+  const int by = 32 >> sh;
+  cg += lane >> sh;
+  if (r >= b.n) return;
+  const int row = b.row0 + r, tok = (row & 127) / a.G;
+  const float2* ml = a.ml + (int64_t)b.cta0 * 512 + row;
+  const float4* x = reinterpret_cast<const float4*>(a.acc) +
+                    ((int64_t)b.cta0 * 2 * (D / 4) + cg) * 256 + row;
+  float4 o[NC];
+  float M = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int k = 0; k < NC; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int c0 = 0; c0 < b.parts; c0 += NP) {
+    float4 v[NP][NC];
+    float2 z[NP];
+    // the first CTA's partial is its second slot, the others' their first
+#pragma unroll
+    for (int e = 0; e < NP; ++e) {
+      const int c = c0 + e, s = 2 * c + (c == 0);
+      z[e] = make_float2(-INFINITY, 0.f);
+      if (c < b.parts) z[e] = __ldcg(ml + s * 256);
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        v[e][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < b.parts && cg + k * by < D / 4)
+          v[e][k] = __ldcg(x + ((int64_t)s * (D / 4) + k * by) * 256);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < NP; ++e) {
+      const float mn = fmax_nan(M, z[e].x), ref = mn == -INFINITY ? 0.f : mn;
+      const float f = ex2_approx(M - ref), w = ex2_approx(z[e].x - ref);
+      M = mn;
+      l = l * f + w * z[e].y;
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        o[k].x = o[k].x * f + w * v[e][k].x;
+        o[k].y = o[k].y * f + w * v[e][k].y;
+        o[k].z = o[k].z * f + w * v[e][k].z;
+        o[k].w = o[k].w * f + w * v[e][k].w;
+      }
+    }
+  }
+  const bool some = l > 0.f || l != l;
+  const float inv = some ? 1.f / l : 0.f;
+  const int64_t token = b.tok0 + tok;
+  const int head = b.h * a.G + (row & 127) - tok * a.G;
+  char* out = (char*)a.out + 2 * (token * a.o_st + head * a.o_sh);
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    if (cg + k * by >= D / 4) continue;
+    const float x0 = o[k].x * inv, x1 = o[k].y * inv;
+    const float x2 = o[k].z * inv, x3 = o[k].w * inv;
+    *reinterpret_cast<uint2*>(out + 8 * (cg + k * by)) =
+        kF16 ? make_uint2(pack_h2(x0, x1), pack_h2(x2, x3))
+             : make_uint2(pack_bf2(x0, x1), pack_bf2(x2, x3));
+  }
+  if (a.lse && cg == 0)
+    a.lse[token * (a.n_kv * a.G) + head] =
+        some ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
+}
+
 template <int D, bool kF16>
 __global__ void __launch_bounds__(kChThreads, 1)
 chunk_kernel(const __grid_constant__ CUtensorMap mq,
@@ -433,6 +522,8 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   extern __shared__ uint8_t dyn[];
   __shared__ __align__(8) uint64_t bars[2 * NS + 16];
   __shared__ float2 ml_s[128];           // warpgroup 1's (m, l), one-tile items
+  __shared__ ChJob jobs[16];             // a run cuts two items, 8 warps' rows
+  __shared__ int n_jobs;
   __shared__ ChPlan plan;
   __shared__ uint32_t tmem_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -462,6 +553,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       mbar_init(p_full + 8 * t, 4);
       mbar_init(o_full + 8 * t, 1);
     }
+    n_jobs = 0;
     mbar_init(v_tmp, 1);
     mbar_init(drain, 1);
     mbar_init(pair, 4);
@@ -481,7 +573,6 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   ch_plan(a, &plan);                     // ends with a barrier
   tc_after();
   const uint32_t tmem = tmem_s;
-  if (tid == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
 
   // bounded wait: after about a second the CTA records the fault and unwinds
   const auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
@@ -699,9 +790,24 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
         __syncwarp();
         if (lane == 0) mbar_arrive(pair_done);
       }
-      if (!whole && sg.first && tid == 0) {
-        a.meta[blockIdx.x] =
-            make_int4(sg.parts, sg.q0 + sg.tok0, sg.ntok, sg.h);
+      if (!whole && live) {
+        // rows whose last partial this is are joined when the run is done
+        __threadfence();
+        const int n = __popc(__ballot_sync(~0u, valid));
+        if (lane == 0) {
+          int32_t* ticket = a.tickets + sg.cta0 * 8 + warp;
+          if (atomicAdd(ticket, 1) == sg.parts - 1) {
+            *ticket = 0;
+            ChJob& b = jobs[atomicAdd(&n_jobs, 1)];
+            b.cta0 = sg.cta0;
+            b.parts = sg.parts;
+            b.h = sg.h;
+            b.n = n;
+            b.row0 = (two ? t : 0) * 128 + (warp & 3) * 32;
+            b.tok0 = (two ? t * tm : 0) + sg.q0 + sg.tok0;
+          }
+        }
+        __syncwarp();
       }
     }
   } else {
@@ -933,67 +1039,21 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
                  :: "r"(tmem), "r"(X::kCols));
   }
-}
-
-// Joins the partials of the item that starts in CTA blockIdx.x's run and ends
-// in a later one: out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c.  One
-// thread per row and 16 columns.
-template <int D, bool kF16>
-__global__ void __launch_bounds__(256) chunk_merge_kernel(const ChunkArgs a) {
-  grid_dep_wait();
-  grid_dep_launch();
-  const int4 mt = a.meta[blockIdx.x];
-  if (mt.x <= 0) return;
-  const int row256 = threadIdx.x, t = row256 >> 7, row = row256 & 127;
-  const int tok = row / a.G, g = row - tok * a.G, tm = 1 << a.tm_log2;
-  const int it = t * tm + tok;
-  if (tok >= tm || it >= mt.z) return;
-  const int64_t p0 = (int64_t)blockIdx.x * 2 + 1;      // then slot 0 of the
-  const int64_t p1 = (int64_t)blockIdx.x * 2 + 2;      // following CTAs
-  float M = -INFINITY;
-  for (int c = 0; c <= mt.x; ++c)
-    M = fmaxf(M, a.ml[(c ? p1 + 2 * (c - 1) : p0) * 256 + row256].x);
-  const float ref = M == -INFINITY ? 0.f : M;
-  const int cg = blockIdx.y * 4;
-  float o[16], l = 0.f;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) o[e] = 0.f;
-#pragma unroll 2
-  for (int c = 0; c <= mt.x; ++c) {
-    const int64_t p = c ? p1 + 2 * (c - 1) : p0;
-    const float2 ml = a.ml[p * 256 + row256];
-    const float w = ex2_approx(ml.x - ref);
-    l += w * ml.y;
-    const float4* x = reinterpret_cast<const float4*>(a.acc) +
-                      (p * (D / 4) + cg) * 256 + row256;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float4 v = x[e * 256];
-      o[4 * e] += w * v.x;
-      o[4 * e + 1] += w * v.y;
-      o[4 * e + 2] += w * v.z;
-      o[4 * e + 3] += w * v.w;
+  // the jobs' column blocks, over all warps: few rows come in many partials,
+  // many rows in few
+  __threadfence();
+  int at = 0;
+  for (int k = 0; k < n_jobs; ++k) {
+    const ChJob b = jobs[k];
+    const int sh = b.n <= 1 ? 0 : 32 - __clz(b.n - 1);
+    const bool few = sh <= 2;
+    const int by = (32 >> sh) * (few ? 1 : 4);
+    for (int cg = 0; cg < D / 4; cg += by, ++at) {
+      if (at % (kChThreads / 32) != warp) continue;
+      if (few) ch_join<D, kF16, 1, 8>(a, b, sh, cg);
+      else ch_join<D, kF16, 4, 4>(a, b, sh, cg);
     }
   }
-  const bool some = l > 0.f || l != l;
-  const float inv = some ? 1.f / l : 0.f;
-  const int head = mt.w * a.G + g;
-  const int64_t token = mt.y + it;
-  uint4* dst = reinterpret_cast<uint4*>(
-      (char*)a.out + 2 * (token * a.o_st + head * a.o_sh + cg * 4));
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    uint32_t w[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const float lo = o[8 * e + 2 * x] * inv, hi = o[8 * e + 2 * x + 1] * inv;
-      w[x] = kF16 ? pack_h2(lo, hi) : pack_bf2(lo, hi);
-    }
-    dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  if (a.lse && blockIdx.y == 0)
-    a.lse[token * (a.n_kv * a.G) + head] =
-        some ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
 }
 
 // ------------------------------------------------------------------- host --
@@ -1050,11 +1110,8 @@ int chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk,
                            cudaFuncAttributeMaxDynamicSharedMemorySize,
                            X::kSmem) != cudaSuccess)
     return AMASS_ERR_CUDA;
-  const int rc = launch_pdl(chunk_kernel<D, kF16>, dim3(ctas),
-                            dim3(kChThreads), X::kSmem, st, mq, mk, mv, a);
-  if (rc) return rc;
-  return launch_pdl(chunk_merge_kernel<D, kF16>, dim3(ctas, D / 16),
-                    dim3(256), 0, st, a);
+  return launch_pdl(chunk_kernel<D, kF16>, dim3(ctas), dim3(kChThreads),
+                    X::kSmem, st, mq, mk, mv, a);
 }
 
 }  // namespace
@@ -1072,7 +1129,7 @@ extern "C" int amass_paged_chunk(const AmassChunk* args, void* stream) {
     return AMASS_ERR_ARG;
   if (x.n_tokens == 0 || x.n_req == 0) return AMASS_OK;
   if (!x.q || !x.k || !x.v || !x.block_table || !x.seq_lens ||
-      !x.query_start_loc || !x.acc_part || !x.ml_part || !x.meta ||
+      !x.query_start_loc || !x.acc_part || !x.ml_part || !x.tickets ||
       !x.fault || !x.out)
     return AMASS_ERR_ARG;
   if ((x.head_dim != 64 && x.head_dim != 128) || x.G > 8 || x.page != kPg ||
@@ -1081,7 +1138,7 @@ extern "C" int amass_paged_chunk(const AmassChunk* args, void* stream) {
   // TMA and 16-byte stores: 16-byte aligned bases and strides
   const uintptr_t bases = (uintptr_t)x.q | (uintptr_t)x.k | (uintptr_t)x.v |
                           (uintptr_t)x.out | (uintptr_t)x.acc_part |
-                          (uintptr_t)x.ml_part | (uintptr_t)x.meta;
+                          (uintptr_t)x.ml_part;
   if ((bases & 15) || ((x.o_st | x.o_sh) & 7)) return AMASS_ERR_ARG;
   const uint64_t d = (uint64_t)x.head_dim;
   const uint64_t qdim[3] = {d, (uint64_t)(x.n_kv * x.G),
@@ -1119,7 +1176,7 @@ extern "C" int amass_paged_chunk(const AmassChunk* args, void* stream) {
   a.qsl = x.query_start_loc; a.out = x.out; a.o_st = x.o_st; a.o_sh = x.o_sh;
   a.lse = x.lse; a.acc = x.acc_part;
   a.ml = reinterpret_cast<float2*>(x.ml_part);
-  a.meta = reinterpret_cast<int4*>(x.meta); a.fault = x.fault;
+  a.tickets = x.tickets; a.fault = x.fault;
   a.scale_log2 = x.scale * kLog2e;
   a.n_req = x.n_req; a.n_kv = x.n_kv; a.G = x.G; a.T = x.n_tokens;
   a.bh = (int)bh; a.max_pages = x.max_pages; a.nb = x.num_blocks; a.window = x.window;
