@@ -422,6 +422,9 @@ AMASS_DEV void ch_plan(const ChunkArgs& a, ChPlan* out) {
   __syncthreads();
 }
 
+constexpr int kFewRows = 8;              // of a warp: joined by all warps
+constexpr int kStage = 4096;             // a warp's 32 rows x 64 columns
+
 template <int D>
 struct ChShape {
   static constexpr int kPanels = D / 64;
@@ -431,11 +434,37 @@ struct ChShape {
   // by side, so that one copy brings a whole page
   static constexpr int kRows8 = kPanels * 1024;
   static constexpr int kPage = 2 * kRows8;
-  static constexpr int kStages = 163840 / kTile;     // 160 KB of ring
-  static constexpr int kSmem = 2 * kTile + kStages * kTile + 1024;
+  static constexpr int kStages = 131072 / kTile;     // 128 KB of ring
+  static constexpr int kOut = 2 * kTile + kStages * kTile;   // staged rows
+  static constexpr int kSmem = kOut + 8 * kStage + 1024;
   static constexpr uint32_t kCols = 512;             // 2 S/P + 2 O
   static constexpr uint32_t kO = 256;
 };
+
+// Lane r's row of 64 16-bit values goes through 4 KB of shared memory, 16
+// bytes at a time (chunk c of 8), so that eight lanes write a row's 128 bytes
+// together: a store of 32 rows is 32 cycles of the load/store unit, one of 4
+// full lines 4.
+AMASS_DEV void stage_put(uint32_t stage, int c, uint4 v) {
+  const uint32_t r = threadIdx.x & 31;
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+               :: "r"(stage + r * 128 + ((c ^ (r & 7)) << 4)), "r"(v.x),
+                  "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// row: where the lane's 128 bytes go, null for nowhere
+AMASS_DEV void stage_out(uint32_t stage, char* row) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t r = i * 4 + (lane >> 3), c = lane & 7;
+    char* p = reinterpret_cast<char*>(__shfl_sync(
+        ~0u, reinterpret_cast<unsigned long long>(row), (int)r));
+    const uint4 v = lds128(stage + r * 128 + ((c ^ (r & 7)) << 4));
+    if (p) *reinterpret_cast<uint4*>(p + c * 16) = v;
+  }
+  __syncwarp();
+}
 
 // The rows of one warp of a cut item whose last partial was written here.
 struct ChJob {
@@ -443,26 +472,14 @@ struct ChJob {
   int n, row0, tok0;                     // rows, first of the item's 256, token
 };                                       // of its row tile's row 0
 
-// out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over the item's CTAs in
-// order (the same result whichever CTA finishes last), by one warp: lanes are
-// spread over 2^sh >= n rows, then over groups of 4 columns; NC such blocks
-// from cg on, NP partials' loads in flight for each.
-template <int D, bool kF16, int NC, int NP>
-AMASS_DEV void ch_join(const ChunkArgs& a, const ChJob& b, int sh, int cg) {
-  const int lane = threadIdx.x & 31, r = lane & ((1 << sh) - 1);
-  const int by = 32 >> sh;
-  cg += lane >> sh;
-  if (r >= b.n) return;
-  const int row = b.row0 + r, tok = (row & 127) / a.G;
-  const float2* ml = a.ml + (int64_t)b.cta0 * 512 + row;
-  const float4* x = reinterpret_cast<const float4*>(a.acc) +
-                    ((int64_t)b.cta0 * 2 * (D / 4) + cg) * 256 + row;
-  float4 o[NC];
+// Joining: out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over the item's
+// CTAs in order (the same result whichever CTA finishes last).
+struct ChSum {
   float M = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int k = 0; k < NC; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-  for (int c0 = 0; c0 < b.parts; c0 += NP) {
+  // adds NP partials from c0 on of NC groups of 4 columns
+  template <int D, int NC, int NP>
+  AMASS_DEV void add(const ChJob& b, const float2* ml, const float4* x,
+                     int c0, float4* o) {
     float4 v[NP][NC];
     float2 z[NP];
     // the first CTA's partial is its second slot, the others' their first
@@ -474,8 +491,8 @@ AMASS_DEV void ch_join(const ChunkArgs& a, const ChJob& b, int sh, int cg) {
 #pragma unroll
       for (int k = 0; k < NC; ++k) {
         v[e][k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < b.parts && cg + k * by < D / 4)
-          v[e][k] = __ldcg(x + ((int64_t)s * (D / 4) + k * by) * 256);
+        if (c < b.parts)
+          v[e][k] = __ldcg(x + ((int64_t)s * (D / 4) + k) * 256);
       }
     }
 #pragma unroll
@@ -493,23 +510,72 @@ AMASS_DEV void ch_join(const ChunkArgs& a, const ChJob& b, int sh, int cg) {
       }
     }
   }
-  const bool some = l > 0.f || l != l;
-  const float inv = some ? 1.f / l : 0.f;
+  AMASS_DEV bool some() const { return l > 0.f || l != l; }
+  AMASS_DEV float inv() const { return some() ? 1.f / l : 0.f; }
+  AMASS_DEV float lse() const {
+    return some() ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  }
+};
+template <bool kF16>
+AMASS_DEV uint2 pack4(float4 o, float f) {
+  return kF16 ? make_uint2(pack_h2(o.x * f, o.y * f), pack_h2(o.z * f, o.w * f))
+              : make_uint2(pack_bf2(o.x * f, o.y * f),
+                           pack_bf2(o.z * f, o.w * f));
+}
+// where row `row` of the job's item goes
+AMASS_DEV char* ch_out(const ChunkArgs& a, const ChJob& b, int row,
+                       int64_t* lse) {
+  const int tok = (row & 127) / a.G;
   const int64_t token = b.tok0 + tok;
   const int head = b.h * a.G + (row & 127) - tok * a.G;
-  char* out = (char*)a.out + 2 * (token * a.o_st + head * a.o_sh);
+  *lse = token * (a.n_kv * a.G) + head;
+  return (char*)a.out + 2 * (token * a.o_st + head * a.o_sh);
+}
+// Few rows (2^sh >= n), many partials: lanes over rows, then over groups of 4
+// columns from cg on, 8 partials in flight.
+template <int D, bool kF16>
+AMASS_DEV void ch_join_few(const ChunkArgs& a, const ChJob& b, int sh, int cg) {
+  const int lane = threadIdx.x & 31, r = lane & ((1 << sh) - 1);
+  cg += lane >> sh;
+  if (r >= b.n) return;
+  const int row = b.row0 + r;
+  const float2* ml = a.ml + (int64_t)b.cta0 * 512 + row;
+  const float4* x = reinterpret_cast<const float4*>(a.acc) +
+                    ((int64_t)b.cta0 * 2 * (D / 4) + cg) * 256 + row;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  ChSum s;
+  for (int c = 0; c < b.parts; c += 8) s.template add<D, 1, 8>(b, ml, x, c, &o);
+  int64_t li;
+  char* out = ch_out(a, b, row, &li);
+  *reinterpret_cast<uint2*>(out + 8 * cg) = pack4<kF16>(o, s.inv());
+  if (a.lse && cg == 0) a.lse[li] = s.lse();
+}
+// A lane per row, 64 columns from 64 half on: two partials' 64 columns in
+// flight.
+template <int D, bool kF16>
+AMASS_DEV void ch_join_many(const ChunkArgs& a, const ChJob& b, int half,
+                            uint32_t stage) {
+  const int lane = threadIdx.x & 31, row = b.row0 + min(lane, b.n - 1);
+  const float2* ml = a.ml + (int64_t)b.cta0 * 512 + row;
+  const float4* x = reinterpret_cast<const float4*>(a.acc) +
+                    ((int64_t)b.cta0 * 2 * (D / 4) + half * 16) * 256 + row;
+  float4 o[16];
+  ChSum s;
 #pragma unroll
-  for (int k = 0; k < NC; ++k) {
-    if (cg + k * by >= D / 4) continue;
-    const float x0 = o[k].x * inv, x1 = o[k].y * inv;
-    const float x2 = o[k].z * inv, x3 = o[k].w * inv;
-    *reinterpret_cast<uint2*>(out + 8 * (cg + k * by)) =
-        kF16 ? make_uint2(pack_h2(x0, x1), pack_h2(x2, x3))
-             : make_uint2(pack_bf2(x0, x1), pack_bf2(x2, x3));
+  for (int e = 0; e < 16; ++e) o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int c = 0; c < b.parts; c += 2)
+    s.template add<D, 16, 2>(b, ml, x, c, o);
+  const float f = s.inv();
+#pragma unroll
+  for (int e = 0; e < 16; e += 2) {
+    const uint2 lo = pack4<kF16>(o[e], f), hi = pack4<kF16>(o[e + 1], f);
+    stage_put(stage, e / 2, make_uint4(lo.x, lo.y, hi.x, hi.y));
   }
-  if (a.lse && cg == 0)
-    a.lse[token * (a.n_kv * a.G) + head] =
-        some ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  int64_t li;
+  char* out = ch_out(a, b, row, &li);
+  if (a.lse && half == 0 && lane < b.n) a.lse[li] = s.lse();
+  stage_out(stage, lane < b.n ? out + half * 128 : nullptr);
 }
 
 template <int D, bool kF16>
@@ -522,8 +588,8 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   extern __shared__ uint8_t dyn[];
   __shared__ __align__(8) uint64_t bars[2 * NS + 16];
   __shared__ float2 ml_s[128];           // warpgroup 1's (m, l), one-tile items
-  __shared__ ChJob jobs[16];             // a run cuts two items, 8 warps' rows
-  __shared__ int n_jobs;
+  __shared__ ChJob jobs[16];             // a run cuts two items: 8 warps' rows
+  __shared__ int few[16], n_few;         // jobs of few rows
   __shared__ ChPlan plan;
   __shared__ uint32_t tmem_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -553,7 +619,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       mbar_init(p_full + 8 * t, 4);
       mbar_init(o_full + 8 * t, 1);
     }
-    n_jobs = 0;
+    n_few = 0;
     mbar_init(v_tmp, 1);
     mbar_init(drain, 1);
     mbar_init(pair, 4);
@@ -599,9 +665,11 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
     const uint32_t ts = tmem + t * 128 + lanes;
     const uint32_t to = tmem + X::kO + t * D + lanes;
     const int tok = row / a.G, g = row - tok * a.G, tm = 1 << a.tm_log2;
+    const uint32_t stage = base + X::kOut + warp * kStage;
     const float sl2 = a.scale_log2;
     const uint64_t sl2x2 = f2(sl2, sl2);
     uint32_t sph = 0, oph = 0, cph = 0;
+    int mine = 0;                        // this warp's jobs
     bool ok = true;
     while (ok && wk.next(a, plan, sg)) {
       const bool two = sg.ntok > tm;
@@ -756,7 +824,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
               o[e] = __float_as_uint(fmaf(__uint_as_float(o1[e]), f1,
                                           __uint_as_float(o[e])));
           }
-          if (valid && whole) {
+          if (whole) {
             uint32_t w[8];
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
@@ -764,9 +832,11 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
               const float hi = __uint_as_float(o[2 * x + 1]);
               w[x] = kF16 ? pack_h2(lo, hi) : pack_bf2(lo, hi);
             }
-            uint4* d = reinterpret_cast<uint4*>(orow + 2 * c);
-            d[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            const int k = (c & 63) / 8;
+            stage_put(stage, k, make_uint4(w[0], w[1], w[2], w[3]));
+            stage_put(stage, k + 1, make_uint4(w[4], w[5], w[6], w[7]));
+            if (k == 6)
+              stage_out(stage, valid ? orow + 2 * (c - 48) : nullptr);
           } else if (valid) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
@@ -794,21 +864,32 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
         // rows whose last partial this is are joined when the run is done
         __threadfence();
         const int n = __popc(__ballot_sync(~0u, valid));
+        int joins = 0;
         if (lane == 0) {
           int32_t* ticket = a.tickets + sg.cta0 * 8 + warp;
           if (atomicAdd(ticket, 1) == sg.parts - 1) {
             *ticket = 0;
-            ChJob& b = jobs[atomicAdd(&n_jobs, 1)];
+            ChJob& b = jobs[warp * 2 + mine];
             b.cta0 = sg.cta0;
             b.parts = sg.parts;
             b.h = sg.h;
             b.n = n;
             b.row0 = (two ? t : 0) * 128 + (warp & 3) * 32;
             b.tok0 = (two ? t * tm : 0) + sg.q0 + sg.tok0;
+            joins = 1;
+            if (n <= kFewRows) few[atomicAdd(&n_few, 1)] = warp * 2 + mine;
           }
         }
-        __syncwarp();
+        mine += __shfl_sync(~0u, joins, 0);
       }
+    }
+    __threadfence();
+    for (int k = 0; k < mine; ++k) {
+      const ChJob b = jobs[warp * 2 + k];
+      if (b.n <= kFewRows) continue;
+#pragma unroll 1
+      for (int half = 0; half < X::kPanels; ++half)
+        ch_join_many<D, kF16>(a, b, half, stage);
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
@@ -1039,19 +1120,16 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
                  :: "r"(tmem), "r"(X::kCols));
   }
-  // the jobs' column blocks, over all warps: few rows come in many partials,
-  // many rows in few
+  // few rows of many partials: column blocks over all warps
   __threadfence();
-  int at = 0;
-  for (int k = 0; k < n_jobs; ++k) {
-    const ChJob b = jobs[k];
+  int at = warp;
+  for (int k = 0; k < n_few; ++k) {
+    const ChJob b = jobs[few[k]];
     const int sh = b.n <= 1 ? 0 : 32 - __clz(b.n - 1);
-    const bool few = sh <= 2;
-    const int by = (32 >> sh) * (few ? 1 : 4);
-    for (int cg = 0; cg < D / 4; cg += by, ++at) {
-      if (at % (kChThreads / 32) != warp) continue;
-      if (few) ch_join<D, kF16, 1, 8>(a, b, sh, cg);
-      else ch_join<D, kF16, 4, 4>(a, b, sh, cg);
+    for (int cg = 0; cg < D / 4; cg += 32 >> sh) {
+      if (at-- != 0) continue;
+      at = kChThreads / 32 - 1;
+      ch_join_few<D, kF16>(a, b, sh, cg);
     }
   }
 }
