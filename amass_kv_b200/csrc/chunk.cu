@@ -15,6 +15,7 @@
 //                   a page (a copy takes some 80-100 cycles of the TMA unit
 //                   whatever its size: at one per page and 64 columns K and V
 //                   came at 26 bytes a cycle, the tensor core wants 32)
+//   warp 10         walks the run and tells the others its pieces
 //   warp 9          issues the tcgen05 MMAs: S = Q K^T (both operands in
 //                   shared memory, fp32 S in TMEM), O += P V (P in TMEM over
 //                   S's columns, V as a column-major operand, fp32 O in TMEM)
@@ -267,17 +268,19 @@ AMASS_DEV int64_t ch_cost(const ChunkArgs& a, const ChReq& q, int m) {
   return s + u * kCost2;
 }
 
-struct ChSeg {
-  int r, h, q0, tok0, ntok, off, sl, t0, n;
-  int cta0, parts;                       // a cut item's CTAs
-  bool first, last;
+// A piece of an item: key tiles [t0, t0 + n) for ntok tokens from tok0 on;
+// first / last: with the item's first / last key tile; n = 0 ends the run.
+struct alignas(16) ChSeg {
+  int r, h, tok0, ntok;                  // request, kv head; row in q
+  int pos0, sl, t0, n;                   // position of tok0, tokens, tiles
+  int first, last, cta0, parts;          // a cut item's CTAs
 };
 struct ChPlan {
   ChReq q;
   int r, h, i, from, to, share;          // run [from, to) from item i's start
 };
 
-// Walks the segments of a CTA's run; every role keeps its own copy.  Key tile
+// Walks the segments of a CTA's run (one warp does, a few ahead of the others).  Key tile
 // k of an item belongs to the CTA whose run holds its place, item start + k *
 // weight.  A first segment that starts inside its item goes last: then every
 // CTA starts at its item's first key tile, and since the runs are equally
@@ -331,14 +334,16 @@ struct ChWalk {
       return w == kCost2 ? (c + kCost2 - 1) / kCost2 : (c + kCost1 - 1) / kCost1;
     };
     const int k0 = tiles(from), k1 = to >= nu * w ? nu : tiles(to);
-    if (k0 >= k1) return false;          // a run inside an item's overhead
-    s.r = r; s.h = h; s.q0 = q.q0; s.off = q.off; s.sl = q.sl;
-    s.tok0 = i << tl;
-    s.ntok = min(1 << tl, q.ql - s.tok0);
+    if (k0 >= k1) return false;          // a run inside an item's overhead (s.n = 0)
+    s.r = r; s.h = h; s.sl = q.sl;
+    s.tok0 = q.q0 + (i << tl);
+    s.pos0 = q.off + (i << tl);
+    s.ntok = min(1 << tl, q.ql - (i << tl));
     s.t0 = lo + k0;
     s.n = k1 - k0;
     s.first = k0 == 0;
     s.last = k1 == nu;
+    s.cta0 = s.parts = 0;
     if (!(s.first && s.last)) {          // floor divisions by the run length
       const int b = at < 0 ? -((p.share - 1 - at) / p.share) : 0;
       s.cta0 = (int)blockIdx.x + b;
@@ -422,6 +427,7 @@ AMASS_DEV void ch_plan(const ChunkArgs& a, ChPlan* out) {
   __syncthreads();
 }
 
+constexpr int kSegs = 4;
 constexpr int kFewRows = 8;              // of a warp: joined by all warps
 constexpr int kStage = 4096;             // a warp's 32 rows x 64 columns
 
@@ -454,15 +460,22 @@ AMASS_DEV void stage_put(uint32_t stage, int c, uint4 v) {
 // row: where the lane's 128 bytes go, null for nowhere
 AMASS_DEV void stage_out(uint32_t stage, char* row) {
   const int lane = threadIdx.x & 31;
+  const uint32_t c = lane & 7;
+  unsigned long long p[8];
+  uint4 v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    p[i] = __shfl_sync(~0u, reinterpret_cast<unsigned long long>(row),
+                       i * 4 + (lane >> 3));
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint32_t r = i * 4 + (lane >> 3), c = lane & 7;
-    char* p = reinterpret_cast<char*>(__shfl_sync(
-        ~0u, reinterpret_cast<unsigned long long>(row), (int)r));
-    const uint4 v = lds128(stage + r * 128 + ((c ^ (r & 7)) << 4));
-    if (p) *reinterpret_cast<uint4*>(p + c * 16) = v;
+    const uint32_t r = i * 4 + (lane >> 3);
+    v[i] = lds128(stage + r * 128 + ((c ^ (r & 7)) << 4));
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (p[i]) *reinterpret_cast<uint4*>(p[i] + c * 16) = v[i];
   __syncwarp();
 }
 
@@ -586,11 +599,11 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   using X = ChShape<D>;
   constexpr int NS = X::kStages;
   extern __shared__ uint8_t dyn[];
-  __shared__ __align__(8) uint64_t bars[2 * NS + 16];
-  __shared__ float2 ml_s[128];           // warpgroup 1's (m, l), one-tile items
+  __shared__ __align__(8) uint64_t bars[2 * NS + 16 + 2 * kSegs];
   __shared__ ChJob jobs[16];             // a run cuts two items: 8 warps' rows
   __shared__ int few[16], n_few;         // jobs of few rows
   __shared__ ChPlan plan;
+  __shared__ ChSeg segs[kSegs];          // the walk, a few pieces ahead
   __shared__ uint32_t tmem_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -605,6 +618,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   const uint32_t p_full = q_full + 64, o_full = q_full + 80;
   const uint32_t v_tmp = q_full + 96, drain = v_tmp + 8;
   const uint32_t pair = v_tmp + 16, pair_done = v_tmp + 24;
+  const uint32_t seg_full = v_tmp + 32, seg_empty = seg_full + 8 * kSegs;
 
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
@@ -622,6 +636,10 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
     n_few = 0;
     mbar_init(v_tmp, 1);
     mbar_init(drain, 1);
+    for (int s = 0; s < kSegs; ++s) {
+      mbar_init(seg_full + 8 * s, 1);
+      mbar_init(seg_empty + 8 * s, 10);  // softmax, producer, MMA warps
+    }
     mbar_init(pair, 4);
     mbar_init(pair_done, 4);
     mbar_init_fence();
@@ -651,9 +669,19 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
     return __all_sync(~0u, wait(bar, parity));
   };
 
-  ChWalk wk;
-  wk.start(a, plan);
+  // the run's next piece; false at its end
   ChSeg sg;
+  int seg_at = 0;
+  bool ok = true;
+  const auto next_seg = [&]() -> bool {
+    const int k = seg_at++;
+    if (!(ok = wait_warp(seg_full + 8 * (k % kSegs), (k / kSegs) & 1)))
+      return false;
+    sg = segs[k % kSegs];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(seg_empty + 8 * (k % kSegs));
+    return sg.n > 0;
+  };
 
   // a softmax thread holds a row of 128 scores: 384 * 168 registers at launch
   // = 128 * (2 * 192 + 120)
@@ -666,16 +694,20 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
     const uint32_t to = tmem + X::kO + t * D + lanes;
     const int tok = row / a.G, g = row - tok * a.G, tm = 1 << a.tm_log2;
     const uint32_t stage = base + X::kOut + warp * kStage;
+    // warpgroup 1's (m, l) of an item it shares with warpgroup 0: in its own
+    // stage, which it does not use then
+    float2* pair_ml = reinterpret_cast<float2*>(
+        dyn + (base - smem_u32(dyn)) + X::kOut + (4 + (warp & 3)) * kStage) +
+        lane;
     const float sl2 = a.scale_log2;
     const uint64_t sl2x2 = f2(sl2, sl2);
     uint32_t sph = 0, oph = 0, cph = 0;
     int mine = 0;                        // this warp's jobs
-    bool ok = true;
-    while (ok && wk.next(a, plan, sg)) {
+    while (ok && next_seg()) {
       const bool two = sg.ntok > tm;
       const int it = (two ? t * tm : 0) + tok;   // token within the item
       const bool valid = tok < tm && it < sg.ntok;
-      const int pos = sg.off + sg.tok0 + it;
+      const int pos = sg.pos0 + it;
       // rows of nobody compute on whatever Q's buffer holds, unmasked
       const int khi = valid ? max(pos + 1, 0) : 0x7fffffff;
       const int klo = valid && a.window ? max(pos - a.window + 1, 0) : 0;
@@ -773,11 +805,11 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       }
       if (!two && t == 1) {
         if (!paired) continue;
-        ml_s[row] = make_float2(m, l);
+        *pair_ml = make_float2(m, l);
         tc_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(pair);
-        // warpgroup 0 reads O_1 and ml_s until then
+        // warpgroup 0 reads O_1 and (m, l) until then
         if (!(ok = wait_warp(pair_done, cph))) break;
         cph ^= 1;
         continue;
@@ -787,7 +819,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
         if (!(ok = wait_warp(pair, cph))) break;
         cph ^= 1;
         tc_after();
-        const float2 o = ml_s[row];
+        const float2 o = *pair_ml;
         const float mn = fmax_nan(m, o.x), ref = mn == -INFINITY ? 0.f : mn;
         f0 = ex2_approx((m - ref) * sl2);
         f1 = ex2_approx((o.x - ref) * sl2);
@@ -801,45 +833,47 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       const float inv = !whole ? 1.f : some ? 1.f / l : 0.f;
       f0 *= inv;
       f1 *= inv;
-      const int token = sg.q0 + sg.tok0 + it;
+      const int token = sg.tok0 + it;
       char* orow = (char*)a.out + 2 * ((int64_t)token * a.o_st +
                                        (int64_t)(sg.h * a.G + g) * a.o_sh);
       float4* prow = reinterpret_cast<float4*>(a.acc) + part * (D / 4) * 256 +
                      (two ? t : 0) * 128 + row;
       if (live) {
 #pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-          uint32_t o[16];
-          tc_ld16(o, to + c);
+        for (int c = 0; c < D; c += 64) {
+          uint32_t o[64];
+          tc_ld32(o, to + c);
+          tc_ld32(o + 32, to + c + 32);
           tc_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
+          for (int e = 0; e < 64; ++e)
             o[e] = __float_as_uint(__uint_as_float(o[e]) * f0);
           if (paired) {
-            uint32_t o1[16];
-            tc_ld16(o1, to + D + c);
+            uint32_t o1[64];
+            tc_ld32(o1, to + D + c);
+            tc_ld32(o1 + 32, to + D + c + 32);
             tc_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
+            for (int e = 0; e < 64; ++e)
               o[e] = __float_as_uint(fmaf(__uint_as_float(o1[e]), f1,
                                           __uint_as_float(o[e])));
           }
           if (whole) {
-            uint32_t w[8];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const float lo = __uint_as_float(o[2 * x]);
-              const float hi = __uint_as_float(o[2 * x + 1]);
-              w[x] = kF16 ? pack_h2(lo, hi) : pack_bf2(lo, hi);
+            for (int k = 0; k < 8; ++k) {
+              uint32_t w[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float lo = __uint_as_float(o[8 * k + 2 * x]);
+                const float hi = __uint_as_float(o[8 * k + 2 * x + 1]);
+                w[x] = kF16 ? pack_h2(lo, hi) : pack_bf2(lo, hi);
+              }
+              stage_put(stage, k, make_uint4(w[0], w[1], w[2], w[3]));
             }
-            const int k = (c & 63) / 8;
-            stage_put(stage, k, make_uint4(w[0], w[1], w[2], w[3]));
-            stage_put(stage, k + 1, make_uint4(w[4], w[5], w[6], w[7]));
-            if (k == 6)
-              stage_out(stage, valid ? orow + 2 * (c - 48) : nullptr);
+            stage_out(stage, valid ? orow + 2 * c : nullptr);
           } else if (valid) {
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
+            for (int e = 0; e < 64; e += 4)
               prow[(c + e) / 4 * 256] = make_float4(
                   __uint_as_float(o[e]), __uint_as_float(o[e + 1]),
                   __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
@@ -875,7 +909,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
             b.h = sg.h;
             b.n = n;
             b.row0 = (two ? t : 0) * 128 + (warp & 3) * 32;
-            b.tok0 = (two ? t * tm : 0) + sg.q0 + sg.tok0;
+            b.tok0 = (two ? t * tm : 0) + sg.tok0;
             joins = 1;
             if (n <= kFewRows) few[atomicAdd(&n_few, 1)] = warp * 2 + mine;
           }
@@ -897,8 +931,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       // ------------------------------------------------------------ producer
       int st = 0;
       uint32_t ph = 1, qph = 3, vph = 0;
-      bool ok = true;
-      while (ok && wk.next(a, plan, sg)) {
+      while (ok && next_seg()) {
         const int tm = 1 << a.tm_log2;
         for (int t = 0; ok && t < (sg.ntok > tm ? 2 : 1); ++t) {
           if (!(ok = wait_warp(q_empty + 8 * t, (qph >> t) & 1))) break;
@@ -907,7 +940,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
             mbar_arrive_expect_tx(q_full + 8 * t, X::kPanels * 128u * a.G * tm);
             for (int p = 0; p < X::kPanels; ++p)
               tma_3d(q_s + t * X::kTile + p * X::kPanel, &mq, q_full + 8 * t,
-                     p * 64, sg.h * a.G, sg.q0 + sg.tok0 + t * tm);
+                     p * 64, sg.h * a.G, sg.tok0 + t * tm);
           }
         }
         if (!ok) break;
@@ -994,7 +1027,6 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       const uint64_t vd = smem_desc(ring, 1024, X::kRows8);
       int st = 0;                        // the next ring entry and its phase
       uint32_t ph = 0, qph = 0, pph = 0;
-      bool ok = true;
       const auto score = [&](int t, uint64_t q0, uint64_t k0, int k) {
         mma_ss(tmem + t * 128, q0 + (((k >> 2) * X::kPanel + (k & 3) * 32) >> 4),
                k0 + (((k >> 2) * 1024 + (k & 3) * 32) >> 4), id_s, k > 0);
@@ -1068,7 +1100,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       const auto scores_of = [&](int t, uint64_t q0, int e, bool done) {
         scores(t, q0, e >= NS ? e - NS : e, done);
       };
-      while (ok && wk.next(a, plan, sg)) {
+      while (ok && next_seg()) {
         const int n = sg.n;
         const bool two = sg.ntok > (1 << a.tm_log2);
         const int k0 = take();
@@ -1111,6 +1143,18 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       // every MMA and its arrivals end before the CTA does
       commit(drain);
       (void)wait_warp(drain, 0);
+    } else if (warp == 10 && lane == 0) {
+      // ------------------------------------------------------------- walk
+      ChWalk wk;
+      wk.start(a, plan);
+      for (int k = 0;; ++k) {
+        ChSeg s = {};
+        const bool more = wk.next(a, plan, s);
+        if (!wait(seg_empty + 8 * (k % kSegs), ((k / kSegs) & 1) ^ 1)) break;
+        segs[k % kSegs] = s;
+        mbar_arrive(seg_full + 8 * (k % kSegs));
+        if (!more) break;
+      }
     }
   }
   tc_before();
