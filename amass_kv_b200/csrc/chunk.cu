@@ -160,6 +160,51 @@ AMASS_DEV void tc_st16(uint32_t t, const uint32_t* r) {
          "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// 16 rows (TMEM lanes) of 128 columns: lane l holds columns 8 j + 2 (l % 4) and
+// the next one of row l / 4 in r[4 j], r[4 j + 1], of row l / 4 + 8 in the
+// other two
+AMASS_DEV void tc_ld_16x256(uint32_t* r, uint32_t t) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, "
+      "[%64];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]),
+        "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
+        "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]),
+        "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]),
+        "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]),
+        "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(t));
+}
+// 16 rows of 64 columns: lane l's column 4 j + l % 4 of rows l / 4 and l / 4 + 8
+AMASS_DEV void tc_st_16x128(uint32_t t, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      :: "r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+         "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+         "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+         "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+         "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+         "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
 AMASS_DEV float fmax_nan(float a, float b) {   // NaN when either is
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -601,7 +646,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   extern __shared__ uint8_t dyn[];
   __shared__ __align__(8) uint64_t bars[2 * NS + 16 + 2 * kSegs];
   __shared__ ChJob jobs[16];             // a run cuts two items: 8 warps' rows
-  __shared__ int few[16], n_few;         // jobs of few rows
+  __shared__ int few_jobs[16], n_few;    // those of few rows
   __shared__ ChPlan plan;
   __shared__ ChSeg segs[kSegs];          // the walk, a few pieces ahead
   __shared__ uint32_t tmem_s;
@@ -711,14 +756,81 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       // rows of nobody compute on whatever Q's buffer holds, unmasked
       const int khi = valid ? max(pos + 1, 0) : 0x7fffffff;
       const int klo = valid && a.window ? max(pos - a.window + 1, 0) : 0;
-      const bool live = __any_sync(~0u, valid);
+      const int rows = __popc(__ballot_sync(~0u, valid));
+      const bool live = rows > 0;
+      // up to eight rows (one token's heads): four lanes share a row, a
+      // quarter of the exponentials and of the code for a lane
+      const bool few = rows <= 8;
+      const int khi4 = __shfl_sync(~0u, khi, lane >> 2);
+      const int klo4 = __shfl_sync(~0u, klo, lane >> 2);
+      const bool valid4 = __shfl_sync(~0u, (int)valid, lane >> 2) != 0;
       const int by = two ? 1 : 2;
+      const auto rescale = [&](float f) {        // row lane of O by f
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          uint32_t o[16];
+          tc_ld16(o, to + c);
+          tc_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tc_st16(to + c, o);
+        }
+      };
       float m = -INFINITY, l = 0.f;
       for (int j = two ? 0 : t; j < sg.n; j += by) {
         if (!(ok = wait_warp(s_full + 8 * t, sph))) break;
         sph ^= 1;
         tc_after();
-        if (live) {
+        if (live && few) {
+          uint32_t s[64];
+          tc_ld_16x256(s, ts);
+          tc_wait_ld();
+          const int k0 = (sg.t0 + j) * kKeys, col = (lane & 3) * 2;
+          if (__any_sync(~0u, khi4 - k0 < kKeys || k0 < klo4)) {
+            const int e = khi4 - k0 - col, b = klo4 - k0 - col;
+#pragma unroll
+            for (int c = 0; c < 128; c += 8) {
+              if (c >= e || c < b) s[c / 2] = 0xff800000u;
+              if (c + 1 >= e || c + 1 < b) s[c / 2 + 1] = 0xff800000u;
+            }
+          }
+          float mx = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 64; c += 4)
+            mx = fmax_nan(fmax_nan(mx, __uint_as_float(s[c])),
+                          __uint_as_float(s[c + 1]));
+          mx = fmax_nan(mx, __shfl_xor_sync(~0u, mx, 1));
+          mx = fmax_nan(mx, __shfl_xor_sync(~0u, mx, 2));
+          if (j < by) {
+            m = mx;
+          } else if (__any_sync(~0u,
+                                valid4 && !((mx - m) * sl2 <= kRescaleLog2))) {
+            const float mn = fmax_nan(m, mx);
+            const float f = m == -INFINITY ? 0.f : ex2_approx((m - mn) * sl2);
+            l *= f;
+            m = mn;
+            rescale(__shfl_sync(~0u, f, (lane & 7) * 4));
+          }
+          const float nm = m == -INFINITY ? 0.f : fmaf(0.f, m, -m * sl2);
+          float sum = 0.f;
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const float p0 =
+                ex2_approx(fmaf(__uint_as_float(s[2 * c]), sl2, nm));
+            const float p1 =
+                ex2_approx(fmaf(__uint_as_float(s[2 * c + 1]), sl2, nm));
+            sum += p0 + p1;
+            s[c] = kF16 ? pack_h2(p0, p1) : pack_bf2(p0, p1);
+            s[c + 1] = 0;
+          }
+          l += sum;
+          tc_st_16x128(ts, s);
+          tc_wait_st();
+          tc_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_part + 8 * t);
+        } else if (live) {
           uint32_t s[128];
 #pragma unroll
           for (int c = 0; c < 4; ++c) tc_ld32(s + 32 * c, ts + 32 * c);
@@ -751,16 +863,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
             const float f = m == -INFINITY ? 0.f : ex2_approx((m - mn) * sl2);
             l *= f;
             m = mn;
-#pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
-              uint32_t o[16];
-              tc_ld16(o, to + c);
-              tc_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tc_st16(to + c, o);
-            }
+            rescale(f);
           }
           // an infinite or NaN score makes the row NaN, as the formula does
           const float nm = m == -INFINITY ? 0.f : fmaf(0.f, m, -m * sl2);
@@ -797,6 +900,12 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
         if (lane == 0) mbar_arrive(p_full + 8 * t);
       }
       if (!ok) break;
+      if (few) {                                 // back to a lane per row
+        l += __shfl_xor_sync(~0u, l, 1);
+        l += __shfl_xor_sync(~0u, l, 2);
+        l = __shfl_sync(~0u, l, (lane & 7) * 4);
+        m = __shfl_sync(~0u, m, (lane & 7) * 4);
+      }
       const bool paired = !two && sg.n > 1;      // both hold part of the rows
       if (t == 0 || two || paired) {
         if (!(ok = wait_warp(o_full + 8 * t, oph))) break;
@@ -911,7 +1020,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
             b.row0 = (two ? t : 0) * 128 + (warp & 3) * 32;
             b.tok0 = (two ? t * tm : 0) + sg.tok0;
             joins = 1;
-            if (n <= kFewRows) few[atomicAdd(&n_few, 1)] = warp * 2 + mine;
+            if (n <= kFewRows) few_jobs[atomicAdd(&n_few, 1)] = warp * 2 + mine;
           }
         }
         mine += __shfl_sync(~0u, joins, 0);
@@ -1168,7 +1277,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   __threadfence();
   int at = warp;
   for (int k = 0; k < n_few; ++k) {
-    const ChJob b = jobs[few[k]];
+    const ChJob b = jobs[few_jobs[k]];
     const int sh = b.n <= 1 ? 0 : 32 - __clz(b.n - 1);
     for (int cg = 0; cg < D / 4; cg += 32 >> sh) {
       if (at-- != 0) continue;
