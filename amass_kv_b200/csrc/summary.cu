@@ -219,7 +219,10 @@ summary_kernel(SumArgs a) {
       int rank = 0;                              // descending rank
       for (int j = 0; j < kPg; ++j) {
         const float lj = sm.A[j][j];
-        rank += (lj > li) || (lj == li && j > lane);
+        // NaN (a page with unwritten keys) counts as the smallest: the ranks
+        // are a permutation whatever the keys, so every idx is set
+        const bool ni = li != li, nj = lj != lj;
+        rank += ni != nj ? ni : (lj > li) || ((lj == li || ni) && j > lane);
       }
       if (rank < r) {
         const int k = r - 1 - rank;
