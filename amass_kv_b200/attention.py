@@ -188,13 +188,17 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
     query_start_loc[r] .. query_start_loc[r + 1] - 1 are the last tokens of
     request r's ``seq_lens[r]``; a row at position p sees the keys
     max(0, p - window + 1) .. p (``window=None``: from 0).  Rows without a
-    key become 0, rows outside every request are left as they are.  ``lse``
-    (T, H) fp32, contiguous, receives the rows' natural log-sum-exp (-inf
-    without a key).  ``n_req = seq_lens.shape[0]``; ``buf`` is a
-    ``ChunkBuffers``.  Cache slots behind a request's last token may hold
-    anything; a NaN or infinity at a position a request has reached may
-    reach any row of its tile, as in a product over the whole tile.
-    One pass, no allocation, no synchronisation."""
+    key (or with nothing but scores of -inf) become 0, rows outside every
+    request are left as they are.  ``lse`` (T, H) fp32, contiguous, receives
+    the rows' natural log-sum-exp (-inf without a key).
+    ``n_req = seq_lens.shape[0]``; ``buf`` is a ``ChunkBuffers``; ``out`` may
+    be ``q``.
+
+    Cache slots behind a request's last token may hold anything.  At a
+    position the request has reached, a NaN or infinite key makes the rows
+    that see it NaN; a NaN or infinite value does so for the rows that see
+    it, and may for earlier rows of the same request.  Block ids outside the
+    cache read as zeros.  One launch, no allocation, no synchronisation."""
     nb, page, n_kv, d, (k_sb, k_st, k_sh), k, v = cache_layout(kv_cache)
     v_sb, v_st, v_sh = k_sb, k_st, k_sh
     dtype, dev = q.dtype, buf.index
@@ -264,5 +268,5 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
         query_start_loc.data_ptr(), *buf.scratch, op,
         0 if lse is None else lse.data_ptr(), q_st, q_sh, k_sb, k_st, k_sh,
         v_sb, v_st, v_sh, block_table.stride(0), o_st, o_sh, scale, nb,
-        buf.n_ctas, window or 0, T, n_req, n_kv, buf.G, d, page, max_pages,
+        buf.n_ctas, min(window or 0, 0x7fffffff), T, n_req, n_kv, buf.G, d, page, max_pages,
         DTYPES[dtype]))

@@ -524,6 +524,15 @@ AMASS_DEV void stage_out(uint32_t stage, char* row) {
   __syncwarp();
 }
 
+// draws a ticket: this warp's earlier stores are visible to whoever draws a
+// later one, the stores before earlier ones to this warp
+AMASS_DEV int draw(int32_t* ticket) {
+  int v;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;"
+               : "=r"(v) : "l"(ticket) : "memory");
+  return v;
+}
+
 // The rows of one warp of a cut item whose last partial was written here.
 struct ChJob {
   int cta0, parts, h;                    // the item's CTAs, its kv head
@@ -590,7 +599,7 @@ AMASS_DEV char* ch_out(const ChunkArgs& a, const ChJob& b, int row,
   return (char*)a.out + 2 * (token * a.o_st + head * a.o_sh);
 }
 // Few rows (2^sh >= n), many partials: lanes over rows, then over groups of 4
-// columns from cg on, 8 partials in flight.
+// columns from cg on, 12 partials in flight.
 template <int D, bool kF16>
 AMASS_DEV void ch_join_few(const ChunkArgs& a, const ChJob& b, int sh, int cg) {
   const int lane = threadIdx.x & 31, r = lane & ((1 << sh) - 1);
@@ -602,7 +611,9 @@ AMASS_DEV void ch_join_few(const ChunkArgs& a, const ChJob& b, int sh, int cg) {
                     ((int64_t)b.cta0 * 2 * (D / 4) + cg) * 256 + row;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   ChSum s;
-  for (int c = 0; c < b.parts; c += 8) s.template add<D, 1, 8>(b, ml, x, c, &o);
+  #pragma unroll 1
+  for (int c = 0; c < b.parts; c += 12)
+    s.template add<D, 1, 12>(b, ml, x, c, &o);
   int64_t li;
   char* out = ch_out(a, b, row, &li);
   *reinterpret_cast<uint2*>(out + 8 * cg) = pack4<kF16>(o, s.inv());
@@ -1005,12 +1016,12 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       }
       if (!whole && live) {
         // rows whose last partial this is are joined when the run is done
-        __threadfence();
-        const int n = __popc(__ballot_sync(~0u, valid));
+        __syncwarp();
+        const int n = rows;
         int joins = 0;
         if (lane == 0) {
           int32_t* ticket = a.tickets + sg.cta0 * 8 + warp;
-          if (atomicAdd(ticket, 1) == sg.parts - 1) {
+          if (draw(ticket) == sg.parts - 1) {
             *ticket = 0;
             ChJob& b = jobs[warp * 2 + mine];
             b.cta0 = sg.cta0;
@@ -1024,9 +1035,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
           }
         }
         mine += __shfl_sync(~0u, joins, 0);
+        __syncwarp();
       }
     }
-    __threadfence();
     for (int k = 0; k < mine; ++k) {
       const ChJob b = jobs[warp * 2 + k];
       if (b.n <= kFewRows) continue;
@@ -1114,9 +1125,12 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
         }
       }
       if (!ok) {
-        // copies in flight end before the CTA does
+        // copies in flight end before the CTA does (a stage or a row tile
+        // that never had one passes at once)
         for (int s = 0; s < NS; ++s)
-          (void)mbar_wait(full(s), s < st ? (ph ^ 1) & 1 : ph & 1);
+          (void)mbar_wait(full(s), s < st ? ph ^ 1 : ph);
+        for (int t = 0; t < 2; ++t)
+          (void)mbar_wait(q_full + 8 * t, (qph >> t) & 1);
       }
     } else if (warp == 9) {
       // --------------------------------------------------------------- MMA
@@ -1274,7 +1288,6 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
                  :: "r"(tmem), "r"(X::kCols));
   }
   // few rows of many partials: column blocks over all warps
-  __threadfence();
   int at = warp;
   for (int k = 0; k < n_few; ++k) {
     const ChJob b = jobs[few_jobs[k]];

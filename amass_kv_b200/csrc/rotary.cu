@@ -24,7 +24,9 @@ namespace {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotMaxDim = 256;
-constexpr int kRotMaxTok = 8;            // tokens of one CTA
+constexpr int kRotMaxTok = 16;           // tokens of one CTA
+constexpr int kBatch = 2;
+constexpr int kRotCtas = 4;              // CTAs an SM holds (64 registers)
 
 struct RotArgs {
   const char *q, *k, *v;
@@ -58,31 +60,26 @@ AMASS_DEV void store1(char* p, float x) {
   *reinterpret_cast<uint16_t*>(p) = (uint16_t)pack2<kF16>(x, 0.f);
 }
 
-// source and destination row of row `row` (q heads, k heads, v heads) of
-// token t; false when there is nothing to write
-AMASS_DEV bool rot_row(const RotArgs& a, int t, int row, int64_t slot,
-                       const char** src, char** dst) {
-  if (row < a.H) {
-    *src = a.q + 2 * (t * a.q_st + row * a.q_sh);
-    *dst = a.qo + 2 * (t * a.qo_st + row * a.qo_sh);
-    return true;
-  }
-  if (slot < 0 || slot >= a.n_slots) return false;
+// row `row` (q heads, k heads, v heads) of token t
+AMASS_DEV const char* rot_src(const RotArgs& a, int t, int row) {
+  if (row < a.H) return a.q + 2 * (t * a.q_st + row * a.q_sh);
+  row -= a.H;
+  if (row < a.n_kv) return a.k + 2 * (t * a.k_st + row * a.k_sh);
+  return a.v + 2 * (t * a.v_st + (row - a.n_kv) * a.v_sh);
+}
+// where it goes; null when there is nothing to write
+AMASS_DEV char* rot_dst(const RotArgs& a, int t, int row, int64_t slot) {
+  if (row < a.H) return a.qo + 2 * (t * a.qo_st + row * a.qo_sh);
+  if (slot < 0 || slot >= a.n_slots) return nullptr;
   const int64_t b = slot / a.page, o = slot - b * a.page;
-  int h = row - a.H;
-  if (h < a.n_kv) {
-    *src = a.k + 2 * (t * a.k_st + h * a.k_sh);
-    *dst = a.kd + 2 * (b * a.kd_sb + o * a.kd_st + h * a.kd_sh);
-  } else {
-    h -= a.n_kv;
-    *src = a.v + 2 * (t * a.v_st + h * a.v_sh);
-    *dst = a.vd + 2 * (b * a.vd_sb + o * a.vd_st + h * a.vd_sh);
-  }
-  return true;
+  row -= a.H;
+  if (row < a.n_kv)
+    return a.kd + 2 * (b * a.kd_sb + o * a.kd_st + row * a.kd_sh);
+  return a.vd + 2 * (b * a.vd_sb + o * a.vd_st + (row - a.n_kv) * a.vd_sh);
 }
 
 template <bool kF16, bool kHalf, bool kVec>
-__global__ void __launch_bounds__(kRotThreads)
+__global__ void __launch_bounds__(kRotThreads, kRotCtas)
 rotary_write_kernel(const __grid_constant__ RotArgs a) {
   grid_dep_wait();
   grid_dep_launch();
@@ -91,80 +88,104 @@ rotary_write_kernel(const __grid_constant__ RotArgs a) {
   __shared__ int64_t slot_s[kRotMaxTok];
   const int t0 = blockIdx.x * a.tok;
   const int nt = min(a.tok, a.T - t0), half = a.rot >> 1;
-  for (int i = threadIdx.x; i < nt * half; i += kRotThreads) {
-    const int j = i / half, p = i - j * half;
-    const int64_t pos = a.pos64
-        ? static_cast<const int64_t*>(a.pos)[t0 + j]
-        : (int64_t)static_cast<const int32_t*>(a.pos)[t0 + j];
-    const uint64_t turn = (uint64_t)pos * a.freq[p];
-    // [-1/2, 1/2) turns: 2^-31 makes half turns of the upper 32 bits
-    const float x = (float)(int32_t)(turn >> 32) * 4.656612873077393e-10f;
-    float s, c;
-    sincospif(x, &s, &c);
-    cs[j][p] = c * a.mscale;
-    sn[j][p] = s * a.mscale;
-  }
-  if ((int)threadIdx.x < nt)
-    slot_s[threadIdx.x] = a.slots ? a.slots[t0 + threadIdx.x]
-                                  : (int64_t)(t0 + threadIdx.x);
-  __syncthreads();
   const int rows = a.H + a.n_kv + (a.v ? a.n_kv : 0);
+  const auto angles = [&]() {            // ends with a barrier
+    for (int i = threadIdx.x; i < nt * half; i += kRotThreads) {
+      const int j = i / half, p = i - j * half;
+      const int64_t pos = a.pos64
+          ? static_cast<const int64_t*>(a.pos)[t0 + j]
+          : (int64_t)static_cast<const int32_t*>(a.pos)[t0 + j];
+      const uint64_t turn = (uint64_t)pos * a.freq[p];
+      // [-1/2, 1/2) turns: 2^-31 makes half turns of the upper 32 bits
+      const float x = (float)(int32_t)(turn >> 32) * 4.656612873077393e-10f;
+      float s, c;
+      sincospif(x, &s, &c);
+      cs[j][p] = c * a.mscale;
+      sn[j][p] = s * a.mscale;
+    }
+    if ((int)threadIdx.x < nt)
+      slot_s[threadIdx.x] = a.slots ? a.slots[t0 + threadIdx.x]
+                                    : (int64_t)(t0 + threadIdx.x);
+    __syncthreads();
+  };
   if (kVec) {
     const int per = a.d >> 4, rper = a.rot >> 4;     // items: row, rotated
-    const int tok_items = rows * per;
-    for (int i = threadIdx.x; i < nt * tok_items; i += kRotThreads) {
-      const int j = i / tok_items, w = i - j * tok_items;
-      const int row = w / per, c = w - row * per;
-      const char* src;
-      char* dst;
-      if (!rot_row(a, t0 + j, row, slot_s[j], &src, &dst)) continue;
-      const bool turn = row < a.H + a.n_kv && c < rper;
-      // byte offsets of the item's two 16-byte words
-      const int o0 = kHalf && turn ? c * 16 : c * 32;
-      const int o1 = kHalf && turn ? o0 + a.rot : o0 + 16;
-      uint4 x = *reinterpret_cast<const uint4*>(src + o0);
-      uint4 y = *reinterpret_cast<const uint4*>(src + o1);
-      if (turn) {
-        const float4* cp = reinterpret_cast<const float4*>(&cs[j][c * 8]);
-        const float4* sp = reinterpret_cast<const float4*>(&sn[j][c * 8]);
-        const float4 c0 = cp[0], c1 = cp[1], s0 = sp[0], s1 = sp[1];
-        const float cv[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-        const float sv[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-        uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
-        if (kHalf) {
+    const int tok_items = rows * per, n = nt * tok_items;
+    // kBatch items of a thread in flight; the first ones' loads run while the
+    // angles are formed
+    for (int i0 = 0; i0 < n; i0 += kBatch * kRotThreads) {
+      uint4 x[kBatch], y[kBatch];
+      int at[kBatch], row[kBatch], tk[kBatch];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 u = unpack2<kF16>(xw[e]), z = unpack2<kF16>(yw[e]);
-            const float ca = cv[2 * e], cb = cv[2 * e + 1];
-            const float sa = sv[2 * e], sb = sv[2 * e + 1];
-            xw[e] = pack2<kF16>(u.x * ca - z.x * sa, u.y * cb - z.y * sb);
-            yw[e] = pack2<kF16>(z.x * ca + u.x * sa, z.y * cb + u.y * sb);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 u = unpack2<kF16>(xw[e]), z = unpack2<kF16>(yw[e]);
-            xw[e] = pack2<kF16>(u.x * cv[e] - u.y * sv[e],
-                                u.y * cv[e] + u.x * sv[e]);
-            yw[e] = pack2<kF16>(z.x * cv[e + 4] - z.y * sv[e + 4],
-                                z.y * cv[e + 4] + z.x * sv[e + 4]);
-          }
-        }
-        x = make_uint4(xw[0], xw[1], xw[2], xw[3]);
-        y = make_uint4(yw[0], yw[1], yw[2], yw[3]);
+      for (int b = 0; b < kBatch; ++b) {
+        const int i = i0 + b * kRotThreads + threadIdx.x;
+        tk[b] = -1;
+        if (i >= n) continue;
+        const int j = i / tok_items, w = i - j * tok_items;
+        row[b] = w / per;
+        const int c = w - row[b] * per;
+        tk[b] = j;
+        // the item's chunk, rotated ones with their sign bit clear
+        at[b] = row[b] < a.H + a.n_kv && c < rper ? c : ~c;
+        const char* src = rot_src(a, t0 + j, row[b]);
+        const bool pair = kHalf && at[b] >= 0;
+        const int o0 = pair ? c * 16 : c * 32, o1 = pair ? o0 + a.rot : o0 + 16;
+        x[b] = *reinterpret_cast<const uint4*>(src + o0);
+        y[b] = *reinterpret_cast<const uint4*>(src + o1);
       }
-      *reinterpret_cast<uint4*>(dst + o0) = x;
-      *reinterpret_cast<uint4*>(dst + o1) = y;
+      if (i0 == 0) angles();
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        if (tk[b] < 0) continue;
+        char* dst = rot_dst(a, t0 + tk[b], row[b], slot_s[tk[b]]);
+        if (!dst) continue;
+        const int c = at[b] >= 0 ? at[b] : ~at[b];
+        if (at[b] >= 0) {
+          const float4* cp = reinterpret_cast<const float4*>(&cs[tk[b]][c * 8]);
+          const float4* sp = reinterpret_cast<const float4*>(&sn[tk[b]][c * 8]);
+          const float4 c0 = cp[0], c1 = cp[1], s0 = sp[0], s1 = sp[1];
+          const float cv[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+          const float sv[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+          uint32_t xw[4] = {x[b].x, x[b].y, x[b].z, x[b].w};
+          uint32_t yw[4] = {y[b].x, y[b].y, y[b].z, y[b].w};
+          if (kHalf) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 u = unpack2<kF16>(xw[e]), z = unpack2<kF16>(yw[e]);
+              const float ca = cv[2 * e], cb = cv[2 * e + 1];
+              const float sa = sv[2 * e], sb = sv[2 * e + 1];
+              xw[e] = pack2<kF16>(u.x * ca - z.x * sa, u.y * cb - z.y * sb);
+              yw[e] = pack2<kF16>(z.x * ca + u.x * sa, z.y * cb + u.y * sb);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 u = unpack2<kF16>(xw[e]), z = unpack2<kF16>(yw[e]);
+              xw[e] = pack2<kF16>(u.x * cv[e] - u.y * sv[e],
+                                  u.y * cv[e] + u.x * sv[e]);
+              yw[e] = pack2<kF16>(z.x * cv[e + 4] - z.y * sv[e + 4],
+                                  z.y * cv[e + 4] + z.x * sv[e + 4]);
+            }
+          }
+          x[b] = make_uint4(xw[0], xw[1], xw[2], xw[3]);
+          y[b] = make_uint4(yw[0], yw[1], yw[2], yw[3]);
+        }
+        const bool pair = kHalf && at[b] >= 0;
+        const int o0 = pair ? c * 16 : c * 32, o1 = pair ? o0 + a.rot : o0 + 16;
+        *reinterpret_cast<uint4*>(dst + o0) = x[b];
+        *reinterpret_cast<uint4*>(dst + o1) = y[b];
+      }
     }
   } else {
     // pair by pair: any even rotary_dim, strides and alignment
+    angles();
     const int per = a.d >> 1, tok_items = rows * per;
     for (int i = threadIdx.x; i < nt * tok_items; i += kRotThreads) {
       const int j = i / tok_items, w = i - j * tok_items;
       const int row = w / per, p = w - row * per;
-      const char* src;
-      char* dst;
-      if (!rot_row(a, t0 + j, row, slot_s[j], &src, &dst)) continue;
+      const char* src = rot_src(a, t0 + j, row);
+      char* dst = rot_dst(a, t0 + j, row, slot_s[j]);
+      if (!dst) continue;
       const bool turn = row < a.H + a.n_kv && p < half;
       const int e0 = kHalf && turn ? p : 2 * p;
       const int e1 = kHalf && turn ? p + half : 2 * p + 1;
@@ -236,15 +257,12 @@ extern "C" int amass_rotary_write(const AmassRotary* args, void* stream) {
                          (uintptr_t)a.kd | (uintptr_t)a.v | (uintptr_t)a.vd;
   const bool vec = !(head_dim & 15) && !(rotary_dim & 15) && !(strides & 7) &&
                    !(base & 15);
-  // enough items per CTA that its angles and its one barrier are small
-  // beside its copies, while every SM still has several CTAs
-  const int64_t items = (int64_t)(a.H + a.n_kv * (a.v ? 2 : 1)) *
-                        (vec ? head_dim >> 4 : head_dim >> 1);
-  int64_t tok = (6ll * kRotThreads + items - 1) / items;
-  const int64_t spread = ((int64_t)n_tokens + 4 * num_sms() - 1) /
-                         (4 * num_sms());
-  if (tok > spread) tok = spread;
-  a.tok = (int)(tok < 1 ? 1 : tok > kRotMaxTok ? kRotMaxTok : tok);
+  // as many tokens a CTA as make whole waves of the CTAs that fit the GPU
+  // (a last wave of a few CTAs costs as much as a full one), at least one
+  const int64_t fit = (int64_t)kRotCtas * num_sms();
+  const int64_t waves = (n_tokens + fit * kRotMaxTok - 1) /
+                        (fit * kRotMaxTok);
+  a.tok = (int)((n_tokens + fit * waves - 1) / (fit * waves));
   const cudaStream_t st = (cudaStream_t)stream;
   const bool half = x.layout == AMASS_ROTARY_HALF;
   if (x.dtype == AMASS_FP16)

@@ -5,6 +5,7 @@ the paged cache, in one launch.
                     either pairing, the usual long-context scalings
   rotary_write_kv   turn q, turn k into the K cache, copy v into the V cache
                     at the step's slot mapping
+  rotary_write_pools  the same into K and V pools apart (the tier's staging)
   rotary_embed      turn q and k only
 
 Angles are formed in the kernel from 64-bit fixed-point frequencies (turns per
@@ -229,4 +230,32 @@ def rotary_write_kv(rot, q, k, v, positions, kv_cache, slot_mapping, *,
             st if vc else (0, 0, 0), slots, nb, page, positions, T)
 
 
-__all__ = ["Rotary", "rotary_embed", "rotary_write_kv", "rotary_frequencies"]
+def rotary_write_pools(rot, q, k, v, positions, k_pool, v_pool, slot_mapping,
+                       *, q_out=None, n_tokens=None) -> None:
+    """``rotary_write_kv`` into K and V pools that are tensors of their own,
+    (num_blocks, page, n_kv, d) each (the tier's staging pools); v and
+    ``v_pool`` may be None."""
+    if k is None or (q is None and q_out is not None) or \
+            (v is None) != (v_pool is None):
+        raise ValueError("rotary_write_pools needs k, q for q_out, and v and "
+                         "v_pool together")
+    strides = [(0, 0, 0), (0, 0, 0)]
+    for i, (name, t) in enumerate((("k_pool", k_pool), ("v_pool", v_pool))):
+        if t is None:
+            continue
+        if t.dim() != 4 or t.dtype != k.dtype or \
+                t.get_device() != rot.index or t.stride(3) != 1 or \
+                t.shape[2:] != k.shape[1:] or t.shape[:2] != k_pool.shape[:2]:
+            raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not fit "
+                             f"{name} {tuple(t.shape)} {t.dtype}")
+        strides[i] = t.stride()[:3]
+    T = k.shape[0] if n_tokens is None else int(n_tokens)
+    slots = _vector(rot, "slot_mapping", slot_mapping, T, _INDEX[:1])
+    _launch(rot, k, q, q if q_out is None else q_out, k, v,
+            k_pool.data_ptr(), strides[0],
+            0 if v_pool is None else v_pool.data_ptr(), strides[1], slots,
+            k_pool.shape[0], k_pool.shape[1], positions, T)
+
+
+__all__ = ["Rotary", "rotary_embed", "rotary_write_kv", "rotary_write_pools",
+           "rotary_frequencies"]

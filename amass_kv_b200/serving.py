@@ -27,6 +27,7 @@ import dataclasses
 import torch
 
 from . import _lib
+from . import rotary as RT
 from . import selection as S
 from . import summaries as SM
 from . import tier as T
@@ -96,11 +97,30 @@ class MemSession:
         self._n_req, self._bt, self._sl = n_req, block_table, seq_lens
 
     def write_kv(self, layer: int, key, value, slot_mapping,
-                 n_tokens: int) -> None:
+                 n_tokens: int, *, rotary=None, positions=None,
+                 query=None) -> None:
         """This step's K (n_tokens, n_kv, d) into the K-only cache at the
         engine's slot mapping (block * page + offset, -1 skips) under mem-v,
-        and V (and K under mem-kv) into staging at the tier's own slots."""
+        and V (and K under mem-kv) into staging at the tier's own slots.
+
+        With ``rotary`` (a ``rotary.Rotary``) and ``positions`` the keys come
+        unturned: they are turned on their way into the cache (``key`` stays
+        as it is) and ``query`` (T, H, d), when given, in place, in the same
+        launch."""
         l = int(layer)
+        if rotary is not None:
+            n = int(n_tokens)
+            if self.offload_k:
+                stg = self.tier.staging
+                RT.rotary_write_pools(rotary, query, key, value, positions,
+                                      stg.k_pool[l], stg.v_pool[l],
+                                      stg.v_slot_mapping, n_tokens=n)
+            else:
+                RT.rotary_write_pools(rotary, query, key, None, positions,
+                                      self.k_cache[l][:, 0], None,
+                                      slot_mapping, n_tokens=n)
+                self.tier.write_kv(l, value, n)
+            return
         if not self.offload_k:
             kc = self.k_cache[l][:, 0]                 # (NB, page, n_kv, d)
             _lib.call("amass_staging_scatter", ptr(key), key.stride(0),

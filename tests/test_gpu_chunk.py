@@ -133,6 +133,76 @@ def test_strides_and_layouts(dev):
         assert bool((wide[:, H] == 3.0).all())
 
 
+def test_heads_before_tokens(dev):
+    """A cache stored (blocks, 2, heads, page, d), seen as (.., page, heads,
+    d), and q in place."""
+    c = make(dev, [(70, 300), (1, 90), (33, 33)])
+    c["kv"] = c["kv"].permute(0, 1, 3, 2, 4).contiguous().permute(
+        0, 1, 3, 2, 4)
+    a, _ = check(c, dev)
+    buf = ChunkBuffers(dev, n_kv=2, G=4, head_dim=128)
+    q = c["q"].clone()
+    paged_chunk_attention(q, c["kv"], c["bt"], c["sl"], c["qsl"], q, buf)
+    n = c["starts"][-1]
+    assert torch.equal(q[:n], a[:n]) and torch.equal(q[n:], c["q"][n:])
+
+
+def test_padded_cache(dev):
+    """Blocks and heads further apart than their contents."""
+    c = make(dev, [(40, 200), (5, 5)], d=64)
+    NB = c["kv"].shape[0]
+    big = torch.full((NB + 1, 2, PAGE, 4, 64), float("nan"), device=dev,
+                     dtype=torch.bfloat16)
+    big[:NB, :, :, :2] = c["kv"]
+    c["kv"] = big[:NB, :, :, :2]
+    check(c, dev)
+
+
+def test_nan_and_infinite_keys(dev):
+    """A NaN or infinite key in reach: the rows that see it are NaN, all
+    others what they are without it."""
+    for bad in (float("nan"), float("inf")):
+        c = make(dev, [(60, 300), (1, 200)], seed=4)
+        clean, lse = check(c, dev)
+        p = 270                              # seen by rows 30 .. 59
+        c["kv"][c["bt"][0, p // PAGE].long(), 0, p % PAGE, 1] = bad
+        buf = ChunkBuffers(dev, n_kv=2, G=4, head_dim=128)
+        out, got = torch.zeros_like(clean), torch.zeros_like(lse)
+        paged_chunk_attention(c["q"], c["kv"], c["bt"], c["sl"], c["qsl"],
+                              out, buf, lse=got)
+        n = c["starts"][-1]
+        same = torch.ones(n, 8, dtype=torch.bool, device=dev)
+        if bad != bad:
+            same[30:60, 4:] = False
+            assert bool(torch.isnan(out[30:60, 4:]).all())
+            assert bool(torch.isnan(got[30:60, 4:]).all())
+        else:                                # q k is NaN, +inf or -inf
+            same[30:60, 4:] = ~torch.isnan(got[30:60, 4:])
+        assert torch.equal(out[:n][same], clean[:n][same]) or bad == bad
+        assert torch.equal(got[:n, :4], lse[:n, :4])
+        assert torch.equal(out[:30], clean[:30])
+        assert torch.equal(out[60:n], clean[60:n])
+
+
+def test_two_streams(dev):
+    """Two streams at once, each with buffers of its own."""
+    cs = [make(dev, [(50, 3000), (1, 9000)], seed=s) for s in (1, 2)]
+    want = [check(c, dev)[0] for c in cs]
+    bufs = [ChunkBuffers(dev, n_kv=2, G=4, head_dim=128) for _ in cs]
+    outs = [torch.full_like(c["q"], 7.0) for c in cs]
+    streams = [torch.cuda.Stream(dev) for _ in cs]
+    torch.cuda.synchronize(dev)
+    for _ in range(5):
+        for c, b, o, s in zip(cs, bufs, outs, streams):
+            with torch.cuda.stream(s):
+                paged_chunk_attention(c["q"], c["kv"], c["bt"], c["sl"],
+                                      c["qsl"], o, b)
+    torch.cuda.synchronize(dev)
+    for b, o, w in zip(bufs, outs, want):
+        b.check()
+        assert torch.equal(o, w)
+
+
 def test_large_scores(dev):
     """Scores of hundreds: every tile moves the maximum, the rescale path and
     weights far below 1."""

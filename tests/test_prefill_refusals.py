@@ -43,6 +43,8 @@ def chunk_args(**kw):
     (dict(block_table=torch.zeros(3, 2, dtype=torch.int32).t()),
      "contiguous in the last"),
     (dict(block_table=torch.zeros(2, 0, dtype=torch.int32)), "cover"),
+    (dict(kv_cache=torch.zeros(20000, dtype=torch.bfloat16).as_strided(
+        (4, 2, 16, 2, 64), (4104, 2048, 128, 64, 1))), "block strides"),
     (dict(window=0), "window"), (dict(scale=0.0), "scale"),
     (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
     (dict(lse=torch.zeros(5, 4)), "lse"),
