@@ -245,6 +245,15 @@ AMASS_DEV void tma_5d(uint32_t dst, const CUtensorMap* m, uint32_t bar,
 }
 
 // ------------------------------------------------------------- work list ---
+// e / d for 0 <= e < 2^31 and a quotient below 2^20: the reciprocal's quotient
+// is off by one at most (an integer division costs some 150 cycles more)
+AMASS_DEV int quotient(int e, int d) {
+  unsigned q = (unsigned)__fdividef((float)e, (float)d);
+  q -= q * (unsigned)d > (unsigned)e;
+  q += (q + 1) * (unsigned)d <= (unsigned)e;
+  return (int)q;
+}
+
 // One request: its rows start at q0, ql of them; row i has position off + i.
 struct ChReq {
   int q0, ql, sl, off, nt;
@@ -390,10 +399,11 @@ struct ChWalk {
     s.last = k1 == nu;
     s.cta0 = s.parts = 0;
     if (!(s.first && s.last)) {          // floor divisions by the run length
-      const int b = at < 0 ? -((p.share - 1 - at) / p.share) : 0;
-      s.cta0 = (int)blockIdx.x + b;
+      const int b = at < 0 ? quotient(p.share - 1 - at, p.share) : 0;
       const int e = at + (nu - 1) * w;
-      s.parts = (e < 0 ? -((p.share - 1 - e) / p.share) : e / p.share) - b + 1;
+      s.cta0 = (int)blockIdx.x - b;
+      s.parts = (e < 0 ? -quotient(p.share - 1 - e, p.share)
+                       : quotient(e, p.share)) + b + 1;
     }
     if (only) to = 0;
     else step(a, nu * w + kCostItem);
@@ -447,8 +457,8 @@ AMASS_DEV void ch_plan(const ChunkArgs& a, ChPlan* out) {
         u -= all;
         continue;
       }
-      const int h = all >> 32 ? (int)(u / cost)
-                              : (int)((uint32_t)u / (uint32_t)cost);
+      const int h = all >> 31 || a.n_kv >> 20 ? (int)(u / cost)
+                                              : quotient((int)u, (int)cost);
       u -= h * cost;
       int lo = 0;                        // last item that starts at or before
       if (q.nt > 1) {
@@ -543,16 +553,16 @@ struct ChJob {
 // CTAs in order (the same result whichever CTA finishes last).
 struct ChSum {
   float M = -INFINITY, l = 0.f;
-  // adds NP partials from c0 on of NC groups of 4 columns
+  // adds NP partials, every `by`-th from c0 on, of NC groups of 4 columns
   template <int D, int NC, int NP>
   AMASS_DEV void add(const ChJob& b, const float2* ml, const float4* x,
-                     int c0, float4* o) {
+                     int c0, int by, float4* o) {
     float4 v[NP][NC];
     float2 z[NP];
     // the first CTA's partial is its second slot, the others' their first
 #pragma unroll
     for (int e = 0; e < NP; ++e) {
-      const int c = c0 + e, s = 2 * c + (c == 0);
+      const int c = c0 + e * by, s = 2 * c + (c == 0);
       z[e] = make_float2(-INFINITY, 0.f);
       if (c < b.parts) z[e] = __ldcg(ml + s * 256);
 #pragma unroll
@@ -598,22 +608,35 @@ AMASS_DEV char* ch_out(const ChunkArgs& a, const ChJob& b, int row,
   *lse = token * (a.n_kv * a.G) + head;
   return (char*)a.out + 2 * (token * a.o_st + head * a.o_sh);
 }
-// Few rows (2^sh >= n), many partials: lanes over rows, then over groups of 4
-// columns from cg on, 12 partials in flight.
+// Few rows (2^sh >= n, sh <= 3), many partials: lanes over rows, then 4 groups
+// of 4 columns from cg on, then 8 >> sh groups of partials, 12 in flight each.
 template <int D, bool kF16>
 AMASS_DEV void ch_join_few(const ChunkArgs& a, const ChJob& b, int sh, int cg) {
   const int lane = threadIdx.x & 31, r = lane & ((1 << sh) - 1);
-  cg += lane >> sh;
-  if (r >= b.n) return;
-  const int row = b.row0 + r;
+  const int pg = lane >> (sh + 2), pgs = 8 >> sh;
+  cg += (lane >> sh) & 3;
+  const int row = b.row0 + min(r, b.n - 1);
   const float2* ml = a.ml + (int64_t)b.cta0 * 512 + row;
   const float4* x = reinterpret_cast<const float4*>(a.acc) +
                     ((int64_t)b.cta0 * 2 * (D / 4) + cg) * 256 + row;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   ChSum s;
-  #pragma unroll 1
-  for (int c = 0; c < b.parts; c += 12)
-    s.template add<D, 1, 12>(b, ml, x, c, &o);
+#pragma unroll 1
+  for (int c = pg; c < b.parts; c += 12 * pgs)
+    s.template add<D, 1, 12>(b, ml, x, c, pgs, &o);
+  for (int k = 4 << sh; k < 32; k <<= 1) {
+    const float m1 = __shfl_xor_sync(~0u, s.M, k);
+    const float l1 = __shfl_xor_sync(~0u, s.l, k);
+    const float mn = fmax_nan(s.M, m1), ref = mn == -INFINITY ? 0.f : mn;
+    const float f0 = ex2_approx(s.M - ref), f1 = ex2_approx(m1 - ref);
+    s.M = mn;
+    s.l = s.l * f0 + l1 * f1;
+    o.x = o.x * f0 + __shfl_xor_sync(~0u, o.x, k) * f1;
+    o.y = o.y * f0 + __shfl_xor_sync(~0u, o.y, k) * f1;
+    o.z = o.z * f0 + __shfl_xor_sync(~0u, o.z, k) * f1;
+    o.w = o.w * f0 + __shfl_xor_sync(~0u, o.w, k) * f1;
+  }
+  if (r >= b.n || pg) return;
   int64_t li;
   char* out = ch_out(a, b, row, &li);
   *reinterpret_cast<uint2*>(out + 8 * cg) = pack4<kF16>(o, s.inv());
@@ -634,7 +657,7 @@ AMASS_DEV void ch_join_many(const ChunkArgs& a, const ChJob& b, int half,
   for (int e = 0; e < 16; ++e) o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
   for (int c = 0; c < b.parts; c += 2)
-    s.template add<D, 16, 2>(b, ml, x, c, o);
+    s.template add<D, 16, 2>(b, ml, x, c, 1, o);
   const float f = s.inv();
 #pragma unroll
   for (int e = 0; e < 16; e += 2) {
@@ -1292,7 +1315,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   for (int k = 0; k < n_few; ++k) {
     const ChJob b = jobs[few_jobs[k]];
     const int sh = b.n <= 1 ? 0 : 32 - __clz(b.n - 1);
-    for (int cg = 0; cg < D / 4; cg += 32 >> sh) {
+    for (int cg = 0; cg < D / 4; cg += 4) {
       if (at-- != 0) continue;
       at = kChThreads / 32 - 1;
       ch_join_few<D, kF16>(a, b, sh, cg);
