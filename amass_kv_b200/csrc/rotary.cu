@@ -78,7 +78,8 @@ AMASS_DEV char* rot_dst(const RotArgs& a, int t, int row, int64_t slot) {
   return a.vd + 2 * (b * a.vd_sb + o * a.vd_st + (row - a.n_kv) * a.vd_sh);
 }
 
-template <bool kF16, bool kHalf, bool kVec>
+// kWidth: elements a lane moves at a time -- 8 (16 bytes), 2, or 1
+template <bool kF16, bool kHalf, int kWidth>
 __global__ void __launch_bounds__(kRotThreads, kRotCtas)
 rotary_write_kernel(const __grid_constant__ RotArgs a) {
   grid_dep_wait();
@@ -108,7 +109,7 @@ rotary_write_kernel(const __grid_constant__ RotArgs a) {
                                     : (int64_t)(t0 + threadIdx.x);
     __syncthreads();
   };
-  if (kVec) {
+  if constexpr (kWidth == 8) {
     const int per = a.d >> 4, rper = a.rot >> 4;     // items: row, rotated
     const int tok_items = rows * per, n = nt * tok_items;
     // kBatch items of a thread in flight; the first ones' loads run while the
@@ -176,6 +177,47 @@ rotary_write_kernel(const __grid_constant__ RotArgs a) {
         *reinterpret_cast<uint4*>(dst + o1) = y[b];
       }
     }
+  } else if constexpr (kWidth == 2) {
+    // two elements by two: a pair of neighbours, or two pairs whose halves
+    // are a word each
+    angles();
+    const int per = kHalf ? a.d >> 2 : a.d >> 1, tok_items = rows * per;
+    const int turned = kHalf ? half >> 1 : half;     // items of a row
+    for (int i = threadIdx.x; i < nt * tok_items; i += kRotThreads) {
+      const int j = i / tok_items, w = i - j * tok_items;
+      const int row = w / per, p = w - row * per;
+      const char* src = rot_src(a, t0 + j, row);
+      char* dst = rot_dst(a, t0 + j, row, slot_s[j]);
+      if (!dst) continue;
+      const bool turn = row < a.H + a.n_kv && p < turned;
+      const auto ld = [&](int o) {
+        return *reinterpret_cast<const uint32_t*>(src + o);
+      };
+      const auto st = [&](int o, uint32_t v) {
+        *reinterpret_cast<uint32_t*>(dst + o) = v;
+      };
+      if (kHalf) {
+        const int o0 = turn ? 4 * p : 8 * p, o1 = turn ? o0 + a.rot : o0 + 4;
+        uint32_t x = ld(o0), y = ld(o1);
+        if (turn) {
+          const float2 u = unpack2<kF16>(x), z = unpack2<kF16>(y);
+          const float ca = cs[j][2 * p], cb = cs[j][2 * p + 1];
+          const float sa = sn[j][2 * p], sb = sn[j][2 * p + 1];
+          x = pack2<kF16>(u.x * ca - z.x * sa, u.y * cb - z.y * sb);
+          y = pack2<kF16>(z.x * ca + u.x * sa, z.y * cb + u.y * sb);
+        }
+        st(o0, x);
+        st(o1, y);
+      } else {
+        uint32_t x = ld(4 * p);
+        if (turn) {
+          const float2 u = unpack2<kF16>(x);
+          const float c = cs[j][p], s = sn[j][p];
+          x = pack2<kF16>(u.x * c - u.y * s, u.y * c + u.x * s);
+        }
+        st(4 * p, x);
+      }
+    }
   } else {
     // pair by pair: any even rotary_dim, strides and alignment
     angles();
@@ -206,12 +248,16 @@ rotary_write_kernel(const __grid_constant__ RotArgs a) {
 }
 
 template <bool kF16, bool kHalf>
-int rot_launch(const RotArgs& a, bool vec, cudaStream_t st) {
-  const dim3 grid((unsigned)((a.T + a.tok - 1) / a.tok));
-  return vec ? launch_pdl(rotary_write_kernel<kF16, kHalf, true>, grid,
-                          dim3(kRotThreads), 0, st, a)
-             : launch_pdl(rotary_write_kernel<kF16, kHalf, false>, grid,
-                          dim3(kRotThreads), 0, st, a);
+int rot_launch(const RotArgs& a, int width, cudaStream_t st) {
+  const dim3 grid((unsigned)((a.T + a.tok - 1) / a.tok)), block(kRotThreads);
+  if (width == 8)
+    return launch_pdl(rotary_write_kernel<kF16, kHalf, 8>, grid, block, 0, st,
+                      a);
+  if (width == 2)
+    return launch_pdl(rotary_write_kernel<kF16, kHalf, 2>, grid, block, 0, st,
+                      a);
+  return launch_pdl(rotary_write_kernel<kF16, kHalf, 1>, grid, block, 0, st,
+                    a);
 }
 
 }  // namespace
@@ -249,14 +295,21 @@ extern "C" int amass_rotary_write(const AmassRotary* args, void* stream) {
   const int n_tokens = x.n_tokens;
   if (n_tokens == 0 || a.H + a.n_kv == 0) return AMASS_OK;
   // 16-byte items need whole items in the rotated part and in the rest, and
-  // 16-byte aligned rows; anything else goes pair by pair
+  // 16-byte aligned rows; words need the same of two elements (rotary_dim 20
+  // in halves, 8192 tokens of 8 / 2 heads of 64: 17 us, one by one 36);
+  // what is left goes one by one
   const int64_t strides = a.q_st | a.q_sh | a.qo_st | a.qo_sh | a.k_st |
                           a.k_sh | a.v_st | a.v_sh | a.kd_sb | a.kd_st |
                           a.kd_sh | a.vd_sb | a.vd_st | a.vd_sh;
   const uintptr_t base = (uintptr_t)a.q | (uintptr_t)a.qo | (uintptr_t)a.k |
                          (uintptr_t)a.kd | (uintptr_t)a.v | (uintptr_t)a.vd;
-  const bool vec = !(head_dim & 15) && !(rotary_dim & 15) && !(strides & 7) &&
-                   !(base & 15);
+  const bool half = x.layout == AMASS_ROTARY_HALF;
+  const int width =
+      !(head_dim & 15) && !(rotary_dim & 15) && !(strides & 7) && !(base & 15)
+          ? 8
+      : !(strides & 1) && !(base & 3) &&
+              (!half || (!(head_dim & 3) && !(rotary_dim & 3)))
+          ? 2 : 1;
   // as many tokens a CTA as make whole waves of the CTAs that fit the GPU
   // (a last wave of a few CTAs costs as much as a full one), at least one
   const int64_t fit = (int64_t)kRotCtas * num_sms();
@@ -264,10 +317,9 @@ extern "C" int amass_rotary_write(const AmassRotary* args, void* stream) {
                         (fit * kRotMaxTok);
   a.tok = (int)((n_tokens + fit * waves - 1) / (fit * waves));
   const cudaStream_t st = (cudaStream_t)stream;
-  const bool half = x.layout == AMASS_ROTARY_HALF;
   if (x.dtype == AMASS_FP16)
-    return half ? rot_launch<true, true>(a, vec, st)
-                : rot_launch<true, false>(a, vec, st);
-  return half ? rot_launch<false, true>(a, vec, st)
-              : rot_launch<false, false>(a, vec, st);
+    return half ? rot_launch<true, true>(a, width, st)
+                : rot_launch<true, false>(a, width, st);
+  return half ? rot_launch<false, true>(a, width, st)
+              : rot_launch<false, false>(a, width, st);
 }
