@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotMaxDim = 256;
-constexpr int kRotMaxTok = 16;           // tokens of one CTA
+constexpr int kRotMaxTok = 8;            // tokens of one CTA
 constexpr int kBatch = 2;
 constexpr int kRotCtas = 4;              // CTAs an SM holds (64 registers)
 
@@ -67,16 +67,34 @@ AMASS_DEV const char* rot_src(const RotArgs& a, int t, int row) {
   if (row < a.n_kv) return a.k + 2 * (t * a.k_st + row * a.k_sh);
   return a.v + 2 * (t * a.v_st + (row - a.n_kv) * a.v_sh);
 }
-// where it goes; null when there is nothing to write
-AMASS_DEV char* rot_dst(const RotArgs& a, int t, int row, int64_t slot) {
+// where it goes; null when there is nothing to write.  at: the slot's offset
+// in the K and in the V cache, -1 without a slot
+AMASS_DEV char* rot_dst(const RotArgs& a, int t, int row, longlong2 at) {
   if (row < a.H) return a.qo + 2 * (t * a.qo_st + row * a.qo_sh);
-  if (slot < 0 || slot >= a.n_slots) return nullptr;
-  const int64_t b = slot / a.page, o = slot - b * a.page;
+  if (at.x < 0) return nullptr;
   row -= a.H;
-  if (row < a.n_kv)
-    return a.kd + 2 * (b * a.kd_sb + o * a.kd_st + row * a.kd_sh);
-  return a.vd + 2 * (b * a.vd_sb + o * a.vd_st + (row - a.n_kv) * a.vd_sh);
+  if (row < a.n_kv) return a.kd + 2 * (at.x + row * a.kd_sh);
+  return a.vd + 2 * (at.y + (row - a.n_kv) * a.vd_sh);
 }
+
+// Item i of n a token's `rows` times `per`, then steps of kRotThreads items:
+// divisions once a thread, carries after that.
+struct RotWalk {
+  int j, row, c, sj, sr, sc;
+  AMASS_DEV RotWalk(int rows, int per) {
+    const int tok = rows * per, i = threadIdx.x;
+    j = i / tok; row = (i - j * tok) / per; c = i - j * tok - row * per;
+    sj = kRotThreads / tok; sr = (kRotThreads - sj * tok) / per;
+    sc = kRotThreads - sj * tok - sr * per;
+  }
+  AMASS_DEV void step(int rows, int per) {
+    c += sc;
+    row += sr;
+    j += sj;
+    if (c >= per) { c -= per; ++row; }
+    if (row >= rows) { row -= rows; ++j; }
+  }
+};
 
 // kWidth: elements a lane moves at a time -- 8 (16 bytes), 2, or 1
 template <bool kF16, bool kHalf, int kWidth>
@@ -86,7 +104,7 @@ rotary_write_kernel(const __grid_constant__ RotArgs a) {
   grid_dep_launch();
   __shared__ __align__(16) float cs[kRotMaxTok][kRotMaxDim / 2];
   __shared__ __align__(16) float sn[kRotMaxTok][kRotMaxDim / 2];
-  __shared__ int64_t slot_s[kRotMaxTok];
+  __shared__ longlong2 slot_s[kRotMaxTok];
   const int t0 = blockIdx.x * a.tok;
   const int nt = min(a.tok, a.T - t0), half = a.rot >> 1;
   const int rows = a.H + a.n_kv + (a.v ? a.n_kv : 0);
@@ -104,14 +122,23 @@ rotary_write_kernel(const __grid_constant__ RotArgs a) {
       cs[j][p] = c * a.mscale;
       sn[j][p] = s * a.mscale;
     }
-    if ((int)threadIdx.x < nt)
-      slot_s[threadIdx.x] = a.slots ? a.slots[t0 + threadIdx.x]
-                                    : (int64_t)(t0 + threadIdx.x);
+    if ((int)threadIdx.x < nt) {
+      const int64_t s = a.slots ? a.slots[t0 + threadIdx.x]
+                                : (int64_t)(t0 + threadIdx.x);
+      longlong2 at = make_longlong2(-1, -1);
+      if (s >= 0 && s < a.n_slots) {
+        const int64_t b = s / a.page, o = s - b * a.page;
+        at = make_longlong2(b * a.kd_sb + o * a.kd_st,
+                            b * a.vd_sb + o * a.vd_st);
+      }
+      slot_s[threadIdx.x] = at;
+    }
     __syncthreads();
   };
   if constexpr (kWidth == 8) {
     const int per = a.d >> 4, rper = a.rot >> 4;     // items: row, rotated
-    const int tok_items = rows * per, n = nt * tok_items;
+    const int n = nt * rows * per;
+    RotWalk wk(rows, per);
     // kBatch items of a thread in flight; the first ones' loads run while the
     // angles are formed
     for (int i0 = 0; i0 < n; i0 += kBatch * kRotThreads) {
@@ -119,13 +146,11 @@ rotary_write_kernel(const __grid_constant__ RotArgs a) {
       int at[kBatch], row[kBatch], tk[kBatch];
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
-        const int i = i0 + b * kRotThreads + threadIdx.x;
-        tk[b] = -1;
-        if (i >= n) continue;
-        const int j = i / tok_items, w = i - j * tok_items;
-        row[b] = w / per;
-        const int c = w - row[b] * per;
-        tk[b] = j;
+        const int j = wk.j, c = wk.c;
+        row[b] = wk.row;
+        tk[b] = j < nt ? j : -1;
+        wk.step(rows, per);
+        if (j >= nt) continue;
         // the item's chunk, rotated ones with their sign bit clear
         at[b] = row[b] < a.H + a.n_kv && c < rper ? c : ~c;
         const char* src = rot_src(a, t0 + j, row[b]);
@@ -181,11 +206,10 @@ rotary_write_kernel(const __grid_constant__ RotArgs a) {
     // two elements by two: a pair of neighbours, or two pairs whose halves
     // are a word each
     angles();
-    const int per = kHalf ? a.d >> 2 : a.d >> 1, tok_items = rows * per;
+    const int per = kHalf ? a.d >> 2 : a.d >> 1;
     const int turned = kHalf ? half >> 1 : half;     // items of a row
-    for (int i = threadIdx.x; i < nt * tok_items; i += kRotThreads) {
-      const int j = i / tok_items, w = i - j * tok_items;
-      const int row = w / per, p = w - row * per;
+    for (RotWalk wk(rows, per); wk.j < nt; wk.step(rows, per)) {
+      const int j = wk.j, row = wk.row, p = wk.c;
       const char* src = rot_src(a, t0 + j, row);
       char* dst = rot_dst(a, t0 + j, row, slot_s[j]);
       if (!dst) continue;
@@ -221,10 +245,9 @@ rotary_write_kernel(const __grid_constant__ RotArgs a) {
   } else {
     // pair by pair: any even rotary_dim, strides and alignment
     angles();
-    const int per = a.d >> 1, tok_items = rows * per;
-    for (int i = threadIdx.x; i < nt * tok_items; i += kRotThreads) {
-      const int j = i / tok_items, w = i - j * tok_items;
-      const int row = w / per, p = w - row * per;
+    const int per = a.d >> 1;
+    for (RotWalk wk(rows, per); wk.j < nt; wk.step(rows, per)) {
+      const int j = wk.j, row = wk.row, p = wk.c;
       const char* src = rot_src(a, t0 + j, row);
       char* dst = rot_dst(a, t0 + j, row, slot_s[j]);
       if (!dst) continue;
