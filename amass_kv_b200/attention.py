@@ -268,5 +268,5 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
         query_start_loc.data_ptr(), *buf.scratch, op,
         0 if lse is None else lse.data_ptr(), q_st, q_sh, k_sb, k_st, k_sh,
         v_sb, v_st, v_sh, block_table.stride(0), o_st, o_sh, scale, nb,
-        buf.n_ctas, min(window or 0, 0x7fffffff), T, n_req, n_kv, buf.G, d, page, max_pages,
-        DTYPES[dtype]))
+        buf.n_ctas, min(window or 0, 0x7fffffff), T, n_req, n_kv, buf.G, d,
+        page, max_pages, DTYPES[dtype]))

@@ -15,10 +15,10 @@
 //                   a page (a copy takes some 80-100 cycles of the TMA unit
 //                   whatever its size: at one per page and 64 columns K and V
 //                   came at 26 bytes a cycle, the tensor core wants 32)
-//   warp 10         walks the run and tells the others its pieces
 //   warp 9          issues the tcgen05 MMAs: S = Q K^T (both operands in
 //                   shared memory, fp32 S in TMEM), O += P V (P in TMEM over
 //                   S's columns, V as a column-major operand, fp32 O in TMEM)
+//   warp 10         walks the run and tells the others its pieces
 //
 // While one row tile's softmax runs, the tensor core works for the other.
 // O is rescaled only when a row's maximum grows by more than 2^8 (p stays
@@ -30,9 +30,16 @@
 // each CTA scans the requests and finds its own run.  Items cut by a run's
 // end leave unnormalised partials; the CTA that finishes the last one of a
 // warp's rows joins them (a second kernel for that took 9 us of 20 at one
-// token).  This serves a
-// single token over a long context (all SMs read one request's cache) and a
-// large prefill (no tail of uneven causal tiles) with one rule.
+// token).  This serves a single token over a long context (all SMs read one
+// request's cache) and a large prefill (no tail of uneven causal tiles) with
+// one rule.
+//
+// Measured on a B200, bf16, 32 query / 8 kv heads of 128: 2048 tokens behind
+// 64K 1745 us (1276 TFLOP/s; 2010 us back to back, at the power limit), one
+// token over 4K 12.8 us with the call; 64 / 8 heads, six fresh prompts of
+// 333-2047 tokens 223 us.  What bounds it: the chain scores ->
+// softmax -> product (3300 cycles a key tile of two row tiles, of which the
+// tensor core is busy 2048), then the board's power.
 //
 // Slots behind a request's last token may hold anything: K's scores there
 // are replaced before the maximum, V's rows are zeroed in shared memory.
@@ -43,7 +50,7 @@
 namespace amass {
 namespace {
 
-constexpr int kChThreads = 384;          // three warpgroups (two idle warps)
+constexpr int kChThreads = 384;          // three warpgroups (warp 11 idles)
 constexpr int kKeys = 128;               // keys of a tile
 constexpr int kPg = 16;                  // tokens of a page
 constexpr int kChMaxReq = 4096;
@@ -189,7 +196,7 @@ AMASS_DEV void tc_ld_16x256(uint32_t* r, uint32_t t) {
         "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
       : "r"(t));
 }
-// 16 rows of 64 columns: lane l's column 4 j + l % 4 of rows l / 4 and l / 4 + 8
+// 16 rows of 64 columns: lane l's are 4 j + l % 4 of rows l / 4 and l / 4 + 8
 AMASS_DEV void tc_st_16x128(uint32_t t, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.16x128b.x16.b32 [%0], "
@@ -334,13 +341,13 @@ struct ChPlan {
   int r, h, i, from, to, share;          // run [from, to) from item i's start
 };
 
-// Walks the segments of a CTA's run (one warp does, a few ahead of the others).  Key tile
-// k of an item belongs to the CTA whose run holds its place, item start + k *
-// weight.  A first segment that starts inside its item goes last: then every
-// CTA starts at its item's first key tile, and since the runs are equally
-// long the late pieces of one head's items meet at the same key tiles again.
-// CTAs of a head so stream its K and V together and find them in L2 (2048
-// rows behind 64K tokens: 2290 -> 1920 us).
+// Walks the segments of a CTA's run (one warp does, a few ahead of the others).
+// Key tile k of an item belongs to the CTA whose run holds its place, item
+// start + k * weight.  A first segment that starts inside its item goes last:
+// then every CTA starts at its item's first key tile, and since the runs are
+// equally long the late pieces of one head's items meet at the same key tiles
+// again.  CTAs of a head so stream its K and V together and find them in L2
+// (2048 rows behind 64K tokens: 2290 -> 1920 us).
 struct ChWalk {
   ChReq q;
   int r, h, i, from, to, at;             // at: the item's start in the run
@@ -385,10 +392,11 @@ struct ChWalk {
     int lo;
     const int nu = ch_tiles(a, q, i, &lo);
     const auto tiles = [&](int c) {      // ceil(c / w)
-      return w == kCost2 ? (c + kCost2 - 1) / kCost2 : (c + kCost1 - 1) / kCost1;
+      return w == kCost2 ? (c + kCost2 - 1) / kCost2
+                         : (c + kCost1 - 1) / kCost1;
     };
     const int k0 = tiles(from), k1 = to >= nu * w ? nu : tiles(to);
-    if (k0 >= k1) return false;          // a run inside an item's overhead (s.n = 0)
+    if (k0 >= k1) return false;          // the run is in an item's overhead
     s.r = r; s.h = h; s.sl = q.sl;
     s.tok0 = q.q0 + (i << tl);
     s.pos0 = q.off + (i << tl);
@@ -888,7 +896,8 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
           };
           uint64_t sum[2] = {0ull, 0ull};
           // two weights from two scores, packed
-          const auto weigh = [&](uint32_t s0, uint32_t s1, uint64_t nm2, int k) {
+          const auto weigh = [&](uint32_t s0, uint32_t s1, uint64_t nm2,
+                                 int k) {
             float p0, p1;
             f2_get(f2_fma(f2(__uint_as_float(s0), __uint_as_float(s1)), sl2x2,
                           nm2), p0, p1);
@@ -1096,7 +1105,6 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       if (!whole && live) {
         // rows whose last partial this is are joined when the run is done
         __syncwarp();
-        const int n = rows;
         int joins = 0;
         if (lane == 0) {
           int32_t* ticket = a.tickets + sg.cta0 * 8 + warp;
@@ -1106,11 +1114,12 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
             b.cta0 = sg.cta0;
             b.parts = sg.parts;
             b.h = sg.h;
-            b.n = n;
+            b.n = rows;
             b.row0 = (two ? t : 0) * 128 + (warp & 3) * 32;
             b.tok0 = (two ? t * tm : 0) + sg.tok0;
             joins = 1;
-            if (n <= kFewRows) few_jobs[atomicAdd(&n_few, 1)] = warp * 2 + mine;
+            if (rows <= kFewRows)
+              few_jobs[atomicAdd(&n_few, 1)] = warp * 2 + mine;
           }
         }
         mine += __shfl_sync(~0u, joins, 0);
@@ -1216,10 +1225,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       // The tensor core takes the next MMA about when the last one starts, so
       // what this warp does between two MMAs is time lost.  It looks for the V
       // tile and the next K tile while it would wait for weights anyway, and
-      // the whole warp walks while one elected lane issues (with a lane's own branch around it the
-      // compiler moves every descriptor to uniform registers one by one: 48
-      // cycles a small MMA instead of 37).  Two issuing warps, one per row
-      // tile, were slower: alternating MMAs of two accumulators do not
+      // the whole warp walks while one elected lane issues (48 cycles a small
+      // MMA in a branch of one lane, 37 elected).  Two issuing warps, one per
+      // row tile, were slower: alternating MMAs of two accumulators do not
       // overlap (2048 rows behind 64K: 1900 -> 2490 us).
       constexpr uint32_t id_s = mma_idesc(kF16, false, kKeys);
       constexpr uint32_t id_o = mma_idesc(kF16, true, D);
@@ -1230,7 +1238,8 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       int st = 0;                        // the next ring entry and its phase
       uint32_t ph = 0, qph = 0, pph = 0;
       const auto score = [&](int t, uint64_t q0, uint64_t k0, int k) {
-        mma_ss(tmem + t * 128, q0 + (((k >> 2) * X::kPanel + (k & 3) * 32) >> 4),
+        mma_ss(tmem + t * 128,
+               q0 + (((k >> 2) * X::kPanel + (k & 3) * 32) >> 4),
                k0 + (((k >> 2) * 1024 + (k & 3) * 32) >> 4), id_s, k > 0);
       };
       // S_t of ring entry e, which then is free when `done`
@@ -1345,18 +1354,21 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       // every MMA and its arrivals end before the CTA does
       commit(drain);
       (void)wait_warp(drain, 0);
-    } else if (warp == 10 && lane == 0) {
+    } else if (warp == 10) {
       // ------------------------------------------------------------- walk
-      ChWalk wk;
-      wk.start(a, plan);
-      for (int k = 0;; ++k) {
-        ChSeg s = {};
-        const bool more = wk.next(a, plan, s);
-        if (!wait(seg_empty + 8 * (k % kSegs), ((k / kSegs) & 1) ^ 1)) break;
-        segs[k % kSegs] = s;
-        mbar_arrive(seg_full + 8 * (k % kSegs));
-        if (!more) break;
+      if (lane == 0) {
+        ChWalk wk;
+        wk.start(a, plan);
+        for (int k = 0;; ++k) {
+          ChSeg s = {};
+          const bool more = wk.next(a, plan, s);
+          if (!wait(seg_empty + 8 * (k % kSegs), ((k / kSegs) & 1) ^ 1)) break;
+          segs[k % kSegs] = s;
+          mbar_arrive(seg_full + 8 * (k % kSegs));
+          if (!more) break;
+        }
       }
+      __syncwarp();
     }
   }
   tc_before();
@@ -1502,7 +1514,8 @@ extern "C" int amass_paged_chunk(const AmassChunk* args, void* stream) {
   a.tickets = x.tickets; a.fault = x.fault;
   a.scale_log2 = x.scale * kLog2e;
   a.n_req = x.n_req; a.n_kv = x.n_kv; a.G = x.G; a.T = x.n_tokens;
-  a.bh = (int)bh; a.max_pages = x.max_pages; a.nb = x.num_blocks; a.window = x.window;
+  a.bh = (int)bh; a.max_pages = x.max_pages; a.nb = x.num_blocks;
+  a.window = x.window;
   // tokens of a row tile: the largest power of two whose G heads fit 128 rows
   a.tm_log2 = x.G == 1 ? 7 : x.G == 2 ? 6 : x.G <= 4 ? 5 : 4;
   const bool f16 = x.dtype == AMASS_FP16;

@@ -2,11 +2,13 @@
 // table, query start offsets, token positions and slot mapping from the new
 // token count of each request, and the way back (truncate / release).
 //
-//   begin   have_r = ceil(old_r / P), need_r = ceil((old_r + new_r)/P) - have_r,
+//   begin   have_r = ceil(old_r / P), need_r = ceil((old_r + new_r) / P) -
+//           have_r,
 //           upto_r = need_0 + .. + need_r; request r is granted its pages iff
 //           need_r = 0 or upto_r <= free blocks (in order: the first that
 //           does not fit also refuses every later one that needs pages);
-//           its j-th new page takes free_stack[top - 1 - (upto_r - need_r + j)];
+//           its j-th new page takes
+//           free_stack[top - 1 - (upto_r - need_r + j)];
 //           token t of request r (start_r <= t < start_r + new_r) has position
 //           old_r + t - start_r and slot table[r][pos / P] * P + pos % P.
 //   trim    the pages behind the kept tokens return to the stack, last

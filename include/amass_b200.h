@@ -665,14 +665,14 @@ typedef struct AmassChunk {
  * exp(scale q.k), -inf without a key.  Cache slots behind a request's last
  * token may hold anything; block ids outside [0, num_blocks) read as zeros;
  * seq_lens is cut at max_pages * page.  n_ctas is the GPU's SM count.  Of
- * the scratch (acc_part, ml_part, tickets) only the tickets need to be 0 before
- * the first call, and are left 0; calls that overlap on the GPU need scratch of
- * their own.  fault[0] becomes 1 when a CTA gave up a bounded wait: its rows
- * are then incomplete and the scratch has to be replaced.  head_dim in {64, 128}, G <= 8, page =
- * 16, n_req <= 4096, scale > 0; bases 16-byte aligned, strides positive
- * multiples of 8 elements, block strides multiples of the head strides, with
- * the same quotient for K and V.  One launch; the first call on a device sets a
- * kernel attribute. */
+ * the scratch (acc_part, ml_part, tickets) only the tickets need to be 0
+ * before the first call, and are left 0; calls that overlap on the GPU need
+ * scratch of their own.  fault[0] becomes 1 when a CTA gave up a bounded wait:
+ * its rows are then incomplete and the scratch has to be replaced.  head_dim
+ * in {64, 128}, G <= 8, page = 16, n_req <= 4096, scale > 0; bases 16-byte
+ * aligned, strides positive multiples of 8 elements, block strides multiples
+ * of the head strides, with the same quotient for K and V.  One launch; the
+ * first call on a device sets a kernel attribute. */
 int amass_paged_chunk(const AmassChunk* args, void* stream);
 
 #ifdef __cplusplus
