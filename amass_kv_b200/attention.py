@@ -194,11 +194,12 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
     ``n_req = seq_lens.shape[0]``; ``buf`` is a ``ChunkBuffers``; ``out`` may
     be ``q``.
 
-    Cache slots behind a request's last token may hold anything.  At a
-    position the request has reached, a NaN or infinite key makes the rows
-    that see it NaN; a NaN or infinite value does so for the rows that see
-    it, and may for earlier rows of the same request.  Block ids outside the
-    cache read as zeros.  One launch, no allocation, no synchronisation."""
+    Cache slots behind a request's last token, or before the windows of all
+    its rows, may hold anything.  Between the two, a NaN or infinite key makes
+    the rows that see it NaN; a NaN or infinite value does so for the rows
+    that see it, and may for other rows of the same request.  Block ids
+    outside the cache read as zeros.  One launch, no allocation, no
+    synchronisation."""
     nb, page, n_kv, d, (k_sb, k_st, k_sh), k, v = cache_layout(kv_cache)
     v_sb, v_st, v_sh = k_sb, k_st, k_sh
     dtype, dev = q.dtype, buf.index

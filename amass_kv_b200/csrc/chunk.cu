@@ -41,8 +41,9 @@
 // softmax -> product (3300 cycles a key tile of two row tiles, of which the
 // tensor core is busy 2048), then the board's power.
 //
-// Slots behind a request's last token may hold anything: K's scores there
-// are replaced before the maximum, V's rows are zeroed in shared memory.
+// Slots behind a request's last token, or before all windows of an item's
+// rows, may hold anything: K's scores there are replaced before the maximum,
+// V's rows are zeroed in shared memory, whole pages are not read.
 #include <cuda.h>
 
 #include "common.cuh"
@@ -1153,19 +1154,25 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
         }
         if (!ok) break;
         const int npg = (sg.sl + kPg - 1) / kPg;
+        // the first key that any of the item's rows sees
+        const int lo = a.window ? max(sg.pos0 - a.window + 1, 0) : 0;
+        // tiles whose V has pages with rows that somebody sees and rows that
+        // nobody does
+        const int tlo = lo & (kPg - 1) ? lo >> 7 : -1;
+        const int thi = sg.sl & (kPg - 1) ? sg.sl >> 7 : -1;
         const int32_t* row = a.bt + (int64_t)sg.r * a.bt_stride;
         // block of the tile's page (lane & 7); pages that are not the
-        // request's read as zeros (a block behind the cache)
+        // request's, or before all windows, read as zeros (a block behind the
+        // cache)
         const auto block_of = [&](int tile) {
           const int p = tile * (kKeys / kPg) + (lane & 7);
           int b = -1;
-          if (p < npg) b = row[p];
+          if (p < npg && p >= (lo >> 4)) b = row[p];
           return b < 0 || b >= a.nb ? a.nb : b;
         };
         const auto load = [&](bool is_v, int tile, int blk) -> bool {
           if (!wait_warp(empty(st), ph)) return false;
-          const bool part = is_v && (sg.sl & (kPg - 1)) &&
-                            tile == (sg.sl - 1) >> 7;
+          const bool part = is_v && (tile == tlo || tile == thi);
           const uint32_t dst = ring + st * X::kTile;
           const uint32_t bar = part ? v_tmp : full(st);
           if (lane == 0) mbar_arrive_expect_tx(bar, X::kTile);
@@ -1174,20 +1181,26 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
             tma_5d(dst + lane * X::kPage, is_v ? &mv : &mk, bar,
                    blk * a.bh + sg.h);
           if (part) {
-            // rows behind the last token: whatever they hold, 0 * it must be
-            // 0 in P V
+            // whatever the others hold, 0 * it must be 0 in P V (one small
+            // loop: unrolled and once a side, these few cold instructions
+            // cost the whole kernel 3 %)
             if (!wait_warp(v_tmp, vph)) return false;
             vph ^= 1;
             constexpr int kWords = 8 * X::kPanels;
-            const int r0 = sg.sl & (kPg - 1);
-            const uint32_t pg =
-                dst + ((sg.sl - 1) & (kKeys - 1)) / kPg * X::kPage;
-            for (int i = lane; i < (kPg - r0) * kWords; i += 32) {
-              const int c = i % kWords, r = r0 + i / kWords;
-              const uint32_t d = pg + (r >> 3) * X::kRows8 + (c >> 3) * 1024 +
-                                 (r & 7) * 128 + (c & 7) * 16;
-              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};"
-                           :: "r"(d), "r"(0) : "memory");
+            const int z0 = lo - tile * kKeys, z1 = sg.sl - tile * kKeys;
+#pragma unroll 1
+            for (int e = 0; e < 2; ++e) {
+              const int r0 = e ? z1 : max(z0 & -kPg, 0);
+              const int r1 = e ? min((z1 + kPg - 1) & -kPg, kKeys) : max(z0, 0);
+#pragma unroll 1
+              for (int i = lane; i < (r1 - r0) * kWords; i += 32) {
+                const int c = i % kWords, r = r0 + i / kWords;
+                const uint32_t d = dst + (r >> 3) * X::kRows8 +
+                                   (c >> 3) * 1024 + (r & 7) * 128 +
+                                   (c & 7) * 16;
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};"
+                             :: "r"(d), "r"(0) : "memory");
+              }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();

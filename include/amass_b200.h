@@ -663,8 +663,8 @@ typedef struct AmassChunk {
  * without a key become 0, rows outside every request are left as they are;
  * lse (n_tokens, n_kv * G) fp32 or null: natural log of the row's sum of
  * exp(scale q.k), -inf without a key.  Cache slots behind a request's last
- * token may hold anything; block ids outside [0, num_blocks) read as zeros;
- * seq_lens is cut at max_pages * page.  n_ctas is the GPU's SM count.  Of
+ * token, or before the windows of all its rows, may hold anything; block ids
+ * outside [0, num_blocks) read as zeros; seq_lens is cut at max_pages * page.  n_ctas is the GPU's SM count.  Of
  * the scratch (acc_part, ml_part, tickets) only the tickets need to be 0
  * before the first call, and are left 0; calls that overlap on the GPU need
  * scratch of their own.  fault[0] becomes 1 when a CTA gave up a bounded wait:

@@ -105,6 +105,32 @@ def test_window(dev, window, d):
           window=window)
 
 
+@pytest.mark.parametrize("window,dtype,d,G", [
+    (5, torch.bfloat16, 128, 4), (40, torch.float16, 64, 4),
+    (129, torch.bfloat16, 64, 1), (300, torch.bfloat16, 128, 8)])
+def test_before_the_window(dev, window, dtype, d, G):
+    """Slots before every row's window hold anything (an engine has given
+    their pages away): nothing of it reaches a row."""
+    lens = [(1, 1000), (1, 17), (70, 900), (300, 1333), (3, 128), (1, 645),
+            (33, 33), (2, 2500)]
+    c = make(dev, lens, n_kv=2, G=G, d=d, dtype=dtype, seed=11)
+    clean, lse = check(c, dev, window=window)
+    for r, (new, n) in enumerate(lens):
+        first = max(n - new - window + 1, 0)
+        pos = torch.arange(first, device=dev)
+        blk = c["bt"][r, pos // PAGE].long()
+        c["kv"][blk, 0, pos % PAGE] = float("nan")
+        c["kv"][blk, 1, pos % PAGE] = float("inf")
+        if r % 2:                            # pages of nobody
+            c["bt"][r, :first // PAGE] = -1
+    buf = ChunkBuffers(dev, n_kv=2, G=G, head_dim=d)
+    out, got = torch.full_like(clean, 7.0), torch.full_like(lse, 7.0)
+    paged_chunk_attention(c["q"], c["kv"], c["bt"], c["sl"], c["qsl"], out,
+                          buf, window=window, lse=got)
+    buf.check()
+    assert torch.equal(out, clean) and torch.equal(got, lse)
+
+
 def test_empty_rows_and_requests(dev):
     """Requests without new tokens, with none at all, and with fewer tokens
     than rows (their first rows see nothing: 0 and -inf)."""
