@@ -41,6 +41,11 @@
 // softmax -> product (3300 cycles a key tile of two row tiles, of which the
 // tensor core is busy 2048), then the board's power.
 //
+// Code size counts: hot and cold paths together are about what the instruction
+// caches hold, so loops stay rolled and paths shared where a unit's time does
+// not hang on it (158 KB -> 128 KB: fresh prompts 222 -> 206 us, one token 13.4
+// -> 12.9, 64-wide heads 103 -> 93).
+//
 // Slots behind a request's last token, or before all windows of an item's
 // rows, may hold anything: K's scores there are replaced before the maximum,
 // V's rows are zeroed in shared memory, whole pages are not read.
@@ -60,6 +65,7 @@ constexpr int kChMaxReq = 4096;
 // (query load, first scores, output)
 constexpr int kCost2 = 3, kCost1 = 2, kCostItem = 6, kMinRun = 4;
 constexpr float kRescaleLog2 = 8.f;
+constexpr uint32_t kWaitCycles = 2000000000u;    // a second or so
 constexpr int kPart = 96;                // keys whose weights go to O first
 
 struct ChunkArgs {
@@ -286,25 +292,24 @@ AMASS_DEV int ch_tiles(const ChunkArgs& a, const ChReq& q, int i, int* lo) {
   return end > 0 ? ((end + kKeys - 1) >> 7) - *lo : (*lo = 0, 1);
 }
 // sum over j < x of j >> s
-AMASS_DEV int64_t shift_sum(int64_t x, int s) {
-  const int64_t q = x >> s;
-  return ((q * (q - 1) / 2) << s) + q * (x - (q << s));
+AMASS_DEV int64_t shift_sum(int x, int s) {
+  const int q = x >> s;
+  return (((int64_t)q * (q - 1) / 2) << s) + (int64_t)q * (x - (q << s));
 }
-// sum over i in [i0, i1) of max(b + i * 2^tl, 0) >> 7
-AMASS_DEV int64_t floor_sum(int64_t b, int64_t i0, int64_t i1, int tl) {
+// sum over i in [i0, i1) of max(b + i * 2^tl, 0) >> 7; with c = b >> tl a
+// summand is (c + i) >> (7 - tl) up to tl = 7, and above that (c + i) <<
+// (tl - 7) plus the bits of b in between
+AMASS_DEV int64_t floor_sum(int b, int i0, int i1, int tl) {
   if (b < 0) {                           // first i with a value above 0
-    const int64_t z = ((-b) >> tl) + 1;
-    i0 = (i0 > z ? i0 : z) - z;
+    const int z = ((-b) >> tl) + 1;
+    i0 = max(i0, z) - z;
     i1 -= z;
     b += z << tl;
   }
   if (i0 >= i1) return 0;
-  if (tl >= 7) {
-    const int64_t n = i1 - i0;
-    return n * (b >> 7) + (((i0 + i1 - 1) * n / 2) << (tl - 7));
-  }
-  const int64_t c = b >> tl;
-  return shift_sum(i1 + c, 7 - tl) - shift_sum(i0 + c, 7 - tl);
+  const int c = b >> tl, s = max(7 - tl, 0), k = max(tl - 7, 0);
+  return ((shift_sum(i1 + c, s) - shift_sum(i0 + c, s)) << k) +
+         (int64_t)(i1 - i0) * ((b >> 7) & ((1 << k) - 1));
 }
 // cost of one key tile of item i
 AMASS_DEV int ch_weight(const ChunkArgs& a, const ChReq& q, int i) {
@@ -323,10 +328,8 @@ AMASS_DEV int64_t ch_cost(const ChunkArgs& a, const ChReq& q, int m) {
   }
   // items whose last position is negative visit one (empty) tile
   const int none = q.off < 0 ? min(full, (-q.off) >> tl) : 0;
-  int64_t u = none + floor_sum((int64_t)q.off + (1 << tl) + kKeys - 1, none,
-                               full, tl);
-  if (a.window)
-    u -= floor_sum((int64_t)q.off - a.window + 1, none, full, tl);
+  int64_t u = none + floor_sum(q.off + (1 << tl) + kKeys - 1, none, full, tl);
+  if (a.window) u -= floor_sum(q.off - a.window + 1, none, full, tl);
   return s + u * kCost2;
 }
 
@@ -747,8 +750,13 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   const uint32_t tmem = tmem_s;
 
   // bounded wait: after about a second the CTA records the fault and unwinds
+  // (mbar_wait in fewer instructions: there are some thirty of these)
   const auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
-    if (mbar_wait(bar, parity)) return true;
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint32_t t0 = clock();
+    do {
+      if (mbar_try_wait(bar, parity)) return true;
+    } while ((uint32_t)clock() - t0 < kWaitCycles);
     *a.fault = 1;
     return false;
   };
@@ -1049,27 +1057,25 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
                      (two ? t : 0) * 128 + row;
       if (live) {
 #pragma unroll 1
-        for (int c = 0; c < D; c += 64) {
-          uint32_t o[64];
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
           tc_ld32(o, to + c);
-          tc_ld32(o + 32, to + c + 32);
           tc_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
+          for (int e = 0; e < 32; ++e)
             o[e] = __float_as_uint(__uint_as_float(o[e]) * f0);
           if (paired) {
-            uint32_t o1[64];
+            uint32_t o1[32];
             tc_ld32(o1, to + D + c);
-            tc_ld32(o1 + 32, to + D + c + 32);
             tc_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 64; ++e)
+            for (int e = 0; e < 32; ++e)
               o[e] = __float_as_uint(fmaf(__uint_as_float(o1[e]), f1,
                                           __uint_as_float(o[e])));
           }
           if (whole) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
+            for (int k = 0; k < 4; ++k) {
               uint32_t w[4];
 #pragma unroll
               for (int x = 0; x < 4; ++x) {
@@ -1077,12 +1083,13 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
                 const float hi = __uint_as_float(o[8 * k + 2 * x + 1]);
                 w[x] = kF16 ? pack_h2(lo, hi) : pack_bf2(lo, hi);
               }
-              stage_put(stage, k, make_uint4(w[0], w[1], w[2], w[3]));
+              stage_put(stage, (c & 32) / 8 + k,
+                        make_uint4(w[0], w[1], w[2], w[3]));
             }
-            stage_out(stage, valid ? orow + 2 * c : nullptr);
+            if (c & 32) stage_out(stage, valid ? orow + 2 * c - 64 : nullptr);
           } else if (valid) {
 #pragma unroll
-            for (int e = 0; e < 64; e += 4)
+            for (int e = 0; e < 32; e += 4)
               prow[(c + e) / 4 * 256] = make_float4(
                   __uint_as_float(o[e]), __uint_as_float(o[e + 1]),
                   __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
@@ -1161,30 +1168,44 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
         const int tlo = lo & (kPg - 1) ? lo >> 7 : -1;
         const int thi = sg.sl & (kPg - 1) ? sg.sl >> 7 : -1;
         const int32_t* row = a.bt + (int64_t)sg.r * a.bt_stride;
-        // block of the tile's page (lane & 7); pages that are not the
-        // request's, or before all windows, read as zeros (a block behind the
-        // cache)
-        const auto block_of = [&](int tile) {
-          const int p = tile * (kKeys / kPg) + (lane & 7);
+        // lane 8 (t & 3) + p: block of page p of tile t, four tiles at once;
+        // pages that are not the request's, or before all windows, read as
+        // zeros (a block behind the cache)
+        const auto blocks_of = [&](int group) {
+          const int p = group * 32 + lane;
           int b = -1;
           if (p < npg && p >= (lo >> 4)) b = row[p];
           return b < 0 || b >= a.nb ? a.nb : b;
         };
-        const auto load = [&](bool is_v, int tile, int blk) -> bool {
-          if (!wait_warp(empty(st), ph)) return false;
+        // in the order of use, `lead` tiles of K before the first of V: the
+        // ring then covers the same time for both.  One loop for both: the
+        // kernel is as large as the instruction caches
+        const int lead = sg.ntok > tm ? 1 : 2, end = sg.t0 + sg.n;
+        int kt = sg.t0, vt = sg.t0;      // the next tiles of K and of V
+        int even = 0, odd = 0;           // blocks of groups of four tiles
+        const auto fetch = [&](int group) {
+          const int b = blocks_of(group);
+          if (group & 1) odd = b; else even = b;
+        };
+        fetch(kt >> 2);
+        if ((kt & 3) == 3) fetch((kt >> 2) + 1);
+#pragma unroll 1
+        while (vt < end) {
+          const bool is_v = kt == end || kt - vt == lead;
+          const int tile = is_v ? vt++ : kt++;
+          if (!(ok = wait_warp(empty(st), ph))) break;
           const bool part = is_v && (tile == tlo || tile == thi);
           const uint32_t dst = ring + st * X::kTile;
           const uint32_t bar = part ? v_tmp : full(st);
           if (lane == 0) mbar_arrive_expect_tx(bar, X::kTile);
           __syncwarp();
-          if (lane < 8)
-            tma_5d(dst + lane * X::kPage, is_v ? &mv : &mk, bar,
-                   blk * a.bh + sg.h);
+          if ((lane >> 3) == (tile & 3))
+            tma_5d(dst + (lane & 7) * X::kPage, is_v ? &mv : &mk, bar,
+                   (tile & 4 ? odd : even) * a.bh + sg.h);
+          if (!is_v && (tile & 3) == 2) fetch((tile >> 2) + 1);
           if (part) {
-            // whatever the others hold, 0 * it must be 0 in P V (one small
-            // loop: unrolled and once a side, these few cold instructions
-            // cost the whole kernel 3 %)
-            if (!wait_warp(v_tmp, vph)) return false;
+            // whatever the others hold, 0 * it must be 0 in P V
+            if (!(ok = wait_warp(v_tmp, vph))) break;
             vph ^= 1;
             constexpr int kWords = 8 * X::kPanels;
             const int z0 = lo - tile * kKeys, z1 = sg.sl - tile * kKeys;
@@ -1207,22 +1228,6 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
             if (lane == 0) mbar_arrive(full(st));
           }
           if (++st == NS) { st = 0; ph ^= 1; }
-          return true;
-        };
-        // in the order of use, `lead` tiles of K before the first of V: the
-        // ring then covers the same time for both
-        const int lead = sg.ntok > tm ? 1 : 2;
-        int b0 = block_of(sg.t0);
-        int b1 = sg.n > 1 ? block_of(sg.t0 + 1) : 0;
-        ok = load(false, sg.t0, b0);
-        if (ok && lead == 2 && sg.n > 1) ok = load(false, sg.t0 + 1, b1);
-        for (int j = 0; ok && j < sg.n; ++j) {
-          const int b2 = j + 2 < sg.n ? block_of(sg.t0 + j + 2) : 0;
-          ok = load(true, sg.t0 + j, b0) &&
-               (j + lead >= sg.n ||
-                load(false, sg.t0 + j + lead, lead == 1 ? b1 : b2));
-          b0 = b1;
-          b1 = b2;
         }
       }
       if (!ok) {
@@ -1321,47 +1326,41 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
         __syncwarp();
         return true;
       };
-      const auto scores_of = [&](int t, uint64_t q0, int e, bool done) {
-        scores(t, q0, e >= NS ? e - NS : e, done);
-      };
       while (ok && next_seg()) {
+        // two row tiles share every key tile; one row tile's key tiles go to
+        // the two warpgroups in turn
         const int n = sg.n;
         const bool two = sg.ntok > (1 << a.tm_log2);
-        const int k0 = take();
-        if (!(ok = wait_warp(q_full, qph & 1) && arrived(k0))) break;
-        tc_after();
-        scores_of(0, qd, k0, !two);
-        if (two) {
-          if (!(ok = wait_warp(q_full + 8, (qph >> 1) & 1))) break;
-          qph ^= 3;
+        int k = take(), v = 0;
+        if (!(ok = wait_warp(q_full, qph & 1) && arrived(k))) break;
+        const uint64_t q1 = two ? qd + kStep : qd;
+#pragma unroll 1
+        for (int t = 0; t < (two || n > 1 ? 2 : 1); ++t) {
+          if (t) {
+            if (!two) k = take();
+            if (!(ok = two ? wait_warp(q_full + 8, (qph >> 1) & 1)
+                           : arrived(k)))
+              break;
+          }
           tc_after();
-          scores_of(1, qd + kStep, k0, true);
-          if (n == 1) {
-            commit(q_empty);
-            commit(q_empty + 8);
+          scores(t, t ? q1 : qd, k >= NS ? k - NS : k, !two || t);
+        }
+        if (!ok) break;
+        qph ^= two ? 3 : 1;
+        if (n <= (two ? 1 : 2)) commit(q_empty);
+        if (two && n == 1) commit(q_empty + 8);
+        const int ahead = two ? 1 : 2;
+#pragma unroll 1
+        for (int i = 0; i < (two ? 2 * n : n); ++i) {
+          const int t = i & 1, j = two ? i >> 1 : i;
+          if (!two || !t) {
+            v = take();
+            k = j + ahead < n ? take() : -1;
           }
-          for (int j = 0; j < n; ++j) {
-            const int v = take(), k = j + 1 < n ? take() : -1;
-            if (!(ok = turn(0, v, j > 0, qd, k, 1, false))) break;
-            if (j + 2 == n) commit(q_empty);
-            if (!(ok = turn(1, v, j > 0, qd + kStep, k, 0, true))) break;
-            if (j + 2 == n) commit(q_empty + 8);
-          }
-        } else {
-          // one row tile: the two warpgroups take its key tiles in turn
-          qph ^= 1;
-          if (n > 1) {
-            const int k1 = take();
-            if (!(ok = arrived(k1))) break;
-            tc_after();
-            scores_of(1, qd, k1, true);
-          }
-          if (n <= 2) commit(q_empty);
-          for (int j = 0; j < n; ++j) {
-            const int v = take(), k = j + 2 < n ? take() : -1;
-            if (!(ok = turn(j & 1, v, j > 1, qd, k, 2, true))) break;
-            if (j + 3 == n) commit(q_empty);
-          }
+          if (!(ok = turn(t, v, j >= ahead, t ? q1 : qd, k,
+                          two ? 1 - t : 2, !two || t)))
+            break;
+          if (j + ahead + 1 == n) commit(q_empty + (two && t ? 8 : 0));
         }
       }
       // every MMA and its arrivals end before the CTA does
@@ -1528,7 +1527,8 @@ extern "C" int amass_paged_chunk(const AmassChunk* args, void* stream) {
   a.scale_log2 = x.scale * kLog2e;
   a.n_req = x.n_req; a.n_kv = x.n_kv; a.G = x.G; a.T = x.n_tokens;
   a.bh = (int)bh; a.max_pages = x.max_pages; a.nb = x.num_blocks;
-  a.window = x.window;
+  // no request is longer than 2^30 tokens
+  a.window = x.window < 1 << 30 ? x.window : 0;
   // tokens of a row tile: the largest power of two whose G heads fit 128 rows
   a.tm_log2 = x.G == 1 ? 7 : x.G == 2 ? 6 : x.G <= 4 ? 5 : 4;
   const bool f16 = x.dtype == AMASS_FP16;

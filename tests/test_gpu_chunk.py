@@ -142,6 +142,16 @@ def test_empty_rows_and_requests(dev):
     assert bool((out == 7.0).all())
 
 
+def test_windows_beyond_any_length(dev):
+    """A window as long as the types hold is none, for rows before position 0
+    too."""
+    c = make(dev, [(40, 200), (9, 4), (1, 300), (5, 0)])
+    want = check(c, dev)
+    for window in (2 ** 30, 2 ** 31 - 1, 2 ** 40):
+        got = check(c, dev, window=window)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_strides_and_layouts(dev):
     """q out of a fused projection, out into a wider row, both cache layouts,
     a block table with wider rows."""
