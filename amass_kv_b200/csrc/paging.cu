@@ -6,7 +6,8 @@
 //           have_r,
 //           upto_r = need_0 + .. + need_r; request r is granted its pages iff
 //           need_r = 0 or upto_r <= free blocks (in order: the first that
-//           does not fit also refuses every later one that needs pages);
+//           does not fit also refuses every later one that needs pages), its
+//           row holds old_r + new_r tokens and the step 2^30;
 //           its j-th new page takes
 //           free_stack[top - 1 - (upto_r - need_r + j)];
 //           token t of request r (start_r <= t < start_r + new_r) has position
@@ -29,24 +30,26 @@ namespace {
 
 constexpr int kPgThreads = 512;
 constexpr int kPgMaxReq = 4096;          // 32 KB of request sums
+constexpr int kPgMaxTok = 1 << 30;       // tokens of a step
 
 AMASS_DEV int pages_of(int tokens, int page) {   // tokens + page < 2^32
   return (int)(((unsigned)tokens + (unsigned)page - 1u) / (unsigned)page);
 }
 
 // exclusive prefix of (a, b) over the CTA's threads; *ta, *tb the totals
-AMASS_DEV void scan2(int& a, int& b, int* ta, int* tb) {
-  __shared__ int wa[kPgThreads / 32], wb[kPgThreads / 32];
+AMASS_DEV void scan2(int64_t& a, int64_t& b, int64_t* ta, int64_t* tb) {
+  __shared__ int64_t wa[kPgThreads / 32], wb[kPgThreads / 32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int ia = a, ib = b;
+  int64_t ia = a, ib = b;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int xa = __shfl_up_sync(~0u, ia, o), xb = __shfl_up_sync(~0u, ib, o);
+    const int64_t xa = __shfl_up_sync(~0u, ia, o);
+    const int64_t xb = __shfl_up_sync(~0u, ib, o);
     if (lane >= o) { ia += xa; ib += xb; }
   }
   if (lane == 31) { wa[w] = ia; wb[w] = ib; }
   __syncthreads();
-  int oa = 0, ob = 0, sa = 0, sb = 0;
+  int64_t oa = 0, ob = 0, sa = 0, sb = 0;
 #pragma unroll
   for (int i = 0; i < kPgThreads / 32; ++i) {
     if (i < w) { oa += wa[i]; ob += wb[i]; }
@@ -97,38 +100,41 @@ pages_begin_kernel(const __grid_constant__ AmassPagePool p,
   extern __shared__ int sm[];
   int* start = sm;                       // n_req + 1: first token
   int* pre = sm + n_req + 1;             // n_req: first new block, -1 refused
-  __shared__ int used;                   // blocks granted
+  __shared__ int used, reach;            // blocks granted, last token of one
   const int tid = threadIdx.x, most = p.max_pages * p.page;
-  if (tid == 0) used = 0;                // set before scan2's barriers
+  if (tid == 0) used = reach = 0;        // set before scan2's barriers
   const int top = min(max(*p.free_top, 0), p.num_blocks);
   const int per = (n_req + kPgThreads - 1) / kPgThreads;
   const int r0 = min(n_req, tid * per), r1 = min(n_req, r0 + per);
-  int sn = 0, sd = 0;
+  int64_t sn = 0, sd = 0, all, need_all;  // 4096 rows can ask for 2^43 tokens
   for (int r = r0; r < r1; ++r) {
     const int nw = max(new_tokens[r], 0), old = max(p.seq_lens[r], 0);
     const int64_t want = (int64_t)old + nw;
     sn += nw;
     if (want <= most) sd += pages_of((int)want, p.page) - pages_of(old, p.page);
   }
-  int total, need_all;
-  scan2(sn, sd, &total, &need_all);
+  scan2(sn, sd, &all, &need_all);
+  const int total = (int)min(all, (int64_t)kPgMaxTok);
   int flags = 0;
   for (int r = r0; r < r1; ++r) {
     const int nw = max(new_tokens[r], 0), old = max(p.seq_lens[r], 0);
     const int64_t want = (int64_t)old + nw;
-    start[r] = sn;
+    start[r] = (int)min(sn, (int64_t)kPgMaxTok);
     sn += nw;
     int st = 0, need = 0;
-    if (want > most) {
-      st = 2;
-    } else {
+    if (want <= most)
       need = pages_of((int)want, p.page) - pages_of(old, p.page);
-      if (need > 0 && sd + need > top) st = 1;
-    }
-    pre[r] = st ? -1 : sd;
+    if (want > most || (nw > 0 && sn > kPgMaxTok))
+      st = 2;
+    else if (need > 0 && sd + need > top)
+      st = 1;
+    pre[r] = st ? -1 : (int)min(sd, (int64_t)top);
     sd += need;
     flags |= st;
-    if (st == 0 && need > 0) atomicMax(&used, sd);   // granted: a prefix
+    if (st == 0 && need > 0) {           // granted: a prefix
+      atomicMax(&used, (int)sd);
+      atomicMax(&reach, (int)sn);
+    }
     if (blockIdx.x == 0) {
       p.status[r] = st;
       p.query_start_loc[r] = start[r];
@@ -140,7 +146,7 @@ pages_begin_kernel(const __grid_constant__ AmassPagePool p,
   }
   __syncthreads();
 
-  const int end = max(total, n_tokens);
+  const int end = max(reach, n_tokens);
   for (int64_t t = (int64_t)blockIdx.x * kPgThreads + tid; t < end;
        t += (int64_t)gridDim.x * kPgThreads) {
     int64_t pos = 0, slot = -1;
@@ -150,7 +156,7 @@ pages_begin_kernel(const __grid_constant__ AmassPagePool p,
       pos = (int64_t)old + (t - start[r]);
       const int pg = (int)((unsigned)pos / (unsigned)p.page);
       const int off = (int)pos - pg * p.page;
-      if (pre[r] >= 0 && pg < p.max_pages) {
+      if (pre[r] >= 0 && pos < most) {
         const int have = pages_of(old, p.page);
         int32_t* e = p.block_table + (int64_t)r * p.bt_stride + pg;
         int b = -1;
@@ -176,13 +182,12 @@ pages_begin_kernel(const __grid_constant__ AmassPagePool p,
   if (!last_cta(p.ticket)) return;
   for (int r = r0; r < r1; ++r) {
     if (pre[r] < 0) continue;
-    const int nx = r + 1 < n_req ? start[r + 1] : total;
-    p.seq_lens[r] = max(p.seq_lens[r], 0) + (nx - start[r]);
+    p.seq_lens[r] = max(p.seq_lens[r], 0) + (start[r + 1] - start[r]);
   }
   if (tid == 0) {
     *p.free_top = top - used;
     const int f = (short_f ? 1 : 0) | (long_f ? 2 : 0) |
-                  (total > n_tokens ? 4 : 0);
+                  (all > n_tokens ? 4 : 0);
     if (f) *p.overflow |= f;
   }
 }
@@ -207,18 +212,19 @@ pages_trim_kernel(const __grid_constant__ AmassPagePool p,
     *have = pages_of(old, p.page);
     return old - d;
   };
-  int s = 0, zero = 0, total, z;
+  int64_t s = 0, zero = 0, all, z;
   for (int i = i0; i < i1; ++i) {
     int have;
     const int k = kept(n_req - 1 - i, &have);
     s += have - pages_of(k, p.page);
   }
-  scan2(s, zero, &total, &z);
+  scan2(s, zero, &all, &z);
+  const int total = (int)all;            // held pages: no more than blocks
   for (int i = i0; i < i1; ++i) {
     const int r = n_req - 1 - i;
     int have;
     left[r] = kept(r, &have);
-    start[i] = s;
+    start[i] = (int)s;
     s += have - pages_of(left[r], p.page);
   }
   if (tid == 0) start[n_req] = total;
@@ -258,7 +264,7 @@ slot_map_kernel(const int32_t* __restrict__ block_table, int64_t bt_stride,
       const int r = find_start(sm, n_req, (int)t);
       pos = (int64_t)seq_lens[r] - (sm[r + 1] - t);
       const int pg = (int)((unsigned)pos / (unsigned)page);
-      if (pos >= 0 && pg < max_pages) {
+      if (pos >= 0 && pos < (int64_t)max_pages * page) {
         const int b = block_table[(int64_t)r * bt_stride + pg];
         if (b >= 0) slot = (int64_t)b * page + ((int)pos - pg * page);
       }

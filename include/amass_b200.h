@@ -567,14 +567,14 @@ typedef struct AmassPagePool {
  * up to and including r do not exceed free_top[0].  The k-th block granted is
  * free_stack[top - 1 - k]; it is entered in block_table, free_top and
  * seq_lens follow.  status[r]: 0 granted, 1 too few free blocks, 2 more than
- * max_pages pages (then it counts as needing none); a refused request keeps
- * its pages and length.  query_start_loc (n_req + 1): prefix sums of the new
- * tokens, refused requests included.  For token t < n_tokens of request r:
+ * max_pages pages (then it counts as needing none) or new tokens past the
+ * 2^30th of the step; a refused request keeps its pages and length.
+ * query_start_loc (n_req + 1): prefix sums of the new tokens, refused
+ * requests included, at most 2^30.  For token t < n_tokens of request r:
  * positions[t] = old + (t - query_start_loc[r]), slot_mapping[t] = block *
  * page + offset, or -1 when refused; behind the last token 0 and -1.
  * overflow[0] |= 1 (a status 1), 2 (a status 2), 4 (more than n_tokens new
- * tokens: the maps end there).  One launch.  max_reqs <= 4096; the new
- * tokens' sum fits int32. */
+ * tokens: the maps end there).  One launch.  max_reqs <= 4096. */
 int amass_pages_begin(const AmassPagePool* pool, const int32_t* new_tokens,
                       int n_req, int n_tokens, void* stream);
 

@@ -148,6 +148,23 @@ def test_refusals_on_the_device(dev):
     assert p.query_start_loc.tolist()[0] == 0
 
 
+def test_counts_past_any_step(dev):
+    """New tokens whose sum passes 32 bits: those rows and the later ones are
+    refused, nothing wraps, a row that asks for none stays granted."""
+    big, end = 2 ** 31 - 1, 2 ** 30
+    p = BlockPool(dev, num_blocks=9, max_reqs=6, max_pages=3, max_tokens=40)
+    p.begin_step(i32([5, big, big, 7, 0, big], dev), n_tokens=30)
+    assert p.status.tolist() == [0, 2, 2, 2, 0, 2]
+    assert p.seq_lens.tolist() == [5, 0, 0, 0, 0, 0]
+    assert p.query_start_loc.tolist() == [0, 5] + [end] * 5
+    assert int(p.free_top) == 8 and int(p.overflow) == 2 + 4
+    assert p.block_table[1:].max() == -1 and p.block_table[0, 1:].max() == -1
+    assert p.slot_mapping[:30].tolist() == list(range(5)) + [-1] * 25
+    p.begin_step(i32([30, 30, 3, 0, 16, 16], dev))
+    assert p.seq_lens.tolist() == [35, 30, 3, 0, 16, 16]
+    assert int(p.free_top) == 9 - 3 - 2 - 1 - 1 - 1
+
+
 def test_captured(dev):
     """One graph serves steps of other counts, padded to its size."""
     p = BlockPool(dev, num_blocks=300, max_reqs=8, max_pages=40,
