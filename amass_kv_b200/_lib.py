@@ -161,6 +161,8 @@ def call(name: str, *args) -> None:
 def launch(index: int, name: str, *args) -> None:
     """``call`` with GPU ``index`` current and its current stream as the last
     argument."""
+    if index < 0:
+        raise ValueError(f"{name}: the tensors must be on a GPU")
     fn = getattr(_lib or load(), name)
     if torch.cuda.current_device() == index:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
@@ -177,6 +179,20 @@ def device_of(device) -> torch.device:
     if dev.type == "cuda" and dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())
     return dev
+
+
+class FixedBuffers:
+    """Base of what owns GPU buffers whose addresses it has packed for the C
+    side: once ``_fixed`` is set its attributes stay, and it is not copied."""
+
+    def __setattr__(self, name, value):
+        if getattr(self, "_fixed", False):
+            raise AttributeError(f"{type(self).__name__}.{name} is fixed: "
+                                 "fill the buffers in place")
+        object.__setattr__(self, name, value)
+
+    def __reduce__(self):
+        raise TypeError(f"a {type(self).__name__} is not copied: make another")
 
 
 def ptr(t) -> int:

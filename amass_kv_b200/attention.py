@@ -144,7 +144,7 @@ def cache_layout(kv_cache):
     return (shape[b], shape[2], shape[3], shape[4], (s[b], s[2], s[3]), p, v)
 
 
-class ChunkBuffers:
+class ChunkBuffers(_lib.FixedBuffers):
     """Scratch of ``paged_chunk_attention`` for one head geometry, allocated
     once (outside any graph): the fp32 partials of the rows that two or more
     SMs share.  Calls that may overlap on the GPU -- other streams, two
@@ -171,6 +171,7 @@ class ChunkBuffers:
         self.fault = torch.zeros(1, device=dev, dtype=torch.int32)
         self.scratch = (ptr(self.acc_part), ptr(self.ml_part),
                         ptr(self.tickets), ptr(self.fault))
+        self._fixed = True
 
     def check(self) -> None:
         if int(self.fault.item()):

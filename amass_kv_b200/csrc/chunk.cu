@@ -1486,7 +1486,7 @@ extern "C" int amass_paged_chunk(const AmassChunk* args, void* stream) {
   const uintptr_t bases = (uintptr_t)x.q | (uintptr_t)x.k | (uintptr_t)x.v |
                           (uintptr_t)x.out | (uintptr_t)x.acc_part |
                           (uintptr_t)x.ml_part;
-  if ((bases & 15) || ((x.o_st | x.o_sh) & 7)) return AMASS_ERR_ARG;
+  if (bases & 15) return AMASS_ERR_ARG;
   const uint64_t d = (uint64_t)x.head_dim;
   const uint64_t qdim[3] = {d, (uint64_t)(x.n_kv * x.G),
                             (uint64_t)x.n_tokens};
@@ -1501,6 +1501,7 @@ extern "C" int amass_paged_chunk(const AmassChunk* args, void* stream) {
     return used && (s <= 0 || (s & 7));
   };
   if (bad(x.n_kv * x.G > 1, x.q_sh) || bad(x.n_tokens > 1, x.q_st) ||
+      bad(x.n_kv * x.G > 1, x.o_sh) || bad(x.n_tokens > 1, x.o_st) ||
       bad(true, x.k_st) || bad(true, x.v_st) || bad(x.n_kv > 1, x.k_sh) ||
       bad(x.n_kv > 1, x.v_sh) || bad(x.num_blocks > 1, x.k_sb) ||
       bad(x.num_blocks > 1, x.v_sb))

@@ -24,7 +24,7 @@ from .attention import check_i32
 MAX_REQS = 4096
 
 
-class BlockPool:
+class BlockPool(_lib.FixedBuffers):
     """Device-resident block allocator, allocated once.
 
       free_stack (NB,), free_top (1,)   free blocks, popped from the top
@@ -35,8 +35,8 @@ class BlockPool:
       status (R,), overflow (1,)        what begin_step refused
 
     All int32 but the two token maps.  ``status[r]``: 0 granted, 1 too few
-    free blocks, 2 longer than ``max_pages``; a refused row keeps its pages
-    and length and its new tokens get slot -1.  ``overflow`` latches 1 / 2
+    free blocks, 2 longer than ``max_pages`` or past 2^30 tokens in the step;
+    a refused row keeps its pages and length and its new tokens get slot -1.  ``overflow`` latches 1 / 2
     for such a row and 4 for more new tokens than the step's ``n_tokens``;
     ``check()`` reads it (synchronises) and raises.
 
@@ -81,12 +81,6 @@ class BlockPool:
             self.block_table.stride(0), num_blocks, max_reqs, max_pages,
             max_tokens, page, 0)
         self._fixed = True
-
-    def __setattr__(self, name, value):
-        if getattr(self, "_fixed", False):
-            raise AttributeError(f"BlockPool.{name} is fixed: fill the "
-                                 "buffers in place")
-        object.__setattr__(self, name, value)
 
     def _rows(self, t, name: str) -> int:
         check_i32(self._index, name, t, 1)

@@ -118,7 +118,6 @@ class Rotary:
         turns = [round(x / (2 * math.pi) * 2.0 ** 64)
                  for x in self.inv_freq.tolist()]
         self.freq = torch.tensor(turns, dtype=torch.int64, device=dev)
-        self._freq = self.freq.data_ptr()
 
 
 _NONE = (0, 0, 0, 0)                     # pointer, token / head stride, heads
@@ -164,6 +163,9 @@ def _launch(rot, x, q, q_out, k, v, k_dst, kd, v_dst, vd, slots, nb, page,
         o = _rows(rot, "q_out", q_out, dtype, T, d)
     if o[3] != H:
         raise ValueError("q_out must have q's heads")
+    if (q is not None and 0 in o[1:3]) or (v is not None and 0 in vd) or \
+            (k is not None and 0 in (kd if slots else kd[::2])):
+        raise ValueError("q_out, k_out and the caches must not be expanded")
     kp, k_st, k_sh, n_kv = _NONE if k is None else \
         _rows(rot, "k", k, dtype, T, d)
     vp, v_st, v_sh, nv = _NONE if v is None else \
@@ -174,8 +176,8 @@ def _launch(rot, x, q, q_out, k, v, k_dst, kd, v_dst, vd, slots, nb, page,
     if T == 0:
         return
     _lib.launch(rot.index, "amass_rotary_write", _lib.ROTARY.pack(
-        qp, o[0], kp, vp, k_dst, v_dst, slots, pos, rot._freq, q_st, q_sh,
-        o[1], o[2], k_st, k_sh, v_st, v_sh, *kd, *vd, rot.mscale, nb, page,
+        qp, o[0], kp, vp, k_dst, v_dst, slots, pos, rot.freq.data_ptr(), q_st,
+        q_sh, o[1], o[2], k_st, k_sh, v_st, v_sh, *kd, *vd, rot.mscale, nb, page,
         positions.dtype == torch.int64, LAYOUTS[rot.layout], rot.rotary_dim,
         T, H, n_kv, d, DTYPES[dtype], 0))
 

@@ -108,6 +108,10 @@ class MemSession:
         as it is) and ``query`` (T, H, d), when given, in place, in the same
         launch."""
         l = int(layer)
+        if (rotary is None) != (positions is None) or \
+                (rotary is None and query is not None):
+            raise ValueError("rotary and positions go together, and query "
+                             "goes with them")
         if rotary is not None:
             n = int(n_tokens)
             if self.offload_k:

@@ -169,6 +169,14 @@ def test_strides_and_layouts(dev):
         assert bool((wide[:, H] == 3.0).all())
 
 
+def test_one_row_of_any_stride(dev):
+    """A single token's strides are not used, whatever they are."""
+    c = make(dev, [(1, 77)], tail=0)
+    q, out = (torch.zeros(1, 8 * 128 + 4, device=dev, dtype=torch.bfloat16)
+              [:, :8 * 128].view(1, 8, 128) for _ in range(2))
+    check(c, dev, q=q.copy_(c["q"]), out=out)
+
+
 def test_heads_before_tokens(dev):
     """A cache stored (blocks, 2, heads, page, d), seen as (.., page, heads,
     d), and q in place."""

@@ -1,4 +1,5 @@
 """Rotary positions and the cache write against fp64."""
+import copy
 import math
 
 import pytest
@@ -161,6 +162,18 @@ def test_odd_strides_and_alignment(dev):
     close(odd, want)
     close(kv[0, slots // 16, slots % 16], turned(rot, k, pos))
     assert torch.equal(kv[1, slots // 16, slots % 16], v)
+
+
+def test_copied_rotary(dev):
+    """A copy has frequencies of its own."""
+    rot = Rotary(dev, rotary_dim=64)
+    k = torch.randn(9, 2, 64, device=dev).to(torch.bfloat16)
+    at, other = torch.arange(9, device=dev), copy.deepcopy(rot)
+    a, b = k.clone(), k.clone()
+    rotary_embed(rot, None, a, at)
+    rot.freq.zero_()
+    rotary_embed(other, None, b, at)
+    assert torch.equal(a, b)
 
 
 def test_captured_padded_batch(dev):

@@ -1,5 +1,6 @@
 """Calls the prefill-side entry points refuse, checked before any launch (no
 GPU needed)."""
+import copy
 import ctypes
 
 import pytest
@@ -8,7 +9,9 @@ import torch
 from amass_kv_b200 import _lib
 from amass_kv_b200.attention import paged_chunk_attention
 from amass_kv_b200.paging import BlockPool, build_slot_map
-from amass_kv_b200.rotary import Rotary, rotary_embed, rotary_write_kv
+from amass_kv_b200.rotary import (Rotary, rotary_embed, rotary_write_kv,
+                                  rotary_write_pools)
+from amass_kv_b200.serving import MemSession
 
 CPU = torch.device("cpu")
 
@@ -179,3 +182,67 @@ def test_rotary_calls_refuse():
         rotary_embed(rot, a["q"], None, torch.arange(5), k_out=a["k"])
     with pytest.raises(ValueError):
         rotary_embed(rot, a["q"][..., :32], None, torch.arange(5))
+
+
+def test_host_tensors_are_refused():
+    """Arguments that fit in all but the device never reach a launch."""
+    i32, bf = torch.int32, torch.bfloat16
+    p = BlockPool(CPU, num_blocks=4, max_reqs=2, max_pages=3, max_tokens=9)
+    rot = Rotary(CPU, rotary_dim=64)
+    one = torch.ones(2, dtype=i32)
+    q, at = torch.zeros(5, 8, 64, dtype=bf), torch.arange(5)
+
+    class Whole(Buf):
+        n_ctas, scratch = 1, (64, 64, 64, 64)
+    for call in (
+            lambda: p.begin_step(one), lambda: p.truncate(one),
+            lambda: p.release(one),
+            lambda: build_slot_map(p.block_table, one, torch.zeros(3, dtype=i32),
+                                   p.positions, p.slot_mapping),
+            lambda: rotary_embed(rot, q, None, at),
+            lambda: rotary_embed(rot, None, q, at),
+            lambda: rotary_write_kv(
+                rot, q, q[:, :2], q[:, :2], at,
+                torch.zeros(4, 2, 16, 2, 64, dtype=bf), at),
+            lambda: paged_chunk_attention(**chunk_args(buf=Whole()))):
+        with pytest.raises(ValueError, match="on a GPU"):
+            call()
+
+
+def test_expanded_outputs_are_refused():
+    """One place for two heads, tokens or pages has no one answer."""
+    rot, bf = Rotary(CPU, rotary_dim=64), torch.bfloat16
+    at, q = torch.arange(5), torch.zeros(5, 8, 64, dtype=bf)
+    one, k = torch.zeros(5, 1, 64, dtype=bf), q[:, :2]
+    wide = one.expand(5, 8, 64)
+    for call in (
+            lambda: rotary_embed(rot, wide, None, at),
+            lambda: rotary_embed(rot, q, None, at, q_out=wide),
+            lambda: rotary_embed(rot, None, wide, at),
+            lambda: rotary_embed(rot, None, q, at, k_out=wide),
+            lambda: rotary_write_kv(
+                rot, q, k, k, at, torch.zeros(1, 2, 16, 2, 64, dtype=bf)
+                .expand(4, 2, 16, 2, 64), at),
+            lambda: rotary_write_pools(
+                rot, None, k, k, at, torch.zeros(4, 16, 2, 64, dtype=bf),
+                torch.zeros(4, 1, 2, 64, dtype=bf).expand(4, 16, 2, 64), at)):
+        with pytest.raises(ValueError, match="expanded"):
+            call()
+
+
+def test_buffers_are_not_copied():
+    """Copies would keep the addresses of the buffers they were taken from."""
+    p = BlockPool(CPU, num_blocks=4, max_reqs=2, max_pages=3, max_tokens=9)
+    for f in (copy.copy, copy.deepcopy):
+        with pytest.raises(TypeError, match="not copied"):
+            f(p)
+    assert copy.deepcopy(Rotary(CPU, rotary_dim=8)).freq.numel() == 4
+
+
+def test_write_kv_refuses_half_a_rotary():
+    rot, at = Rotary(CPU, rotary_dim=64), torch.arange(5)
+    q = torch.zeros(5, 8, 64, dtype=torch.bfloat16)
+    for kw in (dict(rotary=rot), dict(positions=at), dict(query=q),
+               dict(rotary=rot, query=q), dict(positions=at, query=q)):
+        with pytest.raises(ValueError, match="go together"):
+            MemSession.write_kv(None, 0, q, q, at, 5, **kw)
