@@ -43,8 +43,8 @@
 //
 // Code size counts: hot and cold paths together are about what the instruction
 // caches hold, so loops stay rolled and paths shared where a unit's time does
-// not hang on it (158 KB -> 128 KB: fresh prompts 222 -> 206 us, one token 13.4
-// -> 12.9, 64-wide heads 103 -> 93).
+// not hang on it (158 KB -> 124 KB: fresh prompts 222 -> 203 us, one token 13.4
+// -> 12.8, 64-wide heads 103 -> 90).
 //
 // Slots behind a request's last token, or before all windows of an item's
 // rows, may hold anything: K's scores there are replaced before the maximum,
@@ -474,12 +474,14 @@ AMASS_DEV void ch_plan(const ChunkArgs& a, ChPlan* out) {
       u -= h * cost;
       int lo = 0;                        // last item that starts at or before
       if (q.nt > 1) {
+        long long base = 0;
         int hi = q.nt;
         while (hi - lo > 1) {
           const int m = (lo + hi) >> 1;
-          if (ch_cost(a, q, m) <= u) lo = m; else hi = m;
+          const long long c = ch_cost(a, q, m);
+          if (c <= u) { lo = m; base = c; } else hi = m;
         }
-        u -= ch_cost(a, q, lo);
+        u -= base;
       }
       out->q = q;
       out->r = r;
@@ -749,16 +751,17 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
   tc_after();
   const uint32_t tmem = tmem_s;
 
-  // bounded wait: after about a second the CTA records the fault and unwinds
+  // bounded wait: after about a second the warp unwinds, the others run into
+  // their own limits, and the fault is recorded at the end
   // (mbar_wait in fewer instructions: there are some thirty of these)
   const auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint32_t t0 = clock();
-    do {
-      if (mbar_try_wait(bar, parity)) return true;
-    } while ((uint32_t)clock() - t0 < kWaitCycles);
-    *a.fault = 1;
-    return false;
+    uint32_t t0 = 0;
+    while (!mbar_try_wait(bar, parity)) {
+      const uint32_t now = clock() | 1u;
+      if (!t0) t0 = now;
+      if (now - t0 >= kWaitCycles) return false;
+    }
+    return true;
   };
   // the same for whole warps, which have to unwind together
   const auto wait_warp = [&](uint32_t bar, uint32_t parity) -> bool {
@@ -1365,7 +1368,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       }
       // every MMA and its arrivals end before the CTA does
       commit(drain);
-      (void)wait_warp(drain, 0);
+      ok = wait_warp(drain, 0) && ok;
     } else if (warp == 10) {
       // ------------------------------------------------------------- walk
       if (lane == 0) {
@@ -1374,7 +1377,8 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
         for (int k = 0;; ++k) {
           ChSeg s = {};
           const bool more = wk.next(a, plan, s);
-          if (!wait(seg_empty + 8 * (k % kSegs), ((k / kSegs) & 1) ^ 1)) break;
+          ok = wait(seg_empty + 8 * (k % kSegs), ((k / kSegs) & 1) ^ 1);
+          if (!ok) break;
           segs[k % kSegs] = s;
           mbar_arrive(seg_full + 8 * (k % kSegs));
           if (!more) break;
@@ -1383,6 +1387,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       __syncwarp();
     }
   }
+  if (!ok) *a.fault = 1;
   tc_before();
   __syncthreads();
   if (warp == 9) {
