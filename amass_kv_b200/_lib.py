@@ -164,7 +164,7 @@ def launch(index: int, name: str, *args) -> None:
     if index < 0:
         raise ValueError(f"{name}: the tensors must be on a GPU")
     fn = getattr(_lib or load(), name)
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):

@@ -123,63 +123,65 @@ class Rotary:
 _NONE = (0, 0, 0, 0)                     # pointer, token / head stride, heads
 
 
-def _rows(rot, name, t, dtype, T, d):
+def _rows(index, name, t, dtype, T, d):
     """(address, token stride, head stride, heads) of (>= T, heads, d)."""
     shape, s = t.shape, t.stride()
     if len(shape) != 3 or shape[0] < T or shape[2] != d or s[2] != 1 or \
-            t.dtype != dtype or t.get_device() != rot.index:
+            t.dtype is not dtype or t.get_device() != index:
         raise ValueError(f"{name} must be (>= {T} tokens, heads, {d}) {dtype} "
-                         f"on GPU {rot.index} with a contiguous head_dim, got "
+                         f"on GPU {index} with a contiguous head_dim, got "
                          f"{tuple(shape)} {t.dtype} on {t.device}")
     return t.data_ptr(), s[0], s[1], shape[1]
 
 
-def _vector(rot, name, t, T, dtypes):
-    if t.dtype not in dtypes or t.get_device() != rot.index or \
-            t.dim() != 1 or t.shape[0] < T or not t.is_contiguous():
+def _vector(index, name, t, T, dtypes):
+    """(address, its place in dtypes) of a vector of >= T tokens."""
+    dtype = t.dtype
+    if dtype not in dtypes or t.get_device() != index or t.dim() != 1 or \
+            t.numel() < T or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous vector of at least "
                          f"{T} tokens, {' or '.join(map(str, dtypes))}, on "
-                         f"GPU {rot.index}")
-    return t.data_ptr()
+                         f"GPU {index}")
+    return t.data_ptr(), dtypes.index(dtype)
 
 
-_INDEX = (torch.int64, torch.int32)
+_SLOTS, _INDEX = (torch.int64,), (torch.int32, torch.int64)
 
 
 def _launch(rot, x, q, q_out, k, v, k_dst, kd, v_dst, vd, slots, nb, page,
             positions, T):
-    dtype, d = x.dtype, x.shape[-1]
-    if dtype not in DTYPES:
+    dtype, shape, index, r = x.dtype, x.shape, rot.index, rot.rotary_dim
+    type_id = DTYPES.get(dtype)
+    if type_id is None:
         raise ValueError(f"q, k and v must be bf16 or fp16, got {dtype}")
-    if x.dim() != 3 or not 0 <= T <= x.shape[0]:
-        raise ValueError(f"n_tokens {T} outside the tokens of "
-                         f"{tuple(x.shape)}")
-    if rot.rotary_dim > d or d > 256 or d % 2:
-        raise ValueError(f"no kernel for head_dim {d} with rotary_dim "
-                         f"{rot.rotary_dim}")
+    if len(shape) != 3 or not 0 <= T <= shape[0]:
+        raise ValueError(f"n_tokens {T} outside the tokens of {tuple(shape)}")
+    d = shape[2]
+    if r > d or d > 256 or d % 2:
+        raise ValueError(f"no kernel for head_dim {d} with rotary_dim {r}")
     qp, q_st, q_sh, H = o = _NONE if q is None else \
-        _rows(rot, "q", q, dtype, T, d)
+        _rows(index, "q", q, dtype, T, d)
     if q_out is not q:
-        o = _rows(rot, "q_out", q_out, dtype, T, d)
-    if o[3] != H:
+        o = _rows(index, "q_out", q_out, dtype, T, d)
+    op, o_st, o_sh, o_h = o
+    if o_h != H:
         raise ValueError("q_out must have q's heads")
-    if (q is not None and 0 in o[1:3]) or (v is not None and 0 in vd) or \
+    if (op and not (o_st and o_sh)) or (v is not None and 0 in vd) or \
             (k is not None and 0 in (kd if slots else kd[::2])):
         raise ValueError("q_out, k_out and the caches must not be expanded")
     kp, k_st, k_sh, n_kv = _NONE if k is None else \
-        _rows(rot, "k", k, dtype, T, d)
+        _rows(index, "k", k, dtype, T, d)
     vp, v_st, v_sh, nv = _NONE if v is None else \
-        _rows(rot, "v", v, dtype, T, d)
+        _rows(index, "v", v, dtype, T, d)
     if v is not None and nv != n_kv:
         raise ValueError("v must have k's heads")
-    pos = _vector(rot, "positions", positions, T, _INDEX)
+    pos, pos64 = _vector(index, "positions", positions, T, _INDEX)
     if T == 0:
         return
-    _lib.launch(rot.index, "amass_rotary_write", _lib.ROTARY.pack(
-        qp, o[0], kp, vp, k_dst, v_dst, slots, pos, rot.freq.data_ptr(), q_st,
-        q_sh, o[1], o[2], k_st, k_sh, v_st, v_sh, *kd, *vd, rot.mscale, nb, page,
-        positions.dtype == torch.int64, LAYOUTS[rot.layout], rot.rotary_dim,
-        T, H, n_kv, d, DTYPES[dtype], 0))
+    _lib.launch(index, "amass_rotary_write", _lib.ROTARY.pack(
+        qp, op, kp, vp, k_dst, v_dst, slots, pos, rot.freq.data_ptr(), q_st,
+        q_sh, o_st, o_sh, k_st, k_sh, v_st, v_sh, *kd, *vd, rot.mscale, nb,
+        page, pos64, LAYOUTS[rot.layout], r, T, H, n_kv, d, type_id, 0))
 
 
 def rotary_embed(rot, q, k, positions, *, q_out=None, k_out=None,
@@ -196,7 +198,7 @@ def rotary_embed(rot, q, k, positions, *, q_out=None, k_out=None,
     kd, dst = (0, 0, 0), 0
     if k is not None:
         k_out = k if k_out is None else k_out
-        dst, st, sh, heads = _rows(rot, "k_out", k_out, x.dtype, T,
+        dst, st, sh, heads = _rows(rot.index, "k_out", k_out, x.dtype, T,
                                    x.shape[-1])
         if heads != k.shape[1]:
             raise ValueError("k_out must have k's heads")
@@ -220,14 +222,16 @@ def rotary_write_kv(rot, q, k, v, positions, kv_cache, slot_mapping, *,
     nb, page, n_kv, d, st, kc, vc = cache_layout(kv_cache)
     if (v is None) != (not vc):
         raise ValueError("v and the cache's V half go together")
-    if kv_cache.dtype != k.dtype or kv_cache.get_device() != rot.index or \
-            k.shape[1:] != (n_kv, d):
-        raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not fit the "
+    shape = k.shape
+    if kv_cache.dtype is not k.dtype or kv_cache.get_device() != rot.index or \
+            len(shape) != 3 or shape[1] != n_kv or shape[2] != d:
+        raise ValueError(f"k {tuple(shape)} {k.dtype} does not fit the "
                          f"cache {tuple(kv_cache.shape)} {kv_cache.dtype}")
     if q is None and q_out is not None:
         raise ValueError("q_out without q")
-    T = k.shape[0] if n_tokens is None else int(n_tokens)
-    slots = _vector(rot, "slot_mapping", slot_mapping, T, _INDEX[:1])
+    T = shape[0] if n_tokens is None else int(n_tokens)
+    slots, _ = _vector(rot.index, "slot_mapping", slot_mapping, T,
+                       _SLOTS)
     _launch(rot, k, q, q if q_out is None else q_out, k, v, kc, st, vc,
             st if vc else (0, 0, 0), slots, nb, page, positions, T)
 
@@ -252,7 +256,8 @@ def rotary_write_pools(rot, q, k, v, positions, k_pool, v_pool, slot_mapping,
                              f"{name} {tuple(t.shape)} {t.dtype}")
         strides[i] = t.stride()[:3]
     T = k.shape[0] if n_tokens is None else int(n_tokens)
-    slots = _vector(rot, "slot_mapping", slot_mapping, T, _INDEX[:1])
+    slots, _ = _vector(rot.index, "slot_mapping", slot_mapping, T,
+                       _SLOTS)
     _launch(rot, k, q, q if q_out is None else q_out, k, v,
             k_pool.data_ptr(), strides[0],
             0 if v_pool is None else v_pool.data_ptr(), strides[1], slots,
