@@ -818,10 +818,8 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       const int khi4 = __shfl_sync(~0u, khi, lane >> 2);
       const int klo4 = __shfl_sync(~0u, klo, lane >> 2);
       const bool valid4 = __shfl_sync(~0u, (int)valid, lane >> 2) != 0;
-      // what the warp's rows see all of, and any of
+      // what all of the warp's rows see
       const int khi_lo = __reduce_min_sync(~0u, khi);
-      const int khi_hi = __reduce_max_sync(~0u, valid ? khi : 0);
-      const int klo_lo = __reduce_min_sync(~0u, valid ? klo : 0x7fffffff);
       const int klo_hi = __reduce_max_sync(~0u, klo);
       const int by = two ? 1 : 2;
       const auto rescale = [&](float f) {        // row lane of O by f
@@ -920,86 +918,57 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
           };
           const int k0 = (sg.t0 + j) * kKeys;
           if (k0 + kKeys > khi_lo || k0 < klo_hi) {
-            // some row does not see all of the tile: 32 keys at a time, those
-            // no row of the warp sees left out
-            const auto hidden = [&](int k) {
-              return k >= khi_hi || k + 32 <= klo_lo;
-            };
-            const auto load = [&](uint32_t* s, int c) {
-              const int k = k0 + c, e = khi - k, b = klo - k;
+            // some row does not see all of the tile: -inf in place of what it
+            // does not see, 32 keys at a time (a path of its own that leaves
+            // hidden keys out: fresh prompts 198 us, so 191)
+#pragma unroll 1
+            for (int c = 0; c < kKeys; c += 32) {
+              const int k = k0 + c;
+              if (k + 32 <= khi_lo && k >= klo_hi) continue;
+              uint32_t s[32];
               tc_ld32(s, ts + c);
               tc_wait_ld();
-              if (k + 32 <= khi_lo && k >= klo_hi) return;
+              const int e = khi - k, b = klo - k;
 #pragma unroll
               for (int i = 0; i < 32; ++i)
                 if (i >= e || i < b) s[i] = 0xff800000u;
-            };
-            float mx = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < kKeys; c += 32) {
-              if (hidden(k0 + c)) continue;
-              uint32_t s[32];
-              load(s, c);
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                mx = fmax_nan(mx, __uint_as_float(s[i]));
+              tc_st32(ts + c, s);
             }
-            const float nm = grow(mx);
-            const uint64_t nm2 = f2(nm, nm);
-            // a chunk's weights take the columns of scores already read
-#pragma unroll 1
-            for (int c = 0; c < kKeys; c += 32) {
-              uint32_t s[32];
-              if (hidden(k0 + c)) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = 0;
-              } else {
-                load(s, c);
-#pragma unroll
-                for (int i = 0; i < 32; i += 2)
-                  s[i >> 1] = weigh(s[i], s[i + 1], nm2, i >> 1);
-              }
-              tc_st16(ts + c / 2, s);
-            }
-            tc_wait_st();
-            tc_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_part + 8 * t);
-          } else {
-            uint32_t s[128];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tc_ld32(s + 32 * c, ts + 32 * c);
-            tc_wait_ld();
-            float x4[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) x4[c] = __uint_as_float(s[c]);
-#pragma unroll
-            for (int c = 4; c < 124; c += 8)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                x4[e] = fmax_nan(fmax_nan(x4[e], __uint_as_float(s[c + e])),
-                                 __uint_as_float(s[c + 4 + e]));
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              x4[c] = fmax_nan(x4[c], __uint_as_float(s[124 + c]));
-            const float nm = grow(fmax_nan(fmax_nan(x4[0], x4[1]),
-                                           fmax_nan(x4[2], x4[3])));
-            const uint64_t nm2 = f2(nm, nm);
-#pragma unroll
-            for (int c = 0; c < 128; c += 2) {
-              s[c >> 1] = weigh(s[c], s[c + 1], nm2, c >> 1);
-              if (c + 2 == kPart) {              // the MMA may start
-                tc_st32(ts, s);
-                tc_st16(ts + 32, s + 32);
-                tc_wait_st();
-                tc_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_part + 8 * t);
-              }
-            }
-            tc_st16(ts + kPart / 2, s + kPart / 2);
             tc_wait_st();
           }
+          uint32_t s[128];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tc_ld32(s + 32 * c, ts + 32 * c);
+          tc_wait_ld();
+          float x4[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) x4[c] = __uint_as_float(s[c]);
+#pragma unroll
+          for (int c = 4; c < 124; c += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              x4[e] = fmax_nan(fmax_nan(x4[e], __uint_as_float(s[c + e])),
+                               __uint_as_float(s[c + 4 + e]));
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            x4[c] = fmax_nan(x4[c], __uint_as_float(s[124 + c]));
+          const float nm = grow(fmax_nan(fmax_nan(x4[0], x4[1]),
+                                         fmax_nan(x4[2], x4[3])));
+          const uint64_t nm2 = f2(nm, nm);
+#pragma unroll
+          for (int c = 0; c < 128; c += 2) {
+            s[c >> 1] = weigh(s[c], s[c + 1], nm2, c >> 1);
+            if (c + 2 == kPart) {              // the MMA may start
+              tc_st32(ts, s);
+              tc_st16(ts + 32, s + 32);
+              tc_wait_st();
+              tc_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(p_part + 8 * t);
+            }
+          }
+          tc_st16(ts + kPart / 2, s + kPart / 2);
+          tc_wait_st();
           float a0, a1;
           f2_get(f2_add(sum[0], sum[1]), a0, a1);
           l += a0 + a1;
