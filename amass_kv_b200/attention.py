@@ -119,14 +119,16 @@ sparse_paged_decode_batched = sparse_paged_decode_batched_cuda
 DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
 
-def check_i32(index: int, name: str, t, dim: int) -> None:
-    """An int32 tensor of ``dim`` dimensions on GPU ``index`` (-1: the host)
-    with a contiguous last one."""
-    if t.dtype != torch.int32 or t.get_device() != index or t.dim() != dim \
-            or (t.stride()[-1] != 1 and t.shape[-1] > 1):
+def check_i32(index: int, name: str, t, dim: int):
+    """The shape of an int32 tensor of ``dim`` dimensions on GPU ``index``
+    (-1: the host) with a contiguous last one."""
+    shape = t.shape
+    if t.dtype is not torch.int32 or t.get_device() != index or \
+            len(shape) != dim or (t.stride()[-1] != 1 and shape[-1] > 1):
         raise ValueError(f"{name} must be int32, of {dim} dimensions, on GPU "
                          f"{index} and contiguous in the last dimension; got "
-                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+                         f"{t.dtype} {tuple(shape)} on {t.device}")
+    return shape
 
 
 def cache_layout(kv_cache):
@@ -201,8 +203,8 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
     that see it, and may for other rows of the same request.  Block ids
     outside the cache read as zeros.  One launch, no allocation, no
     synchronisation."""
-    nb, page, n_kv, d, (k_sb, k_st, k_sh), k, v = cache_layout(kv_cache)
-    v_sb, v_st, v_sh = k_sb, k_st, k_sh
+    nb, page, n_kv, d, strides, k, v = cache_layout(kv_cache)
+    k_sb, k_st, k_sh = v_sb, v_st, v_sh = strides
     dtype, dev = q.dtype, buf.index
     if vsource is not None:
         vt = vsource.args()[0]
@@ -211,12 +213,15 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
             raise ValueError(f"the V source's {tuple(vt.shape)} {vt.dtype} "
                              "does not match K")
         v, (v_sb, v_st, v_sh, _) = vt.data_ptr(), vt.stride()
+        strides += (v_sb, v_st, v_sh)
     if not v:
         raise ValueError("no V source")
     shape = q.shape
     if len(shape) != 3 or out.shape != shape:
         raise ValueError("q and out must be (T, H, d) of the same shape")
-    if dtype not in DTYPES or kv_cache.dtype != dtype or out.dtype != dtype:
+    type_id = DTYPES.get(dtype)
+    if type_id is None or kv_cache.dtype is not dtype or \
+            out.dtype is not dtype:
         raise ValueError("q, kv_cache and out must all be bf16 or all fp16")
     T, H, dq = shape
     if dq != d or H != n_kv * buf.G or d != buf.d or n_kv != buf.n_kv:
@@ -231,11 +236,14 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
             kv_cache.get_device() != dev:
         raise ValueError(f"q, kv_cache and out must be on GPU {dev}")
     qp, op = q.data_ptr(), out.data_ptr()
-    if (qp | op | k | v) % 16 or \
-            (T > 1 and (q_st <= 0 or q_st % 8 or o_st <= 0 or o_st % 8)) or \
-            (H > 1 and (q_sh <= 0 or q_sh % 8 or o_sh <= 0 or o_sh % 8)) or \
-            (k_sb | k_st | k_sh | v_sb | v_st | v_sh) % 8 or \
-            min(k_sb, k_st, k_sh, v_sb, v_st, v_sh) <= 0:
+    if T > 1:
+        strides += (q_st, o_st)
+    if H > 1:
+        strides += (q_sh, o_sh)
+    every = 0
+    for s in strides:
+        every |= s if s > 0 else 1
+    if (qp | op | k | v) & 15 or every & 7:
         raise ValueError("q, kv_cache and out must be 16-byte aligned, with "
                          "strides that are positive multiples of 8 elements")
     if n_kv > 1 and nb > 1 and (
@@ -243,12 +251,10 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
             k_sb < n_kv * k_sh):
         raise ValueError("kv_cache needs block strides that are multiples of "
                          "the head strides, the same for K and V")
-    check_i32(dev, "block_table", block_table, 2)
-    check_i32(dev, "seq_lens", seq_lens, 1)
-    check_i32(dev, "query_start_loc", query_start_loc, 1)
-    n_req = seq_lens.shape[0]
-    rows, max_pages = block_table.shape
-    if rows < n_req or query_start_loc.shape[0] < n_req + 1 or max_pages < 1:
+    rows, max_pages = check_i32(dev, "block_table", block_table, 2)
+    n_req, = check_i32(dev, "seq_lens", seq_lens, 1)
+    starts, = check_i32(dev, "query_start_loc", query_start_loc, 1)
+    if rows < n_req or starts <= n_req or max_pages < 1:
         raise ValueError(f"block_table {(rows, max_pages)} and "
                          f"query_start_loc {tuple(query_start_loc.shape)} do "
                          f"not cover {n_req} requests")
@@ -270,5 +276,5 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
         query_start_loc.data_ptr(), *buf.scratch, op,
         0 if lse is None else lse.data_ptr(), q_st, q_sh, k_sb, k_st, k_sh,
         v_sb, v_st, v_sh, block_table.stride(0), o_st, o_sh, scale, nb,
-        buf.n_ctas, min(window or 0, 0x7fffffff), T, n_req, n_kv, buf.G, d,
-        page, max_pages, DTYPES[dtype]))
+        buf.n_ctas, min(window, 0x7fffffff) if window else 0, T, n_req, n_kv,
+        buf.G, d, page, max_pages, type_id))

@@ -83,8 +83,7 @@ class BlockPool(_lib.FixedBuffers):
         self._fixed = True
 
     def _rows(self, t, name: str) -> int:
-        check_i32(self._index, name, t, 1)
-        n = t.shape[0]
+        n, = check_i32(self._index, name, t, 1)
         if n > self.R:
             raise ValueError(f"{name} has {n} rows, the pool {self.R}")
         return n
@@ -137,12 +136,10 @@ def build_slot_map(block_table, seq_lens, query_start_loc, positions,
     its ``seq_lens[r]``.  Slot -1 for a position without a block (< 0, beyond
     the table's row, block < 0); tokens of no request get 0 and -1."""
     dev = block_table.get_device()
-    check_i32(dev, "block_table", block_table, 2)
-    check_i32(dev, "seq_lens", seq_lens, 1)
-    check_i32(dev, "query_start_loc", query_start_loc, 1)
-    n = seq_lens.shape[0]
-    rows, max_pages = block_table.shape
-    if rows < n or max_pages < 1 or query_start_loc.shape[0] < n + 1:
+    rows, max_pages = check_i32(dev, "block_table", block_table, 2)
+    n, = check_i32(dev, "seq_lens", seq_lens, 1)
+    starts, = check_i32(dev, "query_start_loc", query_start_loc, 1)
+    if rows < n or max_pages < 1 or starts <= n:
         raise ValueError(f"block_table {(rows, max_pages)} and "
                          f"query_start_loc {tuple(query_start_loc.shape)} do "
                          f"not cover {n} requests")
