@@ -158,3 +158,38 @@ def test_mem_session_turns_keys(dev, offload_k):
     assert torch.equal(a.v_pool, b.v_pool)
     if offload_k:
         assert torch.equal(a.k_pool, b.k_pool)
+
+
+def test_blocks_past_32_bit_offsets(dev):
+    """A cache of 4.6e9 elements: its last blocks are written and read where
+    they are."""
+    NB, n_kv, G, d = 140000, 8, 4, 128
+    if torch.cuda.mem_get_info(dev)[0] < 20 << 30:
+        pytest.skip("needs 10 GB")
+    kv = torch.empty((NB, 2, PAGE, n_kv, d), dtype=torch.bfloat16, device=dev)
+    lens, T = [(40, 40), (1, 1)], 41
+    bt = torch.tensor([[NB - 1, 0, NB - 3], [NB - 2, -1, -1]],
+                      dtype=torch.int32, device=dev)
+    kv[[0, NB - 3, NB - 2, NB - 1]] = float("nan")
+    sl = torch.tensor([40, 1], dtype=torch.int32, device=dev)
+    qsl = torch.tensor([0, 40, 41], dtype=torch.int32, device=dev)
+    pos = torch.empty(T, dtype=torch.int64, device=dev)
+    slot = torch.empty_like(pos)
+    build_slot_map(bt, sl, qsl, pos, slot)
+    assert int(slot.max()) == (NB - 1) * PAGE + PAGE - 1
+    gen = torch.Generator(device=dev).manual_seed(3)
+    q, k, v = (torch.randn((T, h, d), generator=gen, device=dev)
+               .to(torch.bfloat16) for h in (n_kv * G, n_kv, n_kv))
+    rot = Rotary(dev, rotary_dim=d)
+    kr = k.clone()
+    rotary_embed(rot, None, kr, pos)
+    rotary_write_kv(rot, q, k, v, pos, kv, slot)
+    assert torch.equal(kv[slot // PAGE, 0, slot % PAGE], kr)
+    assert torch.equal(kv[slot // PAGE, 1, slot % PAGE], v)
+    out = torch.empty_like(q)
+    buf = A.ChunkBuffers(dev, n_kv=n_kv, G=G, head_dim=d)
+    A.paged_chunk_attention(q, kv, bt, sl, qsl, out, buf)
+    buf.check()
+    ref, tol, _, _, _ = chunk_reference(q, kv[:, 0], kv[:, 1], bt, lens,
+                                        [0, 40, 41], d ** -0.5)
+    assert bool(((out.double() - ref).abs() <= tol).all())
