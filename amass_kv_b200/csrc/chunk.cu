@@ -43,8 +43,8 @@
 //
 // Code size counts: hot and cold paths together are about what the instruction
 // caches hold, so loops stay rolled and paths shared where a unit's time does
-// not hang on it (158 KB -> 124 KB: fresh prompts 222 -> 203 us, one token 13.4
-// -> 12.8, 64-wide heads 103 -> 90).
+// not hang on it (158 KB -> 119 KB, old and new in turn: fresh prompts 206 ->
+// 188 us, with heads of 64 107 -> 91, 2048 behind 64K 2030 -> 2002).
 //
 // Slots behind a request's last token, or before all windows of an item's
 // rows, may hold anything: K's scores there are replaced before the maximum,
@@ -818,9 +818,11 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       const int khi4 = __shfl_sync(~0u, khi, lane >> 2);
       const int klo4 = __shfl_sync(~0u, klo, lane >> 2);
       const bool valid4 = __shfl_sync(~0u, (int)valid, lane >> 2) != 0;
-      // what all of the warp's rows see
+      // what all of the warp's rows see, and any of
       const int khi_lo = __reduce_min_sync(~0u, khi);
       const int klo_hi = __reduce_max_sync(~0u, klo);
+      const int khi_hi = __reduce_max_sync(~0u, valid ? khi : 0);
+      const int klo_lo = __reduce_min_sync(~0u, valid ? klo : 0x7fffffff);
       const int by = two ? 1 : 2;
       const auto rescale = [&](float f) {        // row lane of O by f
 #pragma unroll 1
@@ -920,18 +922,23 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
           if (k0 + kKeys > khi_lo || k0 < klo_hi) {
             // some row does not see all of the tile: -inf in place of what it
             // does not see, 32 keys at a time (a path of its own that leaves
-            // hidden keys out: fresh prompts 198 us, so 191)
+            // hidden keys out: 8 prompts of 200-600 tokens 18.3 us, so 19.0,
+            // but 333-2047 tokens 203 us, so 199, and less code)
 #pragma unroll 1
             for (int c = 0; c < kKeys; c += 32) {
               const int k = k0 + c;
               if (k + 32 <= khi_lo && k >= klo_hi) continue;
               uint32_t s[32];
-              tc_ld32(s, ts + c);
-              tc_wait_ld();
-              const int e = khi - k, b = klo - k;
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (i >= e || i < b) s[i] = 0xff800000u;
+              for (int i = 0; i < 32; ++i) s[i] = 0xff800000u;
+              if (k < khi_hi && k + 32 > klo_lo) {
+                tc_ld32(s, ts + c);
+                tc_wait_ld();
+                const int e = khi - k, b = klo - k;
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (i >= e || i < b) s[i] = 0xff800000u;
+              }
               tc_st32(ts + c, s);
             }
             tc_wait_st();
