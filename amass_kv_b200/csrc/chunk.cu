@@ -341,6 +341,7 @@ struct alignas(16) ChSeg {
   int first, last, cta0, parts;          // a cut item's CTAs
 };
 struct ChPlan {
+  long long u;                           // the run's start in the head's items
   ChReq q;
   int r, h, i, from, to, share;          // run [from, to) from item i's start
 };
@@ -472,28 +473,44 @@ AMASS_DEV void ch_plan(const ChunkArgs& a, ChPlan* out) {
       const int h = all >> 31 || a.n_kv >> 20 ? (int)(u / cost)
                                               : quotient((int)u, (int)cost);
       u -= h * cost;
-      int lo = 0;                        // last item that starts at or before
-      if (q.nt > 1) {
-        long long base = 0;
-        int hi = q.nt;
-        while (hi - lo > 1) {
-          const int m = (lo + hi) >> 1;
-          const long long c = ch_cost(a, q, m);
-          if (c <= u) { lo = m; base = c; } else hi = m;
-        }
-        u -= base;
-      }
       out->q = q;
       out->r = r;
       out->h = h;
-      out->i = lo;
-      out->from = (int)u;
-      out->to = (int)(u + end - begin);
+      out->u = u;                        // for ch_plan_item
+      out->to = (int)(end - begin);
       out->share = (int)share;
       break;
     }
   }
   __syncthreads();
+}
+
+// Ends the plan: the last item of the head that starts at or before the run's
+// start, by a whole warp, 32 places at a time (halving by one thread took 2500
+// cycles of a run's start).
+AMASS_DEV void ch_plan_item(const ChunkArgs& a, ChPlan* p) {
+  const int lane = threadIdx.x & 31;
+  const ChReq q = p->q;
+  const long long u = p->u;
+  long long base = 0;
+  int lo = 0, hi = p->to > 0 ? q.nt : 0;
+#pragma unroll 1
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, m = lo + (lane + 1) * step;
+    const long long c = m < hi ? ch_cost(a, q, m) : 0;
+    const int n = __popc(__ballot_sync(~0u, m < hi && c <= u));
+    const long long b = __shfl_sync(~0u, c, max(n - 1, 0));
+    if (n) base = b;
+    lo += n * step;
+    hi = min(hi, lo + step);
+  }
+  __syncwarp();
+  if (lane == 0) {
+    p->i = lo;
+    p->from = (int)(u - base);
+    if (p->to > 0) p->to += p->from;
+  }
+  __syncwarp();
 }
 
 constexpr int kSegs = 4;
@@ -1347,6 +1364,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
       ok = wait_warp(drain, 0) && ok;
     } else if (warp == 10) {
       // ------------------------------------------------------------- walk
+      ch_plan_item(a, &plan);
       if (lane == 0) {
         ChWalk wk;
         wk.start(a, plan);

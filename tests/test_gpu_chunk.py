@@ -259,6 +259,15 @@ def test_batch_of_many(dev):
     check(make(dev, lens, n_kv=1, G=4, d=64), dev)
 
 
+@pytest.mark.parametrize("window", [None, 70])
+def test_many_items_of_a_request(dev, window):
+    """Runs that start deep inside a request: more items than a warp has
+    lanes, with one item a CTA and with several."""
+    for G, new, more in ((8, 2600, 0), (8, 1100, 900), (1, 9000, 0)):
+        c = make(dev, [(new, new + more), (40, 60)], n_kv=1, G=G, d=64)
+        check(c, dev, window=window)
+
+
 def test_long_context_few_rows(dev):
     """One item over all SMs: its partials come from every CTA."""
     check(make(dev, [(2, 40000)], n_kv=1, G=8), dev)
