@@ -36,8 +36,8 @@
 //
 // Measured on a B200, bf16, 32 query / 8 kv heads of 128: 2048 tokens behind
 // 64K 1745 us (1276 TFLOP/s; 2010 us back to back, at the power limit), one
-// token over 4K 12.3 us with the call; 64 / 8 heads, six fresh prompts of
-// 333-2047 tokens 211 us.  What bounds it: the chain scores ->
+// token over 4K 12.4 us with the call; 64 / 8 heads, six fresh prompts of
+// 333-2047 tokens 209 us.  What bounds it: the chain scores ->
 // softmax -> product (3300 cycles a key tile of two row tiles, of which the
 // tensor core is busy 2048), then the board's power.
 //
