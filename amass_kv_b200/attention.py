@@ -192,7 +192,8 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
     request r's ``seq_lens[r]``; a row at position p sees the keys
     max(0, p - window + 1) .. p (``window=None``: from 0).  Rows without a
     key (or with nothing but scores of -inf) become 0, rows outside every
-    request are left as they are.  ``lse`` (T, H) fp32, contiguous, receives
+    request are left as they are; a request's tokens from the T-th row of the
+    step on count as not there.  ``lse`` (T, H) fp32, contiguous, receives
     the rows' natural log-sum-exp (-inf without a key).
     ``n_req = seq_lens.shape[0]``; ``buf`` is a ``ChunkBuffers``; ``out`` may
     be ``q``.

@@ -277,8 +277,11 @@ AMASS_DEV ChReq ch_req(const ChunkArgs& a, int r) {
   const int s0 = a.qsl[r], s1 = a.qsl[r + 1];
   q.q0 = max(s0, 0);
   q.ql = max(min(s1, a.T) - q.q0, 0);
-  // a length beyond the block table's row is cut: no page behind it exists
-  q.sl = max((int)min((int64_t)a.sl[r], (int64_t)a.max_pages * kPg), 0);
+  // a length beyond the block table's row is cut: no page behind it exists;
+  // new tokens behind the last row are not there: the others keep their
+  // positions
+  const int64_t most = min((int64_t)a.sl[r], (int64_t)a.max_pages * kPg);
+  q.sl = (int)max(most - (max(s1, a.T) - a.T), (int64_t)0);
   q.off = q.sl - q.ql;
   q.nt = (q.ql + (2 << a.tm_log2) - 1) >> (a.tm_log2 + 1);
   return q;

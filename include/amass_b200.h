@@ -664,15 +664,17 @@ typedef struct AmassChunk {
  * lse (n_tokens, n_kv * G) fp32 or null: natural log of the row's sum of
  * exp(scale q.k), -inf without a key.  Cache slots behind a request's last
  * token, or before the windows of all its rows, may hold anything; block ids
- * outside [0, num_blocks) read as zeros; seq_lens is cut at max_pages * page.  n_ctas is the GPU's SM count.  Of
- * the scratch (acc_part, ml_part, tickets) only the tickets need to be 0
- * before the first call, and are left 0; calls that overlap on the GPU need
- * scratch of their own.  fault[0] becomes 1 when a CTA gave up a bounded wait:
- * its rows are then incomplete and the scratch has to be replaced.  head_dim
- * in {64, 128}, G <= 8, page = 16, n_req <= 4096, scale > 0; bases 16-byte
- * aligned, strides positive multiples of 8 elements, block strides multiples
- * of the head strides, with the same quotient for K and V.  One launch; the
- * first call on a device sets a kernel attribute. */
+ * outside [0, num_blocks) read as zeros; seq_lens is cut at max_pages * page;
+ * tokens of a request behind row n_tokens - 1 count as not there (q_len and
+ * seq_lens without them: its other rows keep their positions).  n_ctas is the
+ * GPU's SM count.  Of the scratch (acc_part, ml_part, tickets) only the tickets
+ * need to be 0 before the first call, and are left 0; calls that overlap on the
+ * GPU need scratch of their own.  fault[0] becomes 1 when a CTA gave up a
+ * bounded wait: its rows are then incomplete and the scratch has to be
+ * replaced.  head_dim in {64, 128}, G <= 8, page = 16, n_req <= 4096, scale >
+ * 0; bases 16-byte aligned, strides positive multiples of 8 elements, block
+ * strides multiples of the head strides, with the same quotient for K and V.
+ * One launch; the first call on a device sets a kernel attribute. */
 int amass_paged_chunk(const AmassChunk* args, void* stream);
 
 #ifdef __cplusplus
