@@ -109,6 +109,7 @@ _SIGS = {
     "amass_slot_map": [_P, _L, _P, _P, _I, _P, _P, _I, _I, _I, _P],
     "amass_rotary_write": [_P, _P],
     "amass_paged_chunk": [_P, _P],
+    "amass_paged_chunk_granted": [_P, _P, _P],
 }
 
 _lib = None

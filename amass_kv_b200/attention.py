@@ -183,7 +183,7 @@ class ChunkBuffers(_lib.FixedBuffers):
 
 def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
                           out, buf, *, scale=None, window=None, lse=None,
-                          vsource=None) -> None:
+                          vsource=None, status=None) -> None:
     """Dense attention of the step's new tokens over the paged cache, which
     already holds their keys and values.
 
@@ -196,7 +196,10 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
     step on count as not there.  ``lse`` (T, H) fp32, contiguous, receives
     the rows' natural log-sum-exp (-inf without a key).
     ``n_req = seq_lens.shape[0]``; ``buf`` is a ``ChunkBuffers``; ``out`` may
-    be ``q``.
+    be ``q``.  ``status``: a ``BlockPool``'s, when its step may have been
+    refused in part -- a refused request's length is without its new tokens,
+    which without it would be taken for the request's last old ones; with it
+    they become 0 (lse -inf).
 
     Cache slots behind a request's last token, or before the windows of all
     its rows, may hold anything.  Between the two, a NaN or infinite key makes
@@ -266,16 +269,25 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
                             tuple(lse.shape) != (T, H) or
                             not lse.is_contiguous()):
         raise ValueError(f"lse must be a contiguous fp32 ({T}, {H}) tensor")
+    if status is not None and \
+            check_i32(dev, "status", status, 1)[0] < n_req:
+        raise ValueError(f"status {tuple(status.shape)} does not cover "
+                         f"{n_req} requests")
     if scale is None:
         scale = d ** -0.5
     if not 0 < scale < float("inf"):
         raise ValueError(f"scale must be positive, got {scale}")
     if T == 0 or n_req == 0:
         return
-    _lib.launch(dev, "amass_paged_chunk", _lib.CHUNK.pack(
+    args = _lib.CHUNK.pack(
         qp, k, v, block_table.data_ptr(), seq_lens.data_ptr(),
         query_start_loc.data_ptr(), *buf.scratch, op,
         0 if lse is None else lse.data_ptr(), q_st, q_sh, k_sb, k_st, k_sh,
         v_sb, v_st, v_sh, block_table.stride(0), o_st, o_sh, scale, nb,
         buf.n_ctas, min(window, 0x7fffffff) if window else 0, T, n_req, n_kv,
-        buf.G, d, page, max_pages, type_id))
+        buf.G, d, page, max_pages, type_id)
+    if status is None:
+        _lib.launch(dev, "amass_paged_chunk", args)
+    else:
+        _lib.launch(dev, "amass_paged_chunk_granted", args,
+                    status.data_ptr())

@@ -73,6 +73,7 @@ struct ChunkArgs {
   int64_t bt_stride;
   const int32_t* sl;
   const int32_t* qsl;
+  const int32_t* status;                 // null or 0: the request has a step
   void* out;
   int64_t o_st, o_sh;
   float* lse;                            // (T, H) or null
@@ -282,6 +283,8 @@ AMASS_DEV ChReq ch_req(const ChunkArgs& a, int r) {
   // positions
   const int64_t most = min((int64_t)a.sl[r], (int64_t)a.max_pages * kPg);
   q.sl = (int)max(most - (max(s1, a.T) - a.T), (int64_t)0);
+  // a refused request's length is without its new tokens: no key is theirs
+  if (a.status && a.status[r] != 0) q.sl = 0;
   q.off = q.sl - q.ql;
   q.nt = (q.ql + (2 << a.tm_log2) - 1) >> (a.tm_log2 + 1);
   return q;
@@ -1466,7 +1469,8 @@ int chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk,
 }  // namespace
 }  // namespace amass
 
-extern "C" int amass_paged_chunk(const AmassChunk* args, void* stream) {
+extern "C" int amass_paged_chunk_granted(const AmassChunk* args,
+                                         const int32_t* status, void* stream) {
   using namespace amass;
   if (!args) return AMASS_ERR_ARG;
   const AmassChunk& x = *args;
@@ -1523,7 +1527,7 @@ extern "C" int amass_paged_chunk(const AmassChunk* args, void* stream) {
 
   ChunkArgs a = {};
   a.bt = x.block_table; a.bt_stride = x.bt_stride; a.sl = x.seq_lens;
-  a.qsl = x.query_start_loc; a.out = x.out; a.o_st = x.o_st; a.o_sh = x.o_sh;
+  a.qsl = x.query_start_loc; a.status = status; a.out = x.out; a.o_st = x.o_st; a.o_sh = x.o_sh;
   a.lse = x.lse; a.acc = x.acc_part;
   a.ml = reinterpret_cast<float2*>(x.ml_part);
   a.tickets = x.tickets; a.fault = x.fault;
@@ -1549,4 +1553,8 @@ extern "C" int amass_paged_chunk(const AmassChunk* args, void* stream) {
                : chunk_launch<128, false>(mq, mk, mv, a, ctas, st);
   return f16 ? chunk_launch<64, true>(mq, mk, mv, a, ctas, st)
              : chunk_launch<64, false>(mq, mk, mv, a, ctas, st);
+}
+
+extern "C" int amass_paged_chunk(const AmassChunk* args, void* stream) {
+  return amass_paged_chunk_granted(args, nullptr, stream);
 }

@@ -36,9 +36,11 @@ class BlockPool(_lib.FixedBuffers):
 
     All int32 but the two token maps.  ``status[r]``: 0 granted, 1 too few
     free blocks, 2 longer than ``max_pages`` or past 2^30 tokens in the step;
-    a refused row keeps its pages and length and its new tokens get slot -1.  ``overflow`` latches 1 / 2
-    for such a row and 4 for more new tokens than the step's ``n_tokens``;
-    ``check()`` reads it (synchronises) and raises.
+    a refused row keeps its pages and length and its new tokens get slot -1;
+    hand ``status`` to ``attention.paged_chunk_attention``, which cannot see
+    from the lengths that the row's tokens are not among them.  ``overflow``
+    latches 1 / 2 for such a row and 4 for more new tokens than the step's
+    ``n_tokens``; ``check()`` reads it (synchronises) and raises.
 
     Calls on one pool must run one after the other (one stream, or ordered
     by events)."""

@@ -677,6 +677,13 @@ typedef struct AmassChunk {
  * One launch; the first call on a device sets a kernel attribute. */
 int amass_paged_chunk(const AmassChunk* args, void* stream);
 
+/* paged_chunk of a step that amass_pages_begin may have refused in part:
+ * status (n_req,) is its status (null: none refused).  A refused request's
+ * seq_lens lacks the new tokens that query_start_loc counts, so its rows have
+ * no place in it: they see no key and become 0 (lse -inf). */
+int amass_paged_chunk_granted(const AmassChunk* args, const int32_t* status,
+                              void* stream);
+
 #ifdef __cplusplus
 }
 #endif
