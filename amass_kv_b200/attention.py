@@ -134,16 +134,32 @@ def check_i32(index: int, name: str, t, dim: int):
 def cache_layout(kv_cache):
     """(num_blocks, page, n_kv, d, (block, token, head stride), K address, V
     address or 0) of the cache layouts of ``split_kv``, without making views;
-    ValueError when it is none of them."""
+    ValueError when it is none of them.
+
+    A first dimension of 2 is K and V apart, as ``split_kv`` takes it: a cache
+    of two blocks of both halves cannot be told from it and has to come as
+    (2, 2, ...) with K first.  (2, 1, ...) could be two blocks of keys only or
+    one block of both, and is refused."""
     shape, s = kv_cache.shape, kv_cache.stride()
-    if len(shape) != 5 or (s[4] != 1 and shape[4] > 1):
+    if len(shape) != 5 or (s[4] != 1 and shape[4] > 1) or \
+            (shape[0] != 2 and not 1 <= shape[1] <= 2):
         raise ValueError("kv_cache must be (blocks, 1 or 2, page, n_kv, d) or "
                          "(2, blocks, page, n_kv, d) with a contiguous "
                          f"head_dim, got {tuple(shape)}")
+    n0, n1, page, n_kv, d = shape
+    s0, s1, st, sh, _ = s
+    if not (n0 and n1 and page and n_kv and d):
+        raise ValueError(f"kv_cache {tuple(shape)} is empty")
     p = kv_cache.data_ptr()
-    b, half = (1, 0) if shape[0] == 2 else (0, 1)
-    v = 0 if shape[half] == 1 else p + s[half] * kv_cache.element_size()
-    return (shape[b], shape[2], shape[3], shape[4], (s[b], s[2], s[3]), p, v)
+    if n0 != 2:
+        v = 0 if n1 == 1 else p + s1 * kv_cache.element_size()
+        return n0, page, n_kv, d, (s0, st, sh), p, v
+    if n1 == 1:
+        raise ValueError(f"kv_cache {tuple(shape)} may be two blocks of keys "
+                         "or one block of keys and values: give it another "
+                         "block")
+    return (n1, page, n_kv, d, (s1, st, sh), p,
+            p + s0 * kv_cache.element_size())
 
 
 class ChunkBuffers(_lib.FixedBuffers):
