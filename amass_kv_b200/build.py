@@ -29,6 +29,7 @@ def sources():
 def build(verbose: bool = False, ptxas_v: bool = False, force: bool = False):
     srcs = sources()
     hdrs = glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(
+        os.path.join(CSRC, "*.h")) + glob.glob(
         os.path.join(os.path.dirname(HERE), "include", "*.h"))
     if (not force and os.path.exists(LIB) and os.path.getmtime(LIB) >=
             max(os.path.getmtime(p) for p in srcs + hdrs)):

@@ -1456,12 +1456,8 @@ int chunk_launch(const CUtensorMap& mq, const CUtensorMap& mk,
                  const CUtensorMap& mv, const ChunkArgs& a, int ctas,
                  cudaStream_t st) {
   using X = ChShape<D>;
-  static unsigned long long mask = 0;
-  if (first_on_device(mask) &&
-      cudaFuncSetAttribute(chunk_kernel<D, kF16>,
-                           cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           X::kSmem) != cudaSuccess)
-    return AMASS_ERR_CUDA;
+  static DeviceOnce once;
+  if (!allow_smem(once, chunk_kernel<D, kF16>, X::kSmem)) return AMASS_ERR_CUDA;
   return launch_pdl(chunk_kernel<D, kF16>, dim3(ctas), dim3(kChThreads),
                     X::kSmem, st, mq, mk, mv, a);
 }

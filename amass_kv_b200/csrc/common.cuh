@@ -13,6 +13,7 @@
 #include <stdint.h>
 
 #include "../../include/amass_b200.h"
+#include "once.h"
 
 #define AMASS_DEV __device__ __forceinline__
 
@@ -50,15 +51,17 @@ inline int launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block,
              : AMASS_ERR_CUDA;
 }
 
-// Kernel attributes are per device: true the first time this is called for
-// the current device with this mask (one bit per device id).
-inline bool first_on_device(unsigned long long& mask) {
+// Kernel attributes are per device: allows the kernel `bytes` of dynamic shared
+// memory on the current one, once for each `once` (one per kernel).
+template <typename K>
+inline bool allow_smem(DeviceOnce& once, K kernel, size_t bytes) {
   int dev = 0;
-  cudaGetDevice(&dev);
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (mask & bit) return false;
-  mask |= bit;
-  return true;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  return once.run(dev, [&] {
+    return cudaFuncSetAttribute(kernel,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)bytes) == cudaSuccess;
+  });
 }
 
 inline int num_sms() {

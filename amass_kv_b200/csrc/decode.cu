@@ -655,11 +655,8 @@ int launch_decode(const DecArgs& a, cudaStream_t st) {
   const size_t smem = decode_smem<D, NST>(a.units);
   if (smem > 220 * 1024) return AMASS_ERR_UNSUPPORTED;
   auto kern = decode_kernel<D, NST, TIER>;
-  static unsigned long long configured = 0;
-  if (first_on_device(configured)) {
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         220 * 1024);
-  }
+  static DeviceOnce configured;
+  if (!allow_smem(configured, kern, 220 * 1024)) return AMASS_ERR_CUDA;
   int per_sm = 0;
   cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kDecThreads, smem);
   if (per_sm < 1) per_sm = 1;

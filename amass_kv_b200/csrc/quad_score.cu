@@ -1538,9 +1538,8 @@ int launch_r8_k(const QuadArgs& a, cudaStream_t st) {
   constexpr size_t vst = Item<D, R, VB>::V_PRE ? 0 : VStage<D, R, VB>::BYTES;
   const size_t smem = (size_t)kQuadWarps * (2 * (16 * 16 * RC + 16 * 16 * 2) + vst);
   static int ps = 0;
-  static unsigned long long attr = 0;
-  if (first_on_device(attr))
-    cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static DeviceOnce attr;
+  if (!allow_smem(attr, k, smem)) return AMASS_ERR_CUDA;
   if (ps == 0) {
     cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ps, k, kQuadWarps * 32, smem);
     if (ps < 1) ps = 1;
@@ -1605,10 +1604,10 @@ int launch_quad_pipe(const QuadArgs& a, bool write_h, bool qin,
     if (qin) k = write_h ? AMASS_PIPE_K(true, true) : AMASS_PIPE_K(false, true);
     else k = write_h ? AMASS_PIPE_K(true, false) : AMASS_PIPE_K(false, false);
 #undef AMASS_PIPE_K
-    static unsigned long long attr_set[8] = {};
-    if (first_on_device(attr_set[(write_h ? 1 : 0) + (qin ? 2 : 0) + 4 * pk]))
-      cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           110 * 1024);
+    static DeviceOnce attr_set[8];
+    if (!allow_smem(attr_set[(write_h ? 1 : 0) + (qin ? 2 : 0) + 4 * pk], k,
+                    110 * 1024))
+      return AMASS_ERR_CUDA;
     QuadArgs b = a;
     if (!qin) {
       const int heads = a.n_req * a.n_kv * a.G;

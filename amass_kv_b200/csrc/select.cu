@@ -99,15 +99,14 @@ template <bool FOLD, bool LIN, bool COV>
 int launch_select(const SelArgs& a, int units, cudaStream_t st) {
   const bool g4 = FOLD && a.G <= 4;
   const int cl = COV ? 1 : select_cluster_size(units, a.MP);
-  static unsigned long long configured[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  static DeviceOnce configured[8];
   if (cl > 1) {
     auto k = g4 ? select_kernel<FOLD, LIN, COV, 4, true>
                 : select_kernel<FOLD, LIN, COV, 8, true>;
     const int chunk = ((a.MP + cl - 1) / cl + 3) & ~3;
     const size_t smem = (size_t)chunk * sizeof(float);
-    if (first_on_device(configured[2 + (g4 ? 1 : 0)]))
-      cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           kMaxSmem);
+    if (!allow_smem(configured[2 + (g4 ? 1 : 0)], k, kMaxSmem))
+      return AMASS_ERR_CUDA;
     if (int rc = launch_cluster_pdl(k, dim3(units * cl), dim3(kSelThreads),
                                     smem, st, cl, a))
       return rc;
@@ -132,10 +131,8 @@ int launch_select(const SelArgs& a, int units, cudaStream_t st) {
     k = g4 ? select_kernel<FOLD, LIN, COV, 4> : select_kernel<FOLD, LIN, COV, 8>;
     ci = 0;
   }
-  if (first_on_device(configured[ci + (g4 ? 1 : 0)])) {
-    cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         kMaxSmem);
-  }
+  if (!allow_smem(configured[ci + (g4 ? 1 : 0)], k, kMaxSmem))
+    return AMASS_ERR_CUDA;
   if (int rc = launch_pdl(k, dim3(units), dim3(nt), smem, st, a)) return rc;
   return launch_status();
 }
@@ -190,11 +187,9 @@ extern "C" int amass_nrm_combine(const float* score_h, int64_t sh_stride,
   a.G = G;
   a.MP = max_pages;
   const size_t smem = (size_t)max_pages * sizeof(float);
-  static unsigned long long configured = 0;
-  if (first_on_device(configured)) {
-    cudaFuncSetAttribute(nrm_combine_kernel,
-                         cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
-  }
+  static DeviceOnce configured;
+  if (!allow_smem(configured, nrm_combine_kernel, kMaxSmem))
+    return AMASS_ERR_CUDA;
   if (int rc = launch_pdl(nrm_combine_kernel, dim3(n_req * n_kv),
                           dim3(kSelThreads), smem,
                           static_cast<cudaStream_t>(stream), a))

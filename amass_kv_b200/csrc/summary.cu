@@ -402,14 +402,9 @@ extern "C" int amass_summarize_pages(
   const int grid = (int)std::min<long long>((items + kSumWarps - 1) / kSumWarps,
                                             (long long)num_sms() * 8);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  static unsigned long long conf = 0;  // both variants, once per device
-  if (first_on_device(conf)) {
-    cudaFuncSetAttribute(summary_kernel<128>,
-                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    cudaFuncSetAttribute(summary_kernel<64>,
-                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  }
+  static DeviceOnce conf[2];
   auto kern = head_dim == 128 ? summary_kernel<128> : summary_kernel<64>;
+  if (!allow_smem(conf[head_dim == 128], kern, smem)) return AMASS_ERR_CUDA;
   if (int rc = launch_pdl(kern, dim3(grid), dim3(kSumWarps * 32), smem, st, a))
     return rc;
   return launch_status();

@@ -588,12 +588,9 @@ extern "C" int amass_tier_plan(const int32_t* page_table,
                             a))
       return rc;
   }
-  static unsigned long long configured = 0;
-  if (first_on_device(configured)) {
-    cudaFuncSetAttribute(tier_plan_kernel,
-                         cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         (int)kPlanSmem);
-  }
+  static DeviceOnce configured;
+  if (!allow_smem(configured, tier_plan_kernel, kPlanSmem))
+    return AMASS_ERR_CUDA;
   if (int rc = launch_pdl(tier_plan_kernel, dim3(n_kv), dim3(kPlanThreads),
                           smem, st, a))
     return rc;
