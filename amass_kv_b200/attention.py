@@ -218,9 +218,10 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
     they become 0 (lse -inf).
 
     Cache slots behind a request's last token, or before the windows of all
-    its rows, may hold anything.  Between the two, a NaN or infinite key makes
-    the rows that see it NaN; a NaN or infinite value does so for the rows
-    that see it, and may for other rows of the same request.  Block ids
+    its rows, may hold anything.  Between the two, a score of NaN or
+    +inf (a NaN or infinite key) makes its row NaN, one of -inf drops the key
+    from its row; a NaN or infinite value reaches the rows that see it, and
+    may make other rows of the same request NaN.  Block ids
     outside the cache read as zeros.  One launch, no allocation, no
     synchronisation."""
     nb, page, n_kv, d, strides, k, v = cache_layout(kv_cache)

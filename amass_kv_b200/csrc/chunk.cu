@@ -926,7 +926,8 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
               m = mn;
               rescale(f);
             }
-            // an infinite or NaN score makes the row NaN, as the formula does
+            // a score of +inf or NaN makes the row NaN, as the formula does;
+            // one of -inf has no weight
             return m == -INFINITY ? 0.f : fmaf(0.f, m, -m * sl2);
           };
           uint64_t sum[2] = {0ull, 0ull};
