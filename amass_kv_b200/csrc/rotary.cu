@@ -6,10 +6,11 @@
 //
 // Angle: fp32 cannot hold position * f (at position 1e5 the product has two
 // or three digits left of the turn), and a table of every position costs
-// memory and a second read.  f / (2 pi) is held as a 64-bit binary fraction
-// of a turn; the 64-bit product with the position wraps to exactly the
-// fraction that matters (error position * 2^-65 turns, any position), whose
-// upper 32 bits go to sincospi in fp32: about 2^-24 of the result.
+// memory and a second read.  f / (2 pi) is held as the nearest 64-bit binary
+// fraction of a turn; the 64-bit product with the position wraps to the
+// fraction that matters, off by at most |position| * 2^-65 turns.  Its upper
+// 32 bits go to sincospi in fp32, which rounds them to 24: cos and sin are
+// within 2^-22 (absolute) at positions up to 2^37, twice that at 2^40.
 //
 // Bound: HBM.  q, k and v are read once and written once, (2H + 4 n_kv) d
 // 16-bit values a token; the angles are formed once a token for all heads.

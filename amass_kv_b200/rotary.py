@@ -13,6 +13,7 @@ token), so there is no cos / sin table and no largest position.
 """
 from __future__ import annotations
 
+import decimal
 import math
 
 import torch
@@ -21,6 +22,11 @@ from . import _lib
 from .attention import DTYPES, cache_layout
 
 LAYOUTS = {"half": 0, "interleaved": 1}
+# frequencies are formed in 60 digits: fp64 ones would leave an angle off by
+# some 2^-55 turns a token, the 64-bit fractions can hold 2^-65
+_LONG = decimal.Context(prec=60)
+_TAU = decimal.Decimal("6.283185307179586476925286766559005768394338798750"
+                       "21164194988918461563")
 
 
 def rotary_frequencies(rotary_dim: int, base: float, scaling=None):
@@ -35,9 +41,22 @@ def rotary_frequencies(rotary_dim: int, base: float, scaling=None):
               and beta_slow times within original_max_position; cos and sin
               times 0.1 ln(s) + 1 (or ``mscale``)
     """
-    r = rotary_dim
-    f = torch.tensor([float(base) ** (-2.0 * i / r) for i in range(r // 2)],
-                     dtype=torch.float64)
+    with decimal.localcontext(_LONG):
+        f, m = _frequencies(rotary_dim, base, scaling)
+    return torch.tensor([float(x) for x in f], dtype=torch.float64), m
+
+
+def _frequencies(r, base, scaling):
+    """``rotary_frequencies`` as decimals, in the caller's context."""
+    D = decimal.Decimal
+
+    def powers(b):
+        return [b ** (D(-2 * i) / r) for i in range(r // 2)]
+
+    def blend(f, s, keep):                   # f where keep is 1, f / s where 0
+        return [x / s * (1 - k) + x * k for x, k in
+                ((x, min(max(k, D(0)), D(1))) for x, k in zip(f, keep))]
+    f = powers(D(base))
     if scaling is None:
         return f, 1.0
     sc = dict(scaling)
@@ -57,14 +76,13 @@ def rotary_frequencies(rotary_dim: int, base: float, scaling=None):
     s = float(sc["factor"])
     if not 1.0 <= s < float("inf"):
         raise ValueError(f"scaling factor must be at least 1, got {s}")
+    long_s = D(s)
     if kind == "linear":
-        return f / s, 1.0
+        return [x / long_s for x in f], 1.0
     if kind == "ntk":
         if r <= 2:
             raise ValueError("ntk scaling needs rotary_dim > 2")
-        b = float(base) * s ** (r / (r - 2.0))
-        return torch.tensor([b ** (-2.0 * i / r) for i in range(r // 2)],
-                            dtype=torch.float64), 1.0
+        return powers(D(base) * long_s ** (D(r) / (r - 2))), 1.0
     orig = float(sc["original_max_position"])
     if orig <= 0:
         raise ValueError("original_max_position must be positive")
@@ -73,8 +91,8 @@ def rotary_frequencies(rotary_dim: int, base: float, scaling=None):
         if not 0 < lo < hi:
             raise ValueError("llama3 scaling needs 0 < low_freq_factor < "
                              "high_freq_factor")
-        keep = ((orig * f / (2 * math.pi) - lo) / (hi - lo)).clamp(0.0, 1.0)
-        return f / s * (1 - keep) + f * keep, 1.0
+        return blend(f, long_s, [(D(orig) * x / _TAU - D(lo)) /
+                                 (D(hi) - D(lo)) for x in f]), 1.0
     fast = float(sc.get("beta_fast", 32.0))
     slow = float(sc.get("beta_slow", 1.0))
     if not 0 < slow < fast:
@@ -85,11 +103,10 @@ def rotary_frequencies(rotary_dim: int, base: float, scaling=None):
             (2 * math.log(float(base)))
     lo = max(math.floor(dim_of(fast)), 0)
     hi = min(math.ceil(dim_of(slow)), r - 1)
-    ramp = ((torch.arange(r // 2, dtype=torch.float64) - lo)
-            / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
     m = sc.get("mscale")
     m = 0.1 * math.log(s) + 1.0 if m is None else float(m)
-    return f / s * ramp + f * (1 - ramp), m
+    return blend(f, long_s, [1 - D(i - lo) / max(D(hi - lo), D("0.001"))
+                             for i in range(r // 2)]), m
 
 
 class Rotary:
@@ -112,11 +129,14 @@ class Rotary:
         dev = _lib.device_of(device)
         self.index = -1 if dev.index is None else dev.index
         self.device, self.rotary_dim, self.layout = dev, rotary_dim, layout
-        self.inv_freq, self.mscale = rotary_frequencies(rotary_dim, base,
-                                                        scaling)
-        # turns per token as 64-bit binary fractions (f <= 1 rad < 1/6 turn)
-        turns = [round(x / (2 * math.pi) * 2.0 ** 64)
-                 for x in self.inv_freq.tolist()]
+        with decimal.localcontext(_LONG):
+            f, self.mscale = _frequencies(rotary_dim, base, scaling)
+            # turns per token as 64-bit binary fractions (f <= 1 rad < 1/6
+            # turn)
+            turns = [int((x / _TAU * 2 ** 64).to_integral_value())
+                     for x in f]
+        self.inv_freq = torch.tensor([float(x) for x in f],
+                                     dtype=torch.float64)
         self.freq = torch.tensor(turns, dtype=torch.int64, device=dev)
 
 

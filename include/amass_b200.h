@@ -627,9 +627,10 @@ typedef struct AmassRotary {
  * slot / page, row slot % page, slot = slot_mapping[t]; slots outside
  * [0, num_blocks * page) are skipped.  slot_mapping null: slot = t (page 1: a
  * token-major destination, which may be k itself).  freq[i] = f_i / (2 pi) as
- * a 64-bit binary fraction of a turn (the product with the position wraps, so
- * no position is too far).  Products in fp32, one rounding.  head_dim <= 256
- * and rotary_dim <= head_dim, both even.  Two tokens must not share a slot. */
+ * the nearest 64-bit binary fraction of a turn (the product with the position
+ * wraps: off by at most |position| * 2^-65 turns; then cos and sin in fp32).
+ * Products in fp32, one rounding.  head_dim <= 256 and rotary_dim <= head_dim,
+ * both even.  Two tokens must not share a slot. */
 int amass_rotary_write(const AmassRotary* args, void* stream);
 
 /* Arguments of amass_paged_chunk; strides in elements. */
