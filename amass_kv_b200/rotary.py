@@ -39,7 +39,7 @@ def rotary_frequencies(rotary_dim: int, base: float, scaling=None):
               low_freq_factor, f above high_freq_factor, linear in between
       yarn    by dimension, ramp between the dimensions that turn beta_fast
               and beta_slow times within original_max_position; cos and sin
-              times 0.1 ln(s) + 1 (or ``mscale``)
+              times ``attention_factor`` (default 0.1 ln(s) + 1)
     """
     with decimal.localcontext(_LONG):
         f, m = _frequencies(rotary_dim, base, scaling)
@@ -68,7 +68,12 @@ def _frequencies(r, base, scaling):
     if kind not in needs:
         raise ValueError(f"scaling type must be one of {sorted(needs)}, got "
                          f"{kind!r}")
-    optional = {"yarn": ("beta_fast", "beta_slow", "mscale")}.get(kind, ())
+    optional = {"yarn": ("beta_fast", "beta_slow",
+                         "attention_factor")}.get(kind, ())
+    if kind == "yarn" and ("mscale" in sc or "mscale_all_dim" in sc):
+        raise ValueError("mscale and mscale_all_dim are arguments of a formula "
+                         "for the factor on cos and sin: give that factor as "
+                         "attention_factor")
     missing = [k for k in needs[kind] if k not in sc]
     extra = [k for k in sc if k not in needs[kind] + optional]
     if missing or extra:
@@ -103,8 +108,10 @@ def _frequencies(r, base, scaling):
             (2 * math.log(float(base)))
     lo = max(math.floor(dim_of(fast)), 0)
     hi = min(math.ceil(dim_of(slow)), r - 1)
-    m = sc.get("mscale")
+    m = sc.get("attention_factor")
     m = 0.1 * math.log(s) + 1.0 if m is None else float(m)
+    if not 0 < m < float("inf"):
+        raise ValueError(f"attention_factor must be positive, got {m}")
     return blend(f, long_s, [1 - D(i - lo) / max(D(hi - lo), D("0.001"))
                              for i in range(r // 2)]), m
 
