@@ -22,11 +22,12 @@ from . import _lib
 from .attention import DTYPES, cache_layout
 
 LAYOUTS = {"half": 0, "interleaved": 1}
-# frequencies are formed in 60 digits: fp64 ones would leave an angle off by
-# some 2^-55 turns a token, the 64-bit fractions can hold 2^-65
-_LONG = decimal.Context(prec=60)
-_TAU = decimal.Decimal("6.283185307179586476925286766559005768394338798750"
-                       "21164194988918461563")
+# frequencies are formed as integers of 2^-256 from one power in 42 digits: fp64
+# ones would leave an angle off by some 2^-55 turns a token, the 64-bit
+# fractions can hold 2^-65
+_LONG = decimal.Context(prec=42)
+_ONE = 1 << 256
+_TAU = 6283185307179586476925286766559005768394338798750 * _ONE // 10 ** 48
 
 
 def rotary_frequencies(rotary_dim: int, base: float, scaling=None):
@@ -41,24 +42,30 @@ def rotary_frequencies(rotary_dim: int, base: float, scaling=None):
               and beta_slow times within original_max_position; cos and sin
               times ``attention_factor`` (default 0.1 ln(s) + 1)
     """
-    with decimal.localcontext(_LONG):
-        f, m = _frequencies(rotary_dim, base, scaling)
-    return torch.tensor([float(x) for x in f], dtype=torch.float64), m
+    f, m = _frequencies(rotary_dim, base, scaling)
+    return torch.tensor([x / _ONE for x in f], dtype=torch.float64), m
+
+
+def _fixed(x: float) -> int:
+    n, d = x.as_integer_ratio()
+    return n * _ONE // d
+
+
+def _powers(r, log_base):
+    """exp(-2 i log_base / r) in units of 2^-256, i < r / 2."""
+    n, d = _LONG.exp(_LONG.multiply(log_base, _LONG.divide(
+        decimal.Decimal(-2), decimal.Decimal(r)))).as_integer_ratio()
+    q, f = n * _ONE // d, [_ONE]
+    for _ in range(r // 2 - 1):
+        f.append(f[-1] * q >> 256)
+    return f
 
 
 def _frequencies(r, base, scaling):
-    """``rotary_frequencies`` as decimals, in the caller's context."""
-    D = decimal.Decimal
-
-    def powers(b):
-        return [b ** (D(-2 * i) / r) for i in range(r // 2)]
-
-    def blend(f, s, keep):                   # f where keep is 1, f / s where 0
-        return [x / s * (1 - k) + x * k for x, k in
-                ((x, min(max(k, D(0)), D(1))) for x, k in zip(f, keep))]
-    f = powers(D(base))
+    """``rotary_frequencies`` in units of 2^-256."""
+    log_base = _LONG.ln(decimal.Decimal(base))
     if scaling is None:
-        return f, 1.0
+        return _powers(r, log_base), 1.0
     sc = dict(scaling)
     kind = sc.pop("type", None)
     needs = {"linear": ("factor",), "ntk": ("factor",),
@@ -81,23 +88,30 @@ def _frequencies(r, base, scaling):
     s = float(sc["factor"])
     if not 1.0 <= s < float("inf"):
         raise ValueError(f"scaling factor must be at least 1, got {s}")
-    long_s = D(s)
-    if kind == "linear":
-        return [x / long_s for x in f], 1.0
     if kind == "ntk":
         if r <= 2:
             raise ValueError("ntk scaling needs rotary_dim > 2")
-        return powers(D(base) * long_s ** (D(r) / (r - 2))), 1.0
+        return _powers(r, _LONG.add(log_base, _LONG.multiply(
+            _LONG.ln(decimal.Decimal(s)), _LONG.divide(
+                decimal.Decimal(r), decimal.Decimal(r - 2))))), 1.0
+    f = _powers(r, log_base)
+    num, den = s.as_integer_ratio()
+    if kind == "linear":
+        return [x * den // num for x in f], 1.0
+
+    def blend(keep):                         # f where keep is 1, f / s where 0
+        return [(x * den // num * (_ONE - k) + x * k) >> 256 for x, k in
+                ((x, min(max(k, 0), _ONE)) for x, k in zip(f, keep))]
     orig = float(sc["original_max_position"])
-    if orig <= 0:
+    if not 0 < orig < float("inf"):
         raise ValueError("original_max_position must be positive")
     if kind == "llama3":
         lo, hi = float(sc["low_freq_factor"]), float(sc["high_freq_factor"])
-        if not 0 < lo < hi:
+        if not 0 < lo < hi < float("inf"):
             raise ValueError("llama3 scaling needs 0 < low_freq_factor < "
                              "high_freq_factor")
-        return blend(f, long_s, [(D(orig) * x / _TAU - D(lo)) /
-                                 (D(hi) - D(lo)) for x in f]), 1.0
+        o, low, width = _fixed(orig), _fixed(lo), _fixed(hi) - _fixed(lo)
+        return blend([(o * x // _TAU - low) * _ONE // width for x in f]), 1.0
     fast = float(sc.get("beta_fast", 32.0))
     slow = float(sc.get("beta_slow", 1.0))
     if not 0 < slow < fast:
@@ -112,8 +126,9 @@ def _frequencies(r, base, scaling):
     m = 0.1 * math.log(s) + 1.0 if m is None else float(m)
     if not 0 < m < float("inf"):
         raise ValueError(f"attention_factor must be positive, got {m}")
-    return blend(f, long_s, [1 - D(i - lo) / max(D(hi - lo), D("0.001"))
-                             for i in range(r // 2)]), m
+    width = max(_fixed(float(hi - lo)), _ONE // 1000)
+    return blend([_ONE - (i - lo) * _ONE * _ONE // width
+                  for i in range(r // 2)]), m
 
 
 class Rotary:
@@ -136,14 +151,11 @@ class Rotary:
         dev = _lib.device_of(device)
         self.index = -1 if dev.index is None else dev.index
         self.device, self.rotary_dim, self.layout = dev, rotary_dim, layout
-        with decimal.localcontext(_LONG):
-            f, self.mscale = _frequencies(rotary_dim, base, scaling)
-            # turns per token as 64-bit binary fractions (f <= 1 rad < 1/6
-            # turn)
-            turns = [int((x / _TAU * 2 ** 64).to_integral_value())
-                     for x in f]
-        self.inv_freq = torch.tensor([float(x) for x in f],
+        f, self.mscale = _frequencies(rotary_dim, base, scaling)
+        self.inv_freq = torch.tensor([x / _ONE for x in f],
                                      dtype=torch.float64)
+        # turns per token as 64-bit binary fractions (f <= 1 rad < 1/6 turn)
+        turns = [((x << 65) + _TAU) // (2 * _TAU) for x in f]
         self.freq = torch.tensor(turns, dtype=torch.int64, device=dev)
 
 
