@@ -212,18 +212,18 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start_loc,
     step on count as not there.  ``lse`` (T, H) fp32, contiguous, receives
     the rows' natural log-sum-exp (-inf without a key).
     ``n_req = seq_lens.shape[0]``; ``buf`` is a ``ChunkBuffers``; ``out`` may
-    be ``q``.  ``status``: a ``BlockPool``'s, when its step may have been
-    refused in part -- a refused request's length is without its new tokens,
-    which without it would be taken for the request's last old ones; with it
-    they become 0 (lse -inf).
+    be ``q``.
+
+    ``status``: that of a ``BlockPool`` whose step may have been refused in
+    part.  A refused request's length is without its new tokens, so they would
+    be taken for its last old ones; with ``status`` they become 0 (lse -inf).
 
     Cache slots behind a request's last token, or before the windows of all
-    its rows, may hold anything.  Between the two, a score of NaN or
-    +inf (a NaN or infinite key) makes its row NaN, one of -inf drops the key
-    from its row; a NaN or infinite value reaches the rows that see it, and
-    may make other rows of the same request NaN.  Block ids
-    outside the cache read as zeros.  One launch, no allocation, no
-    synchronisation."""
+    its rows, may hold anything.  Between the two, a score of NaN or +inf (a
+    NaN or infinite key) makes its row NaN, one of -inf drops the key from its
+    row; a NaN or infinite value reaches the rows that see it, and may make
+    other rows of the same request NaN.  Block ids outside the cache read as
+    zeros.  One launch, no allocation, no synchronisation."""
     nb, page, n_kv, d, strides, k, v = cache_layout(kv_cache)
     k_sb, k_st, k_sh = v_sb, v_st, v_sh = strides
     dtype, dev = q.dtype, buf.index

@@ -21,9 +21,11 @@
 //   warp 10         walks the run and tells the others its pieces
 //
 // While one row tile's softmax runs, the tensor core works for the other.
-// O is rescaled only when a row's maximum grows by more than 2^8 (p stays
-// below 256, exact in the 16-bit P's range); sums stay in fp32 registers; the
-// one rounding to 16 bits before the end is P's (half a step per weight).
+// O is rescaled only when a row's maximum grows by more than 2^8, so weights
+// stay below 256, which both 16-bit types hold; sums stay in fp32 registers.
+// The one rounding to 16 bits before the end is P's, half a step per weight:
+// the tensor core takes P in V's type.  The row sum keeps the unrounded
+// weights, so the result is about 1.4 times as far off as one rounded once.
 //
 // Work split: the (item, key tile) units of the whole batch form one flat
 // list; every CTA takes an equal run of it.  Lengths live on the device, so
@@ -34,17 +36,17 @@
 // request's cache) and a large prefill (no tail of uneven causal tiles) with
 // one rule.
 //
-// Measured on a B200, bf16, 32 query / 8 kv heads of 128: 2048 tokens behind
-// 64K 1745 us (1276 TFLOP/s; 2010 us back to back, at the power limit), one
-// token over 4K 12.4 us with the call; 64 / 8 heads, six fresh prompts of
-// 333-2047 tokens 209 us.  What bounds it: the chain scores ->
-// softmax -> product (3300 cycles a key tile of two row tiles, of which the
-// tensor core is busy 2048), then the board's power.
+// Measured on a B200, bf16, 32 query / 8 kv heads of 128, back to back (and in
+// runs too short to reach the power limit): 2048 tokens behind 64K 2013 us,
+// 1110 TFLOP/s (1763 us, 1267), one token over 4K 12.4 us with the call; 64 / 8
+// heads, six fresh prompts of 333-2047 tokens 208 us (190).  What bounds it:
+// the chain scores -> softmax -> product (3300 cycles a key tile of two row
+// tiles, of which the tensor core is busy 2048), then the board's power.
 //
 // Code size counts: hot and cold paths together are about what the instruction
 // caches hold, so loops stay rolled and paths shared where a unit's time does
-// not hang on it (158 KB -> 119 KB, old and new in turn: fresh prompts 206 ->
-// 188 us, with heads of 64 107 -> 91, 2048 behind 64K 2030 -> 2002).
+// not hang on it (158 KB -> 119 KB, old and new in turn, short runs: fresh
+// prompts 9 % less time, with heads of 64 15 %, 2048 behind 64K 1 %).
 //
 // Slots behind a request's last token, or before all windows of an item's
 // rows, may hold anything: K's scores there are replaced before the maximum,
@@ -62,7 +64,7 @@ constexpr int kPg = 16;                  // tokens of a page
 constexpr int kChMaxReq = 4096;
 // cost of an item, for equal runs: a key tile of two row tiles (3300 cycles,
 // softmax bound), of one row tile (2100, its loads), and what an item adds
-// (query load, first scores, output)
+// (query load, first scores, output); cycles of heads of 128, used for 64 too
 constexpr int kCost2 = 3, kCost1 = 2, kCostItem = 6, kMinRun = 4;
 constexpr float kRescaleLog2 = 8.f;
 constexpr uint32_t kWaitCycles = 2000000000u;    // a second or so
@@ -946,8 +948,8 @@ chunk_kernel(const __grid_constant__ CUtensorMap mq,
           if (k0 + kKeys > khi_lo || k0 < klo_hi) {
             // some row does not see all of the tile: -inf in place of what it
             // does not see, 32 keys at a time (a path of its own that leaves
-            // hidden keys out: 8 prompts of 200-600 tokens 18.3 us, so 19.0,
-            // but 333-2047 tokens 203 us, so 199, and less code)
+            // hidden keys out takes 4 % less for 8 prompts of 200-600 tokens,
+            // 2 % more for 333-2047, and more code)
 #pragma unroll 1
             for (int c = 0; c < kKeys; c += 32) {
               const int k = k0 + c;

@@ -107,7 +107,8 @@ class BlockPool(_lib.FixedBuffers):
         """Row r loses its last ``drop[r]`` tokens (int32; clipped to what it
         has).  Pages left empty go back to the free stack, last row and last
         page first: dropping all that a ``begin_step`` granted restores the
-        stack's order."""
+        stack's order.  A row that the step refused has none of its tokens:
+        give it 0, or it loses older ones."""
         n = self._rows(drop, "drop")
         _lib.launch(self._index, "amass_pages_trim", self._pool,
                     drop.data_ptr(), n, 0)
