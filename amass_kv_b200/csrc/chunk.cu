@@ -1445,13 +1445,24 @@ int make_map(CUtensorMap* m, bool f16, const void* p, int rank,
     // the stride of a dimension of one element is never used
     if (i) gs[i - 1] = dim[i] == 1 ? 16 : (cuuint64_t)stride[i] * 2;
   }
-  return fn(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-            (cuuint32_t)rank, const_cast<void*>(p), gd, gs, bx, es,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
-             ? AMASS_OK : AMASS_ERR_ARG;
+  const auto encode = [&]() {
+    return fn(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+              (cuuint32_t)rank, const_cast<void*>(p), gd, gs, bx, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult rc = encode();
+  if (rc == CUDA_ERROR_INVALID_CONTEXT || rc == CUDA_ERROR_NOT_INITIALIZED) {
+    // a host thread that has made no CUDA call yet: this one needs the
+    // device's context, which the runtime's calls bind by themselves
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess)
+      return AMASS_ERR_CUDA;
+    rc = encode();
+  }
+  return rc == CUDA_SUCCESS ? AMASS_OK : AMASS_ERR_ARG;
 }
 
 template <int D, bool kF16>
