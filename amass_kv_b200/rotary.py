@@ -63,7 +63,7 @@ def _powers(r, log_base):
 
 def _frequencies(r, base, scaling):
     """``rotary_frequencies`` in units of 2^-256."""
-    log_base = _LONG.ln(decimal.Decimal(base))
+    r, log_base = int(r), _LONG.ln(decimal.Decimal(float(base)))
     if scaling is None:
         return _powers(r, log_base), 1.0
     sc = dict(scaling)

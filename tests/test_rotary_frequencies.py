@@ -4,6 +4,7 @@ import math
 from decimal import Decimal, localcontext
 from fractions import Fraction
 
+import numpy as np
 import pytest
 import torch
 
@@ -77,3 +78,13 @@ def test_turns(r, base, sc):
     g, _ = rotary_frequencies(r, base, sc)
     assert g.dtype == torch.float64
     assert g.tolist() == [float(x) for x in f]
+
+
+def test_numbers_of_other_types():
+    want = Rotary("cpu", rotary_dim=64, base=500000.0,
+                  scaling=dict(type="ntk", factor=4.0))
+    for r, base, s in ((np.int64(64), np.float32(500000), np.int32(4)),
+                       (64, 500000, 4), (64, torch.tensor(5e5), 4.0)):
+        rot = Rotary("cpu", rotary_dim=r, base=base,
+                     scaling=dict(type="ntk", factor=s))
+        assert torch.equal(rot.freq, want.freq)
